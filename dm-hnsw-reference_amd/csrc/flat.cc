@@ -1,0 +1,321 @@
+// C entries of flat scoring (include/shine_gpu.h shine_flat_*): checks, workspaces and launches.  Kernels:
+// flat_kernels.hip.  Nothing is allocated and nothing waits for the GPU here, so every entry can be captured.
+#include "flat.h"
+
+#include <algorithm>
+#include <string>
+
+#include "index_internal.h"
+
+using namespace shine;
+namespace F = shine::flat;
+
+namespace {
+
+constexpr uint32_t kRowBlock = 32768;        // rows of one launch (the grid's second extent ends at 65,535)
+constexpr uint64_t kQuantizeBlock = 1 << 24;  // rows of one quantising launch (threads of a grid are a 32-bit number)
+constexpr uint64_t kAlign = 256;
+
+uint64_t aligned(uint64_t bytes) { return (bytes + kAlign - 1) & ~(kAlign - 1); }
+
+// The call's device, and the caller's again afterwards.
+struct OnDevice {
+  int was = -1;
+  hipError_t e;
+  explicit OnDevice(int gpu) {
+    e = hipGetDevice(&was);
+    if (e == hipSuccess && was != gpu) e = hipSetDevice(gpu);
+    else if (e == hipSuccess) was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
+int fail(const char* what) { return set_error(SHINE_ERR_ARG, what); }
+int hip(const char* what, hipError_t e) {
+  return e == hipSuccess ? SHINE_OK : set_error(SHINE_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+bool float_elem(int e) { return e == F::kF32 || e == F::kF16 || e == F::kBF16; }
+uint64_t elem_size(int e) { return e == F::kF32 ? 4 : 2; }
+bool on(const void* p, uint64_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+const char* check_rows(const void* rows, int elem, uint64_t n, uint64_t width, uint64_t ld) {
+  if (!float_elem(elem)) return "element type must be SHINE_ELEM_F32, _F16 or _BF16";
+  if (n && width && !rows) return "NULL device pointer";
+  if (ld < width && n > 1) return "row stride is shorter than a row";
+  if (!on(rows, elem_size(elem))) return "a pointer is not aligned to its element type";
+  return nullptr;
+}
+
+const char* check_table(const shine_flat_table* t) {
+  if (!t) return "table is NULL";
+  if (t->dim == 0 || t->dim > F::kMaxDim) return "dim must be in [1, 16384]";
+  if (t->n > F::kMaxRecords) return "a table holds at most 2^30 records";
+  if (t->n && (!t->codes || !t->scales)) return "NULL device pointer";
+  if (!on(t->codes, 64) || !on(t->scales, 4) || !on(t->bias, 4)) return "table codes must be 64-byte, scales and bias 4-byte aligned";
+  return nullptr;
+}
+
+const char* check_adjustment(const shine_flat_adjustment* a, uint32_t nq, uint64_t n) {
+  if (a->bias && a->bias_ld && a->bias_ld < n && nq > 1) return "bias row stride is shorter than a row";
+  if (a->allow && a->allow_ld && a->allow_ld < (n + 31) / 32 && nq > 1) return "allow row stride is shorter than a row";
+  if (a->seen_n && !a->seen) return "seen is NULL with seen_n > 0";
+  if (a->seen_n && a->seen_ld < a->seen_n && nq > 1) return "seen row stride is shorter than a row";
+  if (!on(a->bias, 4) || !on(a->allow, 4) || !on(a->seen, 4) || !on(a->repetition, 4) || !on(a->frequency, 4) ||
+      !on(a->presence, 4))
+    return "an adjustment array is not 4-byte aligned";
+  return nullptr;
+}
+
+F::AdjustArgs adjust_args(const shine_flat_adjustment& a, uint32_t row) {
+  F::AdjustArgs r{};
+  r.bias = a.bias ? a.bias + row * a.bias_ld : nullptr;
+  r.bias_ld = a.bias_ld;
+  r.allow = a.allow ? a.allow + row * a.allow_ld : nullptr;
+  r.allow_ld = a.allow_ld;
+  r.seen = a.seen_n ? a.seen + row * a.seen_ld : nullptr;
+  r.seen_ld = a.seen_ld;
+  r.seen_n = a.seen_n;
+  r.repetition = a.repetition ? a.repetition + row : nullptr;
+  r.frequency = a.frequency ? a.frequency + row : nullptr;
+  r.presence = a.presence ? a.presence + row : nullptr;
+  return r;
+}
+
+bool neutral(const shine_flat_adjustment* a) { return !a || (!a->bias && !a->allow && !a->seen_n); }
+
+hipError_t quantize(const void* rows, int elem, uint64_t n, uint32_t dim, uint64_t ld, int8_t* codes, float* scales,
+                    float* half_norms, hipStream_t s) {
+  for (uint64_t at = 0; at < n; at += kQuantizeBlock) {
+    F::QuantizeArgs a{};
+    a.rows = static_cast<const char*>(rows) + at * ld * elem_size(elem);
+    a.n = std::min(kQuantizeBlock, n - at);
+    a.ld = ld;
+    a.dim = dim;
+    a.codes = codes + at * F::code_pitch(dim);
+    a.scales = scales + at;
+    a.half_norms = half_norms ? half_norms + at : nullptr;
+    if (hipError_t e = F::launch_quantize(elem, a, s); e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// search: blocks of rows x chunks of records whose scores fit kChunkScores
+constexpr uint64_t kChunkScores = 1ull << 26;
+struct SearchPlan {
+  uint32_t rows;       // rows of a block
+  uint64_t cols;       // records of a chunk, whole tiles of 4,096
+  uint32_t chunks, slices;
+  uint64_t codes, scales, scores, keys, total;  // offsets into the workspace
+};
+SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k) {
+  SearchPlan p{};
+  p.rows = std::min(std::max(nq, 1u), 2048u);
+  p.cols = std::max<uint64_t>(4096, kChunkScores / p.rows / 4096 * 4096);
+  p.cols = std::min(p.cols, std::max<uint64_t>(1, n));
+  p.chunks = static_cast<uint32_t>((n + p.cols - 1) / p.cols);
+  p.slices = F::topk_slices(p.rows, p.cols);
+  p.codes = 0;
+  p.scales = aligned(static_cast<uint64_t>(p.rows) * F::code_pitch(dim));
+  p.scores = p.scales + aligned(4ull * p.rows);
+  p.keys = p.scores + aligned(4ull * p.rows * p.cols);
+  p.total = p.keys + aligned(8ull * p.rows * p.chunks * p.slices * k);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint32_t shine_flat_pitch(uint32_t dim) { return F::code_pitch(dim); }
+
+int shine_flat_quantize(int gpu_id, const void* d_rows, int elem, uint64_t n, uint32_t dim, uint64_t ld, int8_t* d_codes,
+                        float* d_scales, float* d_half_norms, void* stream) {
+  if (dim == 0 || dim > F::kMaxDim) return fail("dim must be in [1, 16384]");
+  if (const char* w = check_rows(d_rows, elem, n, dim, ld)) return fail(w);
+  if (n == 0) return SHINE_OK;
+  if (!d_codes || !d_scales) return fail("NULL device pointer");
+  if (!on(d_codes, 8) || !on(d_scales, 4) || !on(d_half_norms, 4)) return fail("codes must be 8-byte, scales and norms 4-byte aligned");
+  OnDevice dev(gpu_id);
+  if (dev.e != hipSuccess) return hip("flat quantize: device", dev.e);
+  return hip("flat quantize", quantize(d_rows, elem, n, dim, ld, d_codes, d_scales, d_half_norms, static_cast<hipStream_t>(stream)));
+}
+
+uint64_t shine_flat_scores_workspace(uint32_t nq, uint32_t dim) {
+  const uint64_t rows = std::min(nq, kRowBlock);
+  return aligned(rows * F::code_pitch(dim)) + aligned(4 * rows);
+}
+
+int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
+                      void* d_out, int out_elem, uint64_t out_ld, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  if (const char* w = check_table(table)) return fail(w);
+  if (const char* w = check_rows(d_queries, elem, nq, table->dim, ld)) return fail(w);
+  if (nq == 0 || table->n == 0) return SHINE_OK;
+  if (const char* w = check_rows(d_out, out_elem, nq, table->n, out_ld)) return fail(w);
+  if (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < shine_flat_scores_workspace(nq, table->dim))
+    return fail("workspace is missing, not 256-byte aligned or smaller than shine_flat_scores_workspace");
+  OnDevice dev(gpu_id);
+  if (dev.e != hipSuccess) return hip("flat scores: device", dev.e);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint32_t pitch = F::code_pitch(table->dim);
+  const uint64_t rows = std::min(nq, kRowBlock);
+  int8_t* codes = static_cast<int8_t*>(d_workspace);
+  float* scales = reinterpret_cast<float*>(codes + aligned(rows * pitch));
+  for (uint32_t q = 0; q < nq; q += kRowBlock) {
+    const uint32_t m = std::min(kRowBlock, nq - q);
+    if (hipError_t e = quantize(static_cast<const char*>(d_queries) + q * ld * elem_size(elem), elem, m, table->dim, ld,
+                                codes, scales, nullptr, s); e != hipSuccess)
+      return hip("flat scores", e);
+    F::ScoresArgs a{};
+    a.qcodes = codes;
+    a.qscales = scales;
+    a.codes = table->codes;
+    a.scales = table->scales;
+    a.bias = table->bias;
+    a.nq = m;
+    a.pitch = pitch;
+    a.n = table->n;
+    a.out = static_cast<char*>(d_out) + q * out_ld * elem_size(out_elem);
+    a.ld = out_ld;
+    if (hipError_t e = F::launch_scores(out_elem, a, s); e != hipSuccess) return hip("flat scores", e);
+  }
+  return SHINE_OK;
+}
+
+int shine_flat_adjust(int gpu_id, const void* d_scores, int elem, uint32_t nq, uint64_t n, uint64_t ld,
+                      const shine_flat_adjustment* adjustment, void* d_out, uint64_t out_ld, void* stream) {
+  if (!adjustment) return fail("adjustment is NULL");
+  if (n > F::kMaxRecords) return fail("a row holds at most 2^30 scores");
+  if (const char* w = check_rows(d_scores, elem, nq, n, ld)) return fail(w);
+  if (const char* w = check_adjustment(adjustment, nq, n)) return fail(w);
+  if (nq == 0 || n == 0) return SHINE_OK;
+  if (const char* w = check_rows(d_out, elem, nq, n, out_ld)) return fail(w);
+  OnDevice dev(gpu_id);
+  if (dev.e != hipSuccess) return hip("flat adjust: device", dev.e);
+  for (uint32_t q = 0; q < nq; q += kRowBlock) {
+    F::AdjustArgs a = adjust_args(*adjustment, q);
+    a.scores = static_cast<const char*>(d_scores) + q * ld * elem_size(elem);
+    a.out = static_cast<char*>(d_out) + q * out_ld * elem_size(elem);
+    a.ld = ld;
+    a.out_ld = out_ld;
+    a.nq = std::min(kRowBlock, nq - q);
+    a.n = n;
+    if (hipError_t e = F::launch_adjust(elem, a, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip("flat adjust", e);
+  }
+  return SHINE_OK;
+}
+
+uint64_t shine_flat_topk_workspace(uint32_t nq, uint64_t n, uint32_t k) {
+  const uint32_t rows = std::min(std::max(nq, 1u), kRowBlock), slices = F::topk_slices(rows, n);
+  return slices > 1 ? aligned(8ull * rows * slices * k) : 0;
+}
+
+int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uint64_t n, uint64_t ld, uint32_t k,
+                    void* d_values, int32_t* d_ids, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  if (k == 0 || k > F::kMaxK) return fail("k must be in [1, 256]");
+  if (n > F::kMaxRecords) return fail("a row holds at most 2^30 scores");
+  if (const char* w = check_rows(d_scores, elem, nq, n, ld)) return fail(w);
+  if (nq == 0) return SHINE_OK;
+  if (!d_values || !d_ids) return fail("NULL device pointer");
+  if (!on(d_values, elem_size(elem)) || !on(d_ids, 4)) return fail("a pointer is not aligned to its element type");
+  const uint64_t need = shine_flat_topk_workspace(nq, n, k);
+  if (need && (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < need))
+    return fail("workspace is missing, not 256-byte aligned or smaller than shine_flat_topk_workspace");
+  OnDevice dev(gpu_id);
+  if (dev.e != hipSuccess) return hip("flat topk: device", dev.e);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint32_t slices = F::topk_slices(std::min(nq, kRowBlock), n);
+  for (uint32_t q = 0; q < nq; q += kRowBlock) {
+    F::TopkArgs a{};
+    a.scores = static_cast<const char*>(d_scores) + q * ld * elem_size(elem);
+    a.ld = ld;
+    a.nq = std::min(kRowBlock, nq - q);
+    a.k = k;
+    a.n = n;
+    a.slices = slices;
+    a.keys = static_cast<uint64_t*>(d_workspace);
+    a.key_ld = slices;
+    a.values = static_cast<char*>(d_values) + static_cast<uint64_t>(q) * k * elem_size(elem);
+    a.ids = d_ids + static_cast<uint64_t>(q) * k;
+    if (hipError_t e = F::launch_topk(elem, false, a, s); e != hipSuccess) return hip("flat topk", e);
+    if (slices > 1) {
+      F::MergeArgs m{a.keys, static_cast<uint64_t>(slices) * k, a.nq, k, a.values, a.ids};
+      if (hipError_t e = F::launch_merge(elem, m, s); e != hipSuccess) return hip("flat topk", e);
+    }
+  }
+  return SHINE_OK;
+}
+
+uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k) {
+  return plan_search(nq, n, dim, k).total;
+}
+
+int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
+                      uint32_t k, const shine_flat_adjustment* adjustment, float* d_values, int32_t* d_ids,
+                      void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  if (const char* w = check_table(table)) return fail(w);
+  if (k == 0 || k > F::kMaxK) return fail("k must be in [1, 256]");
+  if (const char* w = check_rows(d_queries, elem, nq, table->dim, ld)) return fail(w);
+  if (adjustment)
+    if (const char* w = check_adjustment(adjustment, nq, table->n)) return fail(w);
+  if (nq == 0) return SHINE_OK;
+  if (!d_values || !d_ids) return fail("NULL device pointer");
+  if (!on(d_values, 4) || !on(d_ids, 4)) return fail("a pointer is not aligned to its element type");
+  const SearchPlan p = plan_search(nq, table->n, table->dim, k);
+  if (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < p.total)
+    return fail("workspace is missing, not 256-byte aligned or smaller than shine_flat_search_workspace");
+  OnDevice dev(gpu_id);
+  if (dev.e != hipSuccess) return hip("flat search: device", dev.e);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint32_t pitch = F::code_pitch(table->dim);
+  char* ws = static_cast<char*>(d_workspace);
+  for (uint32_t q = 0; q < nq; q += p.rows) {
+    const uint32_t m = std::min(p.rows, nq - q);
+    if (hipError_t e = quantize(static_cast<const char*>(d_queries) + q * ld * elem_size(elem), elem, m, table->dim, ld,
+                                reinterpret_cast<int8_t*>(ws + p.codes), reinterpret_cast<float*>(ws + p.scales), nullptr, s);
+        e != hipSuccess)
+      return hip("flat search", e);
+    for (uint32_t c = 0; c < p.chunks; ++c) {
+      const uint64_t first = c * p.cols, cols = std::min(p.cols, table->n - first);
+      F::ScoresArgs a{};
+      a.qcodes = reinterpret_cast<int8_t*>(ws + p.codes);
+      a.qscales = reinterpret_cast<float*>(ws + p.scales);
+      a.codes = table->codes + first * pitch;
+      a.scales = table->scales + first;
+      a.bias = table->bias ? table->bias + first : nullptr;
+      a.nq = m;
+      a.pitch = pitch;
+      a.n = cols;
+      a.out = ws + p.scores;
+      a.ld = p.cols;
+      if (hipError_t e = F::launch_scores(F::kF32, a, s); e != hipSuccess) return hip("flat search", e);
+      if (!neutral(adjustment)) {
+        F::AdjustArgs b = adjust_args(*adjustment, q);
+        b.scores = b.out = a.out;
+        b.ld = b.out_ld = p.cols;
+        b.nq = m;
+        b.n = cols;
+        b.first = first;
+        if (hipError_t e = F::launch_adjust(F::kF32, b, s); e != hipSuccess) return hip("flat search", e);
+      }
+      F::TopkArgs t{};
+      t.scores = a.out;
+      t.ld = p.cols;
+      t.nq = m;
+      t.k = k;
+      t.n = cols;
+      t.first = first;
+      t.slices = p.slices;
+      t.keys = reinterpret_cast<uint64_t*>(ws + p.keys) + static_cast<uint64_t>(c) * p.slices * k;
+      t.key_ld = p.chunks * p.slices;
+      if (hipError_t e = F::launch_topk(F::kF32, true, t, s); e != hipSuccess) return hip("flat search", e);
+    }
+    F::MergeArgs g{reinterpret_cast<uint64_t*>(ws + p.keys), static_cast<uint64_t>(p.chunks) * p.slices * k, m, k,
+                   d_values + static_cast<uint64_t>(q) * k, d_ids + static_cast<uint64_t>(q) * k};
+    if (hipError_t e = F::launch_merge(F::kF32, g, s); e != hipSuccess) return hip("flat search", e);
+  }
+  return SHINE_OK;
+}
+
+}  // extern "C"

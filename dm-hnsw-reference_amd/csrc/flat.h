@@ -1,0 +1,87 @@
+// Flat scoring: internal interface between the C entries (flat.cc) and the kernels (flat_kernels.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace shine::flat {
+
+constexpr uint32_t kMaxDim = 16384;   // sums of dim products of 8-bit codes stay below 2^31 (16384 * 127^2 = 2.6e8)
+constexpr uint32_t kMaxK = 256;       // answers of a top-k
+constexpr uint64_t kMaxRecords = 1ull << 30;  // ids are int32, a grid's threads a 32-bit number
+
+// bytes of a row of codes: whole 64-byte steps of the matrix instructions, zero behind dim
+inline uint32_t code_pitch(uint32_t dim) { return (dim + 63u) & ~63u; }
+
+enum Elem { kF32 = 0, kF16 = 1, kBF16 = 5 };  // SHINE_ELEM_F32 / _F16 / _BF16
+
+struct QuantizeArgs {
+  const void* rows;
+  uint64_t n, ld;  // ld in elements
+  uint32_t dim;
+  int8_t* codes;
+  float* scales;
+  float* half_norms;  // nullable
+};
+
+struct ScoresArgs {
+  const int8_t* qcodes;
+  const float* qscales;
+  const int8_t* codes;
+  const float* scales;
+  const float* bias;  // nullable
+  uint32_t nq, pitch;
+  uint64_t n;    // records of this launch
+  void* out;
+  uint64_t ld;   // in elements
+};
+
+struct AdjustArgs {
+  const void* scores;
+  void* out;
+  uint64_t ld, out_ld;
+  uint32_t nq;
+  uint64_t n;             // columns of this launch
+  uint64_t first;         // record of its first column
+  const float* bias;      // nullable; record j of row i at bias[i * bias_ld + j]
+  uint64_t bias_ld;
+  const uint32_t* allow;  // nullable; record j of row i: bit j % 32 of allow[i * allow_ld + j / 32]
+  uint64_t allow_ld;
+  const int32_t* seen;    // nullable
+  uint64_t seen_ld;
+  uint32_t seen_n;
+  const float *repetition, *frequency, *presence;  // each nullable
+};
+
+struct TopkArgs {
+  const void* scores;
+  uint64_t ld;
+  uint32_t nq, k;
+  uint64_t n;       // columns of this launch
+  uint64_t first;   // record of its first column
+  uint32_t slices;  // workgroups per row
+  uint64_t* keys;   // slices > 1 or keys_only: k keys of every (row, slice) at (row * key_ld + slice) * k
+  uint32_t key_ld;
+  void* values;
+  int32_t* ids;
+};
+
+struct MergeArgs {
+  const uint64_t* keys;  // per row: count keys
+  uint64_t count;
+  uint32_t nq, k;
+  void* values;
+  int32_t* ids;
+};
+
+uint32_t topk_slices(uint32_t nq, uint64_t n);
+
+hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s);
+hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s);
+hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s);
+hipError_t launch_topk(int elem, bool keys_only, const TopkArgs& a, hipStream_t s);
+hipError_t launch_merge(int elem, const MergeArgs& a, hipStream_t s);
+
+}  // namespace shine::flat

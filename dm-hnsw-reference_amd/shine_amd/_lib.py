@@ -17,6 +17,7 @@ HEADER = REPO_ROOT / "include" / "shine_gpu.h"
 OK, ERR_ARG, ERR_IO, ERR_FORMAT, ERR_HIP, ERR_NOMEM, ERR_OVERFLOW = range(7)
 METRIC_L2, METRIC_IP = 0, 1
 ELEM_F32, ELEM_F16, ELEM_U8, ELEM_I8, ELEM_AUTO = 0, 1, 2, 3, 4
+ELEM_BF16 = 5  # flat scoring only
 QS_DISTCOMPS, QS_VISITED_UPPER, QS_VISITED_L0, QS_LISTS_UPPER, QS_LISTS_L0, QS_MAX_NEXT, QS_STATUS, QS_NRESULT = range(8)
 QS_REMOTE_VEC, QS_REMOTE_LIST, QS_CACHED_VEC, QS_CACHED_LIST = range(8, 12)
 QS_WORDS = 12
@@ -138,6 +139,33 @@ class ViewPiece(C.Structure):
     ]
 
 
+class FlatTable(C.Structure):
+    _fields_ = [
+        ("codes", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("n", C.c_uint64),
+        ("dim", C.c_uint32),
+        ("reserved0", C.c_uint32),
+    ]
+
+
+class FlatAdjustment(C.Structure):
+    _fields_ = [
+        ("bias", C.c_void_p),
+        ("bias_ld", C.c_uint64),
+        ("allow", C.c_void_p),
+        ("allow_ld", C.c_uint64),
+        ("seen", C.c_void_p),
+        ("seen_ld", C.c_uint64),
+        ("seen_n", C.c_uint32),
+        ("reserved0", C.c_uint32),
+        ("repetition", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("presence", C.c_void_p),
+    ]
+
+
 VIEW_OWN, VIEW_COPY, VIEW_PEER = 0, 1, 2
 
 P = C.c_void_p
@@ -197,6 +225,16 @@ PROTOTYPES = {
     "shine_gpu_build_open": (I32, [P, I32, C.POINTER(P)]),
     "shine_gpu_build_open_ex": (I32, [P, U32, I32, C.POINTER(I32), U32, I32, C.c_double, C.POINTER(P)]),
     "shine_gpu_build_free": (I32, [P]),
+    "shine_flat_pitch": (U32, [U32]),
+    "shine_flat_quantize": (I32, [I32, P, I32, U64, U32, U64, P, P, P, P]),
+    "shine_flat_scores_workspace": (U64, [U32, U32]),
+    "shine_flat_scores": (I32, [I32, C.POINTER(FlatTable), P, I32, U32, U64, P, I32, U64, P, U64, P]),
+    "shine_flat_adjust": (I32, [I32, P, I32, U32, U64, U64, C.POINTER(FlatAdjustment), P, U64, P]),
+    "shine_flat_topk_workspace": (U64, [U32, U64, U32]),
+    "shine_flat_topk": (I32, [I32, P, I32, U32, U64, U64, U32, P, P, P, U64, P]),
+    "shine_flat_search_workspace": (U64, [U32, U64, U32, U32]),
+    "shine_flat_search": (I32, [I32, C.POINTER(FlatTable), P, I32, U32, U64, U32, C.POINTER(FlatAdjustment), P, P, P,
+                                U64, P]),
 }
 
 _lib = None

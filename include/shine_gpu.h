@@ -43,6 +43,8 @@ extern "C" {
 #define SHINE_ELEM_I8 3  /* components in {-128, ..., 127} */
 /* The narrowest lossless of U8, I8 and F32 for this index (never F16); shine_index_info.elem reports the choice. */
 #define SHINE_ELEM_AUTO 4
+/* bfloat16, for the operators of flat scoring (shine_flat_*) only: no index stores it. */
+#define SHINE_ELEM_BF16 5
 
 /* Per-query counter layout (u32 words), identical in the oracle and on the GPU. */
 #define SHINE_QS_DISTCOMPS 0     /* stats.distcomps                         (hnsw.hh:272,286,376,459) */
@@ -428,6 +430,78 @@ int shine_gpu_build_open(shine_gpu_build_t b, int elem, shine_index_t* out);
 int shine_gpu_build_open_ex(shine_gpu_build_t b, uint32_t n_shards, int elem, const int* gpu_ids, uint32_t n_gpus,
                             int placement, double cache_fraction, shine_index_t* out);
 int shine_gpu_build_free(shine_gpu_build_t b);
+
+/* ----------------------------------------------------------------------------------------------------------
+ * Flat scoring: every record of a table against every query, for filters that leave a graph search too few records,
+ * tables too small for a graph, candidate lists and ground truth.  Records are rows of 8-bit codes with a scale each;
+ * a score is an inner product of codes times both scales.  All pointers are device pointers of GPU gpu_id, calls are
+ * asynchronous on `stream` (NULL: the default stream), allocate nothing and can be captured into a graph; a workspace
+ * belongs to one call at a time (calls on different streams, and graphs that may run at once, take one each).  The
+ * caller's current device is left as it was.  Element types: SHINE_ELEM_F32, _F16, _BF16; row strides (ld) are in
+ * elements; rows may lie at any address that their element type allows.
+ * -------------------------------------------------------------------------------------------------------- */
+/* A record table: n rows of shine_flat_pitch(dim) code bytes (64-byte aligned; the bytes behind dim are read and change
+ * nothing), a scale for each record and optionally a number added to each record's scores. */
+typedef struct shine_flat_table {
+  const int8_t* codes;
+  const float* scales;
+  const float* bias; /* nullable */
+  uint64_t n;        /* <= 2^30 */
+  uint32_t dim;      /* <= 16384 */
+  uint32_t reserved0;
+} shine_flat_table;
+
+/* What shine_flat_adjust does to score s of record j in row i, in this order and in f32, rounded to the element type once:
+ *   c = how often j is among the row's seen ids; where c > 0: s = s > 0 ? s / repetition[i] : s * repetition[i], then
+ *   s = s - frequency[i] * c - presence[i];  s = s + bias;  where j's allowed bit is 0: s = -infinity, whatever it was.
+ * NULL members change nothing.  A stride of 0 shares one row among all queries. */
+typedef struct shine_flat_adjustment {
+  const float* bias;       /* bias[i * bias_ld + j] */
+  uint64_t bias_ld;
+  const uint32_t* allow;   /* bit j % 32 of allow[i * allow_ld + j / 32] */
+  uint64_t allow_ld;
+  const int32_t* seen;     /* seen[i * seen_ld + 0 .. seen_n - 1]: record ids, repeats counted, others (-1) skipped */
+  uint64_t seen_ld;
+  uint32_t seen_n;
+  uint32_t reserved0;
+  const float* repetition; /* one number per row, > 0 (1: none) */
+  const float* frequency;  /* one per row */
+  const float* presence;   /* one per row */
+} shine_flat_adjustment;
+
+/* Bytes of a row of codes: dim rounded up to 64. */
+uint32_t shine_flat_pitch(uint32_t dim);
+
+/* n rows of dim components -> codes (n * pitch bytes, 8-byte aligned; zero behind dim) and scales (n).  scale = f32(max|x| /
+ * 127), code = the integer nearest to x / scale, halves to even, in [-127, 127]; a row of zeros has scale 0 and codes 0, a
+ * row with an infinity or NaN scale NaN and codes 0.  d_half_norms (nullable, n): -|c * scale|^2 / 2, the bias that turns
+ * inner products into the order of L2 distances: |q - x|^2 = |q|^2 - 2 (<q, x> - |x|^2 / 2). */
+int shine_flat_quantize(int gpu_id, const void* d_rows, int elem, uint64_t n, uint32_t dim, uint64_t ld, int8_t* d_codes,
+                        float* d_scales, float* d_half_norms, void* stream);
+
+/* out[i][j] = (float(sum of code products) * query scale i) * table scale j (+ table bias j), each step rounded to f32 (the
+ * sum is exact), the result rounded to out_elem.  The queries are quantised as shine_flat_quantize does. */
+uint64_t shine_flat_scores_workspace(uint32_t nq, uint32_t dim);
+int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
+                      void* d_out, int out_elem, uint64_t out_ld, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* See shine_flat_adjustment.  d_out may be d_scores (with the same stride); otherwise the two do not overlap. */
+int shine_flat_adjust(int gpu_id, const void* d_scores, int elem, uint32_t nq, uint64_t n, uint64_t ld,
+                      const shine_flat_adjustment* adjustment, void* d_out, uint64_t out_ld, void* stream);
+
+/* The k (<= 256) largest scores of every row in descending order, equal ones in ascending id order: values (nq x k, of the
+ * scores' type) and ids (nq x k).  -infinity and NaN are never returned; places without an answer hold id -1 and value
+ * -infinity.  The workspace may be NULL where its size is 0. */
+uint64_t shine_flat_topk_workspace(uint32_t nq, uint64_t n, uint32_t k);
+int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uint64_t n, uint64_t ld, uint32_t k,
+                    void* d_values, int32_t* d_ids, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* shine_flat_scores (f32), shine_flat_adjust (nullable) and shine_flat_topk of every query, with the same results bit for
+ * bit, without the whole score matrix in memory. */
+uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k);
+int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
+                      uint32_t k, const shine_flat_adjustment* adjustment, float* d_values, int32_t* d_ids,
+                      void* d_workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,569 @@
+"""Flat scoring on the GPU against a plain implementation in 64 bits.
+
+Tolerances: a rounding to a type is off by at most u = finfo(type).eps / 2 of the value.  f32 steps: u32 = 2^-24.
+* quantisation: the codes are defined in real arithmetic on 32-bit numbers: they have to be equal.
+* scores: the sum of products is exact; its conversion, two products and (L2) one sum are rounded to f32:
+  3 u32 |p| (1 + 3 u32) for the product p, u32 |v| for the sum, then u |v| for the output type.
+* adjust: at most 6 f32 roundings, of values no larger than M = |s'| + |f c| + |p| + |b|; then u |v|.
+* top-k and search: values and ids equal those of the scores that they rank.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+NEG = -math.inf
+U32 = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def F():
+    from shine_amd import flat
+    return flat
+
+
+def rows(n, dim, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((n, dim), generator=g) * scale).to(dtype)
+
+
+# ---- the plain forms, in 64 bits on the CPU
+
+def codes64(x):
+    """codes (float64) and scales (float64 holding f32 numbers)"""
+    x = x.double()
+    scale = (x.abs().amax(1) / 127).float().double()
+    q = x / torch.where(scale > 0, scale, torch.ones_like(scale))[:, None]
+    return torch.where(scale[:, None] > 0, torch.round(q).clamp(-127, 127), torch.zeros_like(q)), scale
+
+
+def scores64(table, q, metric):
+    """exact scores, and the largest error that f32 steps may bring"""
+    xc, xs = codes64(table)
+    qc, qs = codes64(q)
+    p = (qc @ xc.T) * qs[:, None] * xs[None, :]
+    err = 3 * U32 * p.abs() * (1 + 3 * U32)
+    if metric == "l2":
+        half = xc.square().sum(1) * xs * xs / 2
+        p = p - half
+        err = err + 3 * U32 * half * (1 + 3 * U32) + U32 * (p.abs() + err)  # the half norm: a conversion, two products
+    return p, err
+
+
+def scores32(table, q, metric):
+    """the same in f32, step by step as the definition rounds"""
+    xc, xs = codes64(table)
+    qc, qs = codes64(q)
+    s = ((qc @ xc.T).float() * qs.float()[:, None]) * xs.float()[None, :]
+    if metric == "l2":
+        s = s + (-0.5 * ((xc.square().sum(1).float() * xs.float()) * xs.float()))
+    return s
+
+
+def adjust64(s, bias=None, allow=None, seen=None, repetition=None, frequency=None, presence=None):
+    s = s.double().clone()
+    nq, n = s.shape
+    big = torch.zeros_like(s)
+    for i in range(nq):
+        if seen is not None:
+            ids, c = np.unique([x for x in seen[i % seen.shape[0]].tolist() if 0 <= x < n], return_counts=True)
+            for j, m in zip(ids.astype(int), c):
+                r = float(repetition[i]) if repetition is not None else 1.0
+                f = float(frequency[i]) if frequency is not None else 0.0
+                p = float(presence[i]) if presence is not None else 0.0
+                v = s[i, j].item()
+                v = v / r if v > 0 else v * r
+                s[i, j] = v - f * m - p
+                big[i, j] = abs(f * m) + abs(p) + abs(v)
+    big = torch.maximum(big, s.abs())
+    if bias is not None:
+        b = bias.double().reshape(-1, n)
+        s = s + b
+        big = big + b.abs()
+    if allow is not None:
+        a = allow.reshape(-1, allow.shape[-1]).numpy().view(np.uint32)
+        on = np.unpackbits(a.view(np.uint8), axis=1, bitorder="little")[:, :n].astype(bool)
+        s = torch.where(torch.from_numpy(on).expand(nq, n), s, torch.tensor(NEG, dtype=torch.float64))
+    return s, 6 * U32 * big
+
+
+def topk_plain(s, k):
+    """by (value descending, id ascending); -inf and NaN are no answers"""
+    s = s.float().numpy() + np.float32(0)
+    nq, n = s.shape
+    values = np.full((nq, k), -np.inf, np.float32)
+    ids = np.full((nq, k), -1, np.int32)
+    for i in range(nq):
+        ok = np.nonzero(s[i] > -np.inf)[0]
+        order = ok[np.lexsort((ok, -s[i][ok].astype(np.float64)))][:k]
+        values[i, :len(order)] = s[i][order]
+        ids[i, :len(order)] = order
+    return torch.from_numpy(values), torch.from_numpy(ids)
+
+
+def close(got, want, err, dtype):
+    got, want = got.double().cpu(), want
+    u = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * u  # half a step below the normal numbers
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = (got - want).abs()
+    bound = err * (1 + u) + u * want.abs() + tiny
+    bad = ~same & ~(off <= bound)
+    assert not bad.any(), (int(bad.sum()), got[bad][:4], want[bad][:4], bound[bad][:4])
+
+
+def bits(n, nq, share, seed):
+    g = np.random.default_rng(seed)
+    on = g.random((nq, n)) < share
+    packed = np.packbits(np.pad(on, ((0, 0), (0, (-n) % 32))), axis=1, bitorder="little")
+    return torch.from_numpy(packed.copy().view(np.int32)), on
+
+
+# ---- quantisation
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 7), (1, 64), (5, 65), (33, 96), (17, 100), (130, 128), (65, 200), (9, 256),
+                                   (4, 257), (3, 1000), (2, 1025), (2, 16384)])
+def test_quantize_equals_the_definition(n, dim, dtype):
+    x = rows(n, dim, n * 1000 + dim, dtype)
+    codes, scales = F().quantize_rows(x.cuda())
+    want, scale = codes64(x)
+    assert codes.shape == (n, dim) and scales.shape == (n,)
+    assert torch.equal(codes.cpu().double(), want)
+    assert torch.equal(scales.cpu().double(), scale)
+
+
+def test_quantize_halves_go_to_even_and_borders_are_exact():
+    """Rows with 127 as their largest have scale 1: halves are exact ties.  A second row is built next to its borders."""
+    halves = torch.arange(-126.5, 127, 1.0)
+    x = torch.stack([torch.cat([torch.tensor([127.0]), halves, torch.zeros(1)])] * 2)
+    s = torch.tensor(0.37, dtype=torch.float32)
+    edge = (halves.double() * s.double()).float()
+    near = torch.cat([torch.tensor([127.0]) * s, edge, torch.zeros(1)])
+    up, down = torch.nextafter(near, torch.full_like(near, 1e9)), torch.nextafter(near, torch.full_like(near, -1e9))
+    up[0] = down[0] = near[0]
+    x = torch.cat([x, torch.stack([near, up, down])])
+    codes, scales = F().quantize_rows(x.cuda())
+    want, scale = codes64(x)
+    assert torch.equal(scales.cpu().double(), scale)
+    assert torch.equal(codes.cpu().double(), want)
+
+
+def test_quantize_extreme_rows():
+    big, tiny = torch.finfo(torch.float32).max, 2.0 ** -149
+    x = torch.tensor([[0.0, -0.0, 0.0], [big, -big, big / 3], [tiny, 0.0, -tiny], [tiny * 100, tiny * 200, -tiny * 50],
+                      [1e-35, -3e-36, 2e-36], [1e-29, 3e-31, -7e-30], [1.0, math.nan, 0.0], [math.inf, 1.0, 2.0],
+                      [-math.inf, math.nan, 1.0]])
+    codes, scales = F().quantize_rows(x.cuda())
+    want, scale = codes64(x[:6])
+    assert torch.equal(scales[:6].cpu().double(), scale)
+    assert torch.equal(codes[:6].cpu().double(), want)
+    assert scales[6:].isnan().all() and not codes[6:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_strided_rows(dtype):
+    """rows at every address that the type allows, with a stride of their own"""
+    base = rows(20, 150, 5, dtype)
+    for off, dim in ((0, 100), (1, 96), (3, 128), (7, 65)):
+        x = base[:, off:off + dim]
+        codes, scales = F().quantize_rows(base.cuda()[:, off:off + dim])
+        want, scale = codes64(x)
+        assert torch.equal(codes.cpu().double(), want) and torch.equal(scales.cpu().double(), scale)
+
+
+# ---- scores
+
+SCORE_SIZES = [(1, 1, 1), (1, 33, 8), (2, 31, 64), (1, 1000, 128), (5, 130, 96), (16, 257, 100), (17, 300, 200), (63, 65, 65),
+               (64, 128, 256), (65, 129, 300), (130, 515, 128), (3, 2000, 1024), (70, 140, 1025), (2, 40, 4096),
+               (200, 33, 513), (257, 1030, 96)]
+
+
+@pytest.mark.parametrize("metric", ["ip", "l2"])
+@pytest.mark.parametrize("nq,n,dim", SCORE_SIZES)
+def test_scores(nq, n, dim, metric):
+    x, q = rows(n, dim, dim + n), rows(nq, dim, dim + nq + 7)
+    table = F().FlatTable(x.cuda(), metric=metric)
+    want, err = scores64(x, q, metric)
+    s = F().scores(table, q.cuda())
+    close(s, want, err, torch.float32)
+    assert torch.equal(s.cpu(), scores32(x, q, metric))
+    for dtype in (torch.float16, torch.bfloat16):
+        t = F().scores(table, q.cuda(), dtype=dtype)
+        close(t, want, err, dtype)
+        assert torch.equal(t, s.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_of_each_query_type(dtype):
+    x, q = rows(150, 200, 1, dtype), rows(40, 200, 2, dtype)
+    table = F().FlatTable(x.cuda())
+    assert torch.equal(F().scores(table, q.cuda()).cpu(), scores32(x, q, "ip"))
+
+
+def test_scores_largest_sums():
+    """every product at its largest: the sums pass 2^24 and stay exact"""
+    for dim in (1040, 1041, 16384):
+        x = torch.ones(3, dim)
+        x[1] = -1
+        table = F().FlatTable(x.cuda())
+        want, err = scores64(x, x, "ip")
+        s = F().scores(table, x.cuda())
+        close(s, want, err, torch.float32)
+        assert torch.equal(s.cpu(), scores32(x, x, "ip"))
+
+
+def test_scores_of_rows_without_a_scale():
+    x = rows(10, 32, 3)
+    x[2] = 0
+    x[5, 7] = math.nan
+    q = rows(4, 32, 4)
+    q[1] = 0
+    q[3, 0] = math.inf
+    s = F().scores(F().FlatTable(x.cuda(), metric="l2"), q.cuda()).cpu()
+    assert s[3].isnan().all() and s[:, 5].isnan().all()
+    keep = [0, 1, 2, 3, 4, 6, 7, 8, 9]
+    assert torch.equal(s[:3][:, keep], scores32(x[keep], q[:3], "l2"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n,dim", [(3, 45, 96), (70, 301, 128), (20, 64, 300)])
+def test_scores_into_a_strided_out(dtype, nq, n, dim):
+    """rows of an odd stride at an odd place: nothing beside them is written"""
+    x, q = rows(n, dim, 8), rows(nq, dim, 9)
+    table = F().FlatTable(x.cuda())
+    whole = torch.full((nq + 2, n + 13), 7.0, dtype=dtype, device="cuda")
+    out = whole[1:nq + 1, 5:5 + n]
+    assert F().scores(table, q.cuda(), out=out).data_ptr() == out.data_ptr()
+    assert torch.equal(out, F().scores(table, q.cuda(), dtype=dtype))
+    whole[1:nq + 1, 5:5 + n] = 7.0
+    assert (whole == 7.0).all()
+
+
+# ---- adjust
+
+def adjustments(nq, n, seed, h=0, bias=None, allow=None):
+    g = torch.Generator().manual_seed(seed)
+    a = {}
+    if bias:
+        a["bias"] = torch.randn((n,) if bias == "shared" else (nq, n), generator=g) * 0.2
+    if allow:
+        a["allow"] = bits(n, 1 if allow == "shared" else nq, 0.6, seed)[0]
+    if h:
+        a["seen"] = torch.randint(-2, min(n, 2 * h) + 3, (nq, h), generator=g, dtype=torch.int32)
+        a["repetition"] = 1 + torch.rand(nq, generator=g)
+        a["frequency"] = torch.rand(nq, generator=g) * 0.1
+        a["presence"] = torch.rand(nq, generator=g) * 0.2
+    return a
+
+
+def cuda(a):
+    return {k: v.cuda() for k, v in a.items()}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n", [(1, 1), (1, 31), (2, 33), (3, 4095), (1, 4097), (5, 8191), (2, 20003)])
+@pytest.mark.parametrize("h,bias,allow", [(0, "shared", None), (0, None, "rows"), (1, None, None), (40, "rows", "shared"),
+                                          (700, "shared", "rows")])
+def test_adjust(dtype, nq, n, h, bias, allow):
+    s = rows(nq, n, nq + n, dtype)
+    a = adjustments(nq, n, n + h, h, bias, allow)
+    want, err = adjust64(s, **a)
+    close(F().adjust(s.cuda(), **cuda(a)), want, err, dtype)
+
+
+def test_adjust_one_at_a_time_and_in_place():
+    s = rows(4, 5000, 1)
+    a = adjustments(4, 5000, 2, 30, "rows", "rows")
+    for some in ([], ["seen"], ["seen", "repetition"], ["seen", "frequency"], ["seen", "presence"], ["bias"], ["allow"]):
+        b = {k: a[k] for k in some}
+        want, err = adjust64(s, **b)
+        close(F().adjust(s.cuda(), **cuda(b)), want, err, torch.float32)
+    x = s.cuda()
+    want = F().adjust(x, **cuda(a))
+    assert F().adjust(x, **cuda(a), out=x) is x
+    assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_adjust_special_values(dtype):
+    """masks win over everything, infinities and NaN pass, the type's lowest value stays, counts of one id in thousands"""
+    n = 300
+    s = rows(3, n, 4, dtype)
+    s[0, 0], s[0, 1], s[0, 2], s[0, 3] = math.nan, math.inf, NEG, torch.finfo(dtype).min
+    s[1, :4] = s[0, :4]
+    s[1, 4] = 0.0
+    allow, on = bits(n, 3, 0.5, 6)
+    a = allow.numpy().view(np.uint32)
+    a[0, 0] &= ~np.uint32(0xF)   # row 0: the special values are masked
+    a[1, 0] |= np.uint32(0xFF)   # row 1: they are not
+    a[2] = 0                     # row 2: nothing is left
+    seen = torch.full((3, 5000), 4, dtype=torch.int32)
+    arg = dict(allow=allow, seen=seen, repetition=torch.full((3,), 2.0), frequency=torch.full((3,), 0.25),
+               presence=torch.full((3,), 0.5))
+    got = F().adjust(s.cuda(), **cuda(arg))
+    want, err = adjust64(s, **arg)
+    close(got, want, err, dtype)
+    assert (got[2] == NEG).all() and (got[0, :4] == NEG).all()
+    assert got[1, 0].isnan() and got[1, 1] == math.inf and got[1, 2] == NEG and got[1, 3] == torch.finfo(dtype).min
+    values, ids = F().topk(got, 5)
+    assert (ids[2] == -1).all() and (values[2] == NEG).all()
+
+
+def test_adjust_strides():
+    whole = rows(7, 999, 3).cuda()
+    s = whole[1:5, 3:903]
+    a = adjustments(4, 900, 2, 30, "rows", "rows")
+    big = {k: torch.zeros((v.shape[0], v.shape[1] + 9), dtype=v.dtype, device="cuda") for k, v in a.items() if v.dim() == 2}
+    b = cuda(a)
+    for k, v in big.items():
+        v[:, 2:2 + a[k].shape[1]] = b[k]
+        b[k] = v[:, 2:2 + a[k].shape[1]]
+    out = torch.full((4, 1001), 5.0, device="cuda")
+    F().adjust(s, **b, out=out[:, 1:901])
+    assert torch.equal(out[:, 1:901], F().adjust(s.contiguous(), **cuda(a)))
+    assert (out[:, 0] == 5).all() and (out[:, 901:] == 5).all()
+
+
+# ---- top-k
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n,k", [(1, 1, 1), (1, 1, 256), (2, 5, 3), (3, 64, 64), (1, 255, 256), (1, 256, 256), (1, 257, 256),
+                                    (4, 1000, 10), (2, 4096, 100), (1, 4097, 1), (1, 70001, 256), (3, 30011, 17),
+                                    (1100, 700, 9)])
+def test_topk(dtype, nq, n, k):
+    s = rows(nq, n, nq * 7 + n + k, dtype)  # 16-bit types: many ties
+    values, ids = F().topk(s.cuda(), k)
+    want_v, want_i = topk_plain(s, k)
+    assert torch.equal(ids.cpu(), want_i)
+    assert torch.equal(values.cpu().float(), want_v)
+    assert values.dtype == dtype
+
+
+@pytest.mark.parametrize("k", [1, 10, 100, 256])
+@pytest.mark.parametrize("order", ["rising", "falling", "equal", "two values", "few left", "none left", "specials"])
+def test_topk_orders(order, k):
+    n = 50001
+    s = torch.arange(n, dtype=torch.float32) / 8 - 3000
+    if order == "falling":
+        s = s.flip(0)
+    elif order == "equal":
+        s = torch.full((n,), -1.5)
+    elif order == "two values":
+        s = torch.where(torch.arange(n) % 3 == 0, 1.0, -2.0)
+    elif order == "few left":
+        s = torch.where(torch.arange(n) % 9001 == 77, s, NEG)
+    elif order == "none left":
+        s = torch.full((n,), NEG)
+    elif order == "specials":
+        s[::7], s[1::11], s[2::5], s[3::13], s[4::17] = math.nan, NEG, 0.0, -0.0, -math.nan
+        s[40000], s[100] = math.inf, math.inf
+        s[5], s[6] = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+        s[s > 0] = torch.where(torch.arange(int((s > 0).sum())) < 150, s[s > 0], NEG)
+    s = torch.stack([s, s.roll(333)])
+    values, ids = F().topk(s.cuda(), k)
+    want_v, want_i = topk_plain(s, k)
+    assert torch.equal(ids.cpu(), want_i)
+    assert torch.equal(values.cpu(), want_v)
+
+
+def test_topk_of_strided_rows_and_no_columns():
+    whole = rows(5, 3001, 3).cuda()
+    s = whole[1:4, 7:2900]
+    assert all(torch.equal(a, b) for a, b in zip(F().topk(s, 20), F().topk(s.contiguous(), 20)))
+    values, ids = F().topk(whole[:, :0], 3)
+    assert (ids == -1).all() and (values == NEG).all()
+    assert F().topk(whole[:0], 3)[0].shape == (0, 3)
+
+
+# ---- search: a run of all of them together
+
+SEARCH = [(1, 1, 4, 1), (1, 100, 16, 10), (1, 40000, 128, 10), (3, 777, 96, 100), (17, 5000, 200, 256), (64, 4099, 128, 10),
+          (65, 8300, 64, 37), (100, 2500, 300, 10), (2100, 600, 32, 5), (5, 3000, 1100, 20)]
+
+
+@pytest.mark.parametrize("metric", ["ip", "l2"])
+@pytest.mark.parametrize("nq,n,dim,k", SEARCH)
+def test_search(nq, n, dim, k, metric):
+    x, q = rows(n, dim, 2 * n + dim), rows(nq, dim, dim + 1)
+    table = F().FlatTable(x.cuda(), metric=metric)
+    values, ids = F().search(table, q.cuda(), k)
+    want_v, want_i = topk_plain(scores32(x, q, metric), k)
+    assert torch.equal(ids.cpu(), want_i)
+    assert torch.equal(values.cpu(), want_v)
+    if metric == "l2":  # the distances of the rows that the codes stand for, in 64 bits
+        xc, xs = codes64(x)
+        qc, qs = codes64(q)
+        xd, qd = xc * xs[:, None], qc * qs[:, None]
+        d = F().FlatTable.distances(table, values, qd.float().cuda()).cpu().double()
+        m = min(k, n)
+        want = (qd[:, None] - xd[want_i[:, :m].long()]).square().sum(2) if nq * m * dim < 1e8 else None
+        if want is not None:
+            size = qd.square().sum(1)[:, None] + 2 * qd.norm(dim=1)[:, None] * xd.norm(dim=1).max() + xd.square().sum(1).max()
+            assert ((d[:, :m] - want).abs() <= (dim + 8) * 2 * U32 * size).all()
+
+
+@pytest.mark.parametrize("nq,n,dim,k,h,bias,allow", [
+    (1, 3000, 128, 10, 0, None, "shared"), (1, 50000, 96, 100, 20, "shared", "rows"), (40, 6000, 200, 50, 300, "shared", "rows"),
+    (70, 5003, 64, 10, 0, "rows", "shared"), (33, 4097, 100, 256, 5, None, None), (130, 900, 128, 10, 64, "rows", "rows"),
+    (9, 9000, 700, 12, 33, "shared", "shared")])
+def test_search_with_adjustments(nq, n, dim, k, h, bias, allow):
+    x, q = rows(n, dim, n), rows(nq, dim, nq)
+    a = adjustments(nq, n, 3, h, bias, allow)
+    flat = F()
+    for metric in ("ip", "l2"):
+        table = flat.FlatTable(x.cuda(), metric=metric)
+        values, ids = flat.search(table, q.cuda(), k, **cuda(a))
+        v, i = flat.topk(flat.adjust(flat.scores(table, q.cuda()), **cuda(a)), k)
+        assert torch.equal(ids, i) and torch.equal(values, v)
+        want, err = adjust64(scores32(x, q, metric), **a)
+        live = ids.cpu() >= 0
+        at = torch.where(live, ids.cpu(), 0).long()
+        close(torch.where(live, values.cpu(), 0.0), torch.where(live, want.gather(1, at), 0.0), err.gather(1, at), torch.float32)
+
+
+def test_search_rows_that_a_filter_leaves_empty_and_short():
+    flat = F()
+    n = 10000
+    table = flat.FlatTable(rows(n, 96, 1).cuda())
+    allow = torch.zeros((3, (n + 31) // 32), dtype=torch.int32)
+    allow[1, 100], allow[1, 312] = 5, 1 << 15      # records 3200, 3202, 9999
+    allow[2] = -1
+    values, ids = flat.search(table, rows(3, 96, 2).cuda(), 10, allow=allow.cuda())
+    assert (ids[0] == -1).all() and (values[0] == NEG).all()
+    assert sorted(ids[1, :3].tolist()) == [3200, 3202, 9999] and (ids[1, 3:] == -1).all()
+    assert (ids[2] >= 0).all()
+
+
+def test_search_equal_records_come_in_id_order():
+    x = rows(50, 64, 1).repeat(200, 1)  # every record 200 times
+    table = F().FlatTable(x.cuda(), metric="l2")
+    q = rows(20, 64, 2)
+    values, ids = F().search(table, q.cuda(), 250)
+    want_v, want_i = topk_plain(scores32(x, q, "l2"), 250)
+    assert torch.equal(ids.cpu(), want_i) and torch.equal(values.cpu(), want_v)
+
+
+def test_search_of_sorted_records():
+    """every record better than all before it: the worst order for what is kept"""
+    n = 30000
+    x = torch.zeros(n, 16)
+    x[:, 0] = torch.linspace(1, 2, n)
+    q = torch.zeros(70, 16)
+    q[:, 0] = 1
+    q[1::2, 0] = -1
+    for k in (10, 256):
+        values, ids = F().search(F().FlatTable(x.cuda()), q.cuda(), k)
+        want_v, want_i = topk_plain(scores32(x, q, "ip"), k)
+        assert torch.equal(ids.cpu(), want_i) and torch.equal(values.cpu(), want_v)
+
+
+def test_search_with_records_and_queries_without_a_scale():
+    x, q = rows(500, 32, 3), rows(4, 32, 4)
+    x[7, 3], x[450, 0] = math.nan, math.inf
+    q[2, 1] = math.nan
+    values, ids = F().search(F().FlatTable(x.cuda()), q.cuda(), 256)
+    assert (ids[2] == -1).all()
+    assert not ((ids == 7) | (ids == 450)).any() and (ids[[0, 1, 3]] >= 0).all() and values[[0, 1, 3]].isfinite().all()
+
+
+def test_empty_tables_and_batches():
+    flat = F()
+    table = flat.FlatTable(torch.empty((0, 32), device="cuda"))
+    q = rows(3, 32, 1).cuda()
+    assert flat.scores(table, q).shape == (3, 0)
+    values, ids = flat.search(table, q, 4)
+    assert (ids == -1).all() and (values == NEG).all()
+    table = flat.FlatTable(rows(10, 32, 1).cuda())
+    assert flat.scores(table, q[:0]).shape == (0, 10)
+    assert flat.search(table, q[:0], 4)[1].shape == (0, 4)
+
+
+# ---- streams, graphs, refusals
+
+def test_calls_on_other_streams_at_once():
+    flat = F()
+    table = flat.FlatTable(rows(40000, 128, 1).cuda(), metric="l2")
+    qs = [rows(32, 128, 10 + i).cuda() for i in range(4)]
+    want = [flat.search(table, q, 10) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = []
+    for q, st in zip(qs, streams):
+        with torch.cuda.stream(st):
+            got.append([flat.search(table, q, 10) for _ in range(3)])
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for values, ids in g:
+            assert torch.equal(values, w[0]) and torch.equal(ids, w[1])
+
+
+def test_captured_and_replayed():
+    """two graphs with workspaces of their own, replayed with new inputs between the program's own calls"""
+    flat = F()
+    table = flat.FlatTable(rows(30000, 96, 1).cuda())
+    a = cuda(adjustments(24, 30000, 5, 50, "shared", "rows"))
+    buffers, graphs, outs = [], [], []
+    for i in range(2):
+        q = rows(24, 96, 20 + i).cuda()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            flat.topk(flat.adjust(flat.scores(table, q), **a), 10), flat.search(table, q, 10, **a)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s = flat.scores(table, q)
+            outs.append((flat.topk(flat.adjust(s, **a), 10), flat.search(table, q, 10, **a)))
+        buffers.append(q)
+        graphs.append(g)
+    for turn in range(4):
+        for i in (0, 1):
+            buffers[i].copy_(rows(24, 96, 100 + 10 * turn + i))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            values, ids = flat.search(table, buffers[i], 10, **a)
+            for v, j in outs[i]:
+                assert torch.equal(v, values) and torch.equal(j, ids)
+
+
+def test_python_refusals():
+    flat = F()
+    x = rows(20, 32, 1).cuda()
+    table = flat.FlatTable(x)
+    with pytest.raises(ValueError, match="dim 31"):
+        flat.scores(table, x[:, :31])
+    with pytest.raises(ValueError, match="unit stride"):
+        flat.quantize_rows(x.T)
+    with pytest.raises(ValueError, match="gradient"):
+        flat.scores(table, x.clone().requires_grad_())
+    with pytest.raises(ValueError, match="k must"):
+        flat.topk(x, 257)
+    with pytest.raises(ValueError, match="k must"):
+        flat.search(table, x, 0)
+    with pytest.raises(ValueError, match="out must"):
+        flat.scores(table, x, out=torch.empty(20, 21, device="cuda"))
+    with pytest.raises(ValueError, match="allow"):
+        flat.adjust(x, allow=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="bias"):
+        flat.adjust(x, bias=torch.zeros(32, dtype=torch.float64, device="cuda"))
+    with pytest.raises(ValueError, match="bias"):
+        flat.adjust(x, bias=torch.zeros(32))
+    with pytest.raises(ValueError, match="needs seen"):
+        flat.adjust(x, presence=torch.zeros(20, device="cuda"))
+    with pytest.raises(ValueError, match="repetition"):
+        flat.adjust(x, seen=torch.zeros((20, 1), dtype=torch.int32, device="cuda"), repetition=torch.ones(19, device="cuda"))
+    with pytest.raises(Exception, match="stride"):
+        flat.topk(x[:1].expand(5, 32), 3)
