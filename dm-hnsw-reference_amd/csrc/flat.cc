@@ -101,27 +101,148 @@ hipError_t quantize(const void* rows, int elem, uint64_t n, uint32_t dim, uint64
   return hipSuccess;
 }
 
-// search: blocks of rows x chunks of records whose scores fit kChunkScores
+// Search, stepwise: blocks of rows x chunks of records whose scores fit kChunkScores, scored, adjusted and ranked.
 constexpr uint64_t kChunkScores = 1ull << 26;
+// Search, fused: bytes that a block of rows may take for its lists, and for its masks.
+constexpr uint64_t kListBytes = 256ull << 20;
+constexpr uint32_t kMaxPasses = 8;
+
 struct SearchPlan {
+  bool fused;
   uint32_t rows;       // rows of a block
-  uint64_t cols;       // records of a chunk, whole tiles of 4,096
+  uint64_t cols;       // stepwise: records of a chunk, whole tiles of 4,096
   uint32_t chunks, slices;
-  uint64_t codes, scales, scores, keys, total;  // offsets into the workspace
+  uint32_t passes;     // fused
+  uint64_t stride[kMaxPasses], cap, words;
+  uint64_t codes, scales, scores, keys, thr, count, mask, extra, extra_count, total;  // offsets into the workspace
 };
-SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k) {
+
+// Fused passes cost less than the score matrix once it is larger than the table: from 17 queries on.  A bias for each row
+// is as large as the matrix itself, and wide rows' queries do not fit the registers: these are searched stepwise.
+SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const shine_flat_adjustment* a) {
   SearchPlan p{};
+  const uint32_t pitch = F::code_pitch(dim), seen_n = a ? a->seen_n : 0;
+  p.fused = nq > 16 && n > 0 && pitch <= F::kMaxFusedPitch && seen_n <= F::kMaxSeen && !(a && a->bias && a->bias_ld);
   p.rows = std::min(std::max(nq, 1u), 2048u);
-  p.cols = std::max<uint64_t>(4096, kChunkScores / p.rows / 4096 * 4096);
-  p.cols = std::min(p.cols, std::max<uint64_t>(1, n));
-  p.chunks = static_cast<uint32_t>((n + p.cols - 1) / p.cols);
-  p.slices = F::topk_slices(p.rows, p.cols);
-  p.codes = 0;
-  p.scales = aligned(static_cast<uint64_t>(p.rows) * F::code_pitch(dim));
-  p.scores = p.scales + aligned(4ull * p.rows);
-  p.keys = p.scores + aligned(4ull * p.rows * p.cols);
-  p.total = p.keys + aligned(8ull * p.rows * p.chunks * p.slices * k);
+  uint64_t at = 0;
+  auto take = [&at](uint64_t bytes) {
+    const uint64_t here = at;
+    at += aligned(bytes);
+    return here;
+  };
+  if (p.fused) {
+    const uint64_t blocks = (n + 31) / 32, coarse = k > 64 ? 256 : 128;  // blocks of the coarsest pass
+    uint64_t ratio = 1;
+    if (blocks <= 256) {
+      p.passes = 1;
+      p.stride[0] = 1;
+    } else {
+      // each pass at most 32 times the one before: its list then holds about 32 k keys
+      const uint64_t s0 = (blocks + coarse - 1) / coarse;
+      uint32_t steps = 1;
+      for (ratio = s0; ratio > 32; ++steps) {
+        ratio = 2;
+        auto power = [&](uint64_t r) {
+          uint64_t v = 1;
+          for (uint32_t i = 0; i < steps + 1; ++i) v *= r;
+          return v;
+        };
+        while (power(ratio) < s0) ++ratio;
+      }
+      p.passes = steps + 1;
+      p.stride[0] = s0;
+      uint64_t v = 1;
+      for (uint32_t i = 0; i < steps; ++i, v *= ratio) p.stride[steps - i] = v;
+    }
+    p.cap = std::max<uint64_t>((blocks + p.stride[0] - 1) / p.stride[0] * 32, p.passes > 1 ? 2 * k * ratio + 1024 : 0);
+    p.words = blocks;
+    p.rows = std::min<uint64_t>(p.rows, std::max<uint64_t>(128, kListBytes / (8 * p.cap) / 128 * 128));
+    if (seen_n) p.rows = std::min<uint64_t>(p.rows, std::max<uint64_t>(32, kListBytes / (4 * p.words) / 32 * 32));
+  } else {
+    p.cols = std::max<uint64_t>(4096, kChunkScores / p.rows / 4096 * 4096);
+    p.cols = std::min(p.cols, std::max<uint64_t>(1, n));
+    p.chunks = static_cast<uint32_t>((n + p.cols - 1) / p.cols);
+    p.slices = F::topk_slices(p.rows, p.cols);
+  }
+  p.codes = take(static_cast<uint64_t>(p.rows) * pitch);
+  p.scales = take(4ull * p.rows);
+  if (p.fused) {
+    p.keys = take(8 * p.cap * p.rows);
+    p.thr = take(8ull * p.rows);
+    p.count = take(4ull * p.rows);
+    if (seen_n) {
+      p.mask = take(4 * p.words * p.rows);
+      p.extra = take(8ull * seen_n * p.rows);
+      p.extra_count = take(4ull * p.rows);
+    }
+  } else {
+    p.scores = take(4ull * p.rows * p.cols);
+    p.keys = take(8ull * p.rows * p.chunks * p.slices * k);
+  }
+  p.total = at;
   return p;
+}
+
+hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const shine_flat_adjustment* a, uint32_t q,
+                        uint32_t m, uint32_t k, char* ws, float* values, int32_t* ids, hipStream_t s) {
+  F::PassArgs pass{};
+  pass.qcodes = reinterpret_cast<int8_t*>(ws + p.codes);
+  pass.qscales = reinterpret_cast<float*>(ws + p.scales);
+  pass.codes = t.codes;
+  pass.scales = t.scales;
+  pass.tbias = t.bias;
+  pass.nq = m;
+  pass.pitch = F::code_pitch(t.dim);
+  pass.n = t.n;
+  pass.thr = reinterpret_cast<uint64_t*>(ws + p.thr);
+  pass.count = reinterpret_cast<uint32_t*>(ws + p.count);
+  pass.keys = reinterpret_cast<uint64_t*>(ws + p.keys);
+  pass.cap = p.cap;
+  F::SelectArgs sel{};
+  if (a) {
+    const F::AdjustArgs r = adjust_args(*a, q);
+    pass.abias = r.bias;
+    pass.allow = r.allow;
+    pass.allow_ld = r.allow_ld;
+    if (r.seen) {
+      F::SeenArgs seen{};
+      seen.pass = pass;
+      seen.seen = r.seen;
+      seen.seen_ld = r.seen_ld;
+      seen.seen_n = r.seen_n;
+      seen.repetition = r.repetition;
+      seen.frequency = r.frequency;
+      seen.presence = r.presence;
+      seen.mask = reinterpret_cast<uint32_t*>(ws + p.mask);
+      seen.mask_ld = p.words;
+      seen.extra = reinterpret_cast<uint64_t*>(ws + p.extra);
+      seen.extra_count = reinterpret_cast<uint32_t*>(ws + p.extra_count);
+      seen.extra_ld = r.seen_n;
+      if (hipError_t e = F::launch_seen(seen, s); e != hipSuccess) return e;
+      pass.allow = seen.mask;
+      pass.allow_ld = seen.mask_ld;
+      sel.extra = seen.extra;
+      sel.extra_count = seen.extra_count;
+      sel.extra_ld = seen.extra_ld;
+    }
+  }
+  const uint64_t* extra = sel.extra;
+  for (uint32_t i = 0; i < p.passes; ++i) {
+    const bool last = i + 1 == p.passes;
+    pass.stride = p.stride[i];
+    pass.blocks = (p.words + pass.stride - 1) / pass.stride;
+    pass.store = i == 0;
+    if (hipError_t e = F::launch_pass(pass, s); e != hipSuccess) return e;
+    sel.pass = pass;
+    sel.k = k;
+    sel.fixed = i == 0 ? pass.blocks * 32 : 0;
+    sel.extra = last ? extra : nullptr;
+    sel.thr = last ? nullptr : const_cast<uint64_t*>(pass.thr);
+    sel.values = values;
+    sel.ids = ids;
+    if (hipError_t e = F::launch_select(sel, s); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -247,8 +368,9 @@ int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uin
   return SHINE_OK;
 }
 
-uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k) {
-  return plan_search(nq, n, dim, k).total;
+uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k,
+                                     const shine_flat_adjustment* adjustment) {
+  return plan_search(nq, n, dim, k, adjustment).total;
 }
 
 int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
@@ -262,7 +384,7 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
   if (nq == 0) return SHINE_OK;
   if (!d_values || !d_ids) return fail("NULL device pointer");
   if (!on(d_values, 4) || !on(d_ids, 4)) return fail("a pointer is not aligned to its element type");
-  const SearchPlan p = plan_search(nq, table->n, table->dim, k);
+  const SearchPlan p = plan_search(nq, table->n, table->dim, k, adjustment);
   if (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < p.total)
     return fail("workspace is missing, not 256-byte aligned or smaller than shine_flat_search_workspace");
   OnDevice dev(gpu_id);
@@ -276,6 +398,12 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
                                 reinterpret_cast<int8_t*>(ws + p.codes), reinterpret_cast<float*>(ws + p.scales), nullptr, s);
         e != hipSuccess)
       return hip("flat search", e);
+    if (p.fused) {
+      if (hipError_t e = search_fused(p, *table, adjustment, q, m, k, ws, d_values + static_cast<uint64_t>(q) * k,
+                                      d_ids + static_cast<uint64_t>(q) * k, s); e != hipSuccess)
+        return hip("flat search", e);
+      continue;
+    }
     for (uint32_t c = 0; c < p.chunks; ++c) {
       const uint64_t first = c * p.cols, cols = std::min(p.cols, table->n - first);
       F::ScoresArgs a{};

@@ -38,6 +38,56 @@ struct ScoresArgs {
   uint64_t ld;   // in elements
 };
 
+// One pass of a fused search over every `stride`-th block of 32 records.
+struct PassArgs {
+  const int8_t* qcodes;
+  const float* qscales;
+  const int8_t* codes;
+  const float* scales;
+  const float* tbias;     // nullable: the table's
+  const float* abias;     // nullable: the adjustment's, shared by all queries
+  const uint32_t* allow;  // nullable; word w of query q at q * allow_ld + w
+  uint64_t allow_ld;
+  uint32_t nq, pitch;
+  uint64_t n;
+  uint64_t blocks;        // ceil(ceil(n / 32) / stride): blocks of this pass
+  uint64_t stride;
+  bool store;             // every key at keys[q * cap + 32 * block + i]; else those from thr on, appended
+  const uint64_t* thr;    // per query; key 0: none
+  uint32_t* count;        // per query: keys offered to its list (may pass cap; the list then holds cap of them)
+  uint64_t* keys;
+  uint64_t cap;
+};
+
+// Selection from a search's lists: the k-th best key (thr) between passes, the answers behind the last one.
+struct SelectArgs {
+  PassArgs pass;          // what a row whose list overflowed is scanned again with (answers only)
+  uint32_t k;
+  uint64_t fixed;         // keys of every list, or 0: count[q]
+  const uint64_t* extra;  // nullable: extra_count[q] more keys at extra + q * extra_ld
+  const uint32_t* extra_count;
+  uint64_t extra_ld;
+  uint64_t* thr;          // not nullptr: write the k-th best key and clear count
+  float* values;
+  int32_t* ids;
+};
+
+// A history's records: taken out of the row's mask, and scored with their penalties.
+struct SeenArgs {
+  PassArgs pass;          // its allow (nullable) is the caller's
+  const int32_t* seen;
+  uint64_t seen_ld;
+  uint32_t seen_n;
+  const float *repetition, *frequency, *presence;
+  uint32_t* mask;         // nq rows of mask_ld words
+  uint64_t mask_ld;
+  uint64_t* extra;
+  uint32_t* extra_count;
+  uint64_t extra_ld;
+};
+constexpr uint32_t kMaxSeen = 4096;       // longest history of a fused search (its ids are sorted in LDS)
+constexpr uint32_t kMaxFusedPitch = 256;  // widest rows of a fused search (the queries' codes stay in registers)
+
 struct AdjustArgs {
   const void* scores;
   void* out;
@@ -80,6 +130,9 @@ uint32_t topk_slices(uint32_t nq, uint64_t n);
 
 hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s);
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s);
+hipError_t launch_pass(const PassArgs& a, hipStream_t s);
+hipError_t launch_select(const SelectArgs& a, hipStream_t s);
+hipError_t launch_seen(const SeenArgs& a, hipStream_t s);
 hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s);
 hipError_t launch_topk(int elem, bool keys_only, const TopkArgs& a, hipStream_t s);
 hipError_t launch_merge(int elem, const MergeArgs& a, hipStream_t s);

@@ -4,6 +4,8 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "flat.h"
 
 namespace shine::flat {
@@ -87,10 +89,119 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a, uint32_t 
   }
 }
 
+// ---------------------------------------------------------------------------------------------- products
+// Records are the rows and queries the columns of the matrix instruction, so that a lane's four sums are neighbours of
+// one output row; tile t's rows 4g .. 4g + 3 are records 8g + 4t .. 8g + 4t + 3 of a block of 32, so two tiles give a
+// lane eight neighbours: records 8 (lane / 16) .. + 7 of the block for query lane % 16 of the tile.
+//
+// Rows of at most 256 codes (kStreamPitch): a wave keeps the codes of QT * 16 queries in registers and streams blocks of
+// records past them, so nothing passes through LDS and a record is read once for all of the wave's queries.  The sums
+// start at kMagic: |sum| <= 256 * 127^2 < 2^22, so kMagic + sum read as a float is 1.5 * 2^23 + sum, with no conversion.
+constexpr uint32_t kStreamPitch = 256;
+constexpr int kMagic = 0x4B400000;
+constexpr float kMagicF = 12582912.0f;
+
+template <int KC>
+struct Block {  // a wave's 32 records
+  v4i x[2][KC];
+};
+
+template <int KC>
+__device__ inline void load_block(Block<KC>& b, const int8_t* codes, uint64_t record0, uint64_t n) {
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+  for (int t = 0; t < 2; ++t) {  // rows behind the last one read the last one; nobody uses their sums
+    const uint64_t r = record0 + (col >> 2) * 8 + t * 4 + (col & 3);
+    const int8_t* p = codes + (r < n ? r : n - 1) * (KC * 64) + group * 16;
+    for (int c = 0; c < KC; ++c) b.x[t][c] = *reinterpret_cast<const v4i*>(p + c * 64);
+  }
+}
+
+template <int KC, int QT>
+__device__ inline void load_queries(v4i (&q)[QT][KC], const int8_t* qcodes, uint32_t query0, uint32_t nq) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (int i = 0; i < QT; ++i) {
+    const uint32_t at = query0 + i * 16 + (lane & 15);
+    const int8_t* p = qcodes + static_cast<uint64_t>(at < nq ? at : nq - 1) * (KC * 64) + (lane >> 4) * 16;
+    for (int c = 0; c < KC; ++c) q[i][c] = *reinterpret_cast<const v4i*>(p + c * 64);
+  }
+}
+
+template <int KC>
+__device__ inline void sums(const Block<KC>& b, const v4i (&q)[KC], float (&f)[8]) {
+  for (int t = 0; t < 2; ++t) {
+    v4i acc = {kMagic, kMagic, kMagic, kMagic};
+    for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.x[t][c], q[c], acc, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) f[t * 4 + j] = __int_as_float(acc[j]);
+  }
+}
+
+// Workgroups of one record range and all query blocks run on one XCD (workgroup b runs on XCD b % 8), so that its L2
+// serves the range to all of them.  False: nothing to do.
+struct Place {
+  uint32_t query_block, range;
+};
+__device__ inline Place place_of(uint32_t query_blocks) {
+  const uint32_t xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+  return {i % query_blocks, (i / query_blocks) * 8 + xcd};
+}
+
 // ---------------------------------------------------------------------------------------------- scores
-// out[i][j] = (float(sum_k qc[i][k] * xc[j][k]) * qscale[i]) * scale[j] (+ bias[j]).  Records are the rows and queries
-// the columns of the matrix instruction, so that a lane's four sums are neighbours of one output row; tile t's rows
-// 4g .. 4g + 3 are records 8g + 4t .. 8g + 4t + 3 of a block of 32, so two tiles give a lane eight neighbours.
+// out[i][j] = (float(sum_k qc[i][k] * xc[j][k]) * qscale[i]) * scale[j] (+ bias[j])
+template <class T>
+__device__ inline void store_scores(T* dst, const float (&v)[8], uint64_t left) {
+  if (left >= 8) {
+    constexpr int N = 16 / sizeof(T);
+    for (int h = 0; h < 8 / N; ++h) {
+      Vec<T, N> o;
+      for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>(v[h * N + j]);
+      *reinterpret_cast<Vec<T, N>*>(dst + h * N) = o;
+    }
+  } else {
+    for (uint32_t j = 0; j < left; ++j) dst[j] = from_f32<T>(v[j]);
+  }
+}
+
+template <class T, int KC, int QT>
+__global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per_range) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+  const Place at = place_of(query_blocks);
+  const uint32_t query0 = at.query_block * QT * 16;
+  const uint64_t blocks = (a.n + 31) / 32, b0 = at.range * per_range,
+                 b1 = b0 + per_range < blocks ? b0 + per_range : blocks;
+  if (b0 + wave >= b1) return;
+  v4i q[QT][KC];
+  load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
+  float qs[QT];
+  for (int i = 0; i < QT; ++i) {
+    const uint32_t r = query0 + i * 16 + col;
+    qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
+  }
+  Block<KC> next;
+  load_block<KC>(next, a.codes, (b0 + wave) * 32, a.n);
+  for (uint64_t b = b0 + wave; b < b1; b += 4) {
+    const Block<KC> x = next;
+    if (b + 4 < b1) load_block<KC>(next, a.codes, (b + 4) * 32, a.n);
+    const uint64_t r0 = b * 32 + group * 8;
+    float xs[8], bias[8];
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
+      xs[j] = a.scales[r];
+      bias[j] = a.bias ? a.bias[r] : 0.0f;
+    }
+    for (int i = 0; i < QT; ++i) {
+      float v[8];
+      sums<KC>(x, q[i], v);
+      for (int j = 0; j < 8; ++j) {
+        v[j] = ((v[j] - kMagicF) * qs[i]) * xs[j];
+        if (a.bias) v[j] += bias[j];
+      }
+      const uint32_t row = query0 + i * 16 + col;
+      if (row < a.nq && r0 < a.n) store_scores<T>(static_cast<T*>(a.out) + row * a.ld + r0, v, a.n - r0);
+    }
+  }
+}
+
+// Rows of any width.
 template <class T>
 __global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -100,7 +211,7 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
   const uint32_t col = lane & 15, group = lane >> 4;
   const int8_t* qp[4];
   const int8_t* xp[2];
-  for (int i = 0; i < 4; ++i) {  // rows behind the last one read the last one; their sums are not written
+  for (int i = 0; i < 4; ++i) {
     const uint32_t q = query0 + i * 16 + col;
     qp[i] = a.qcodes + static_cast<uint64_t>(q < a.nq ? q : a.nq - 1) * a.pitch + group * 16;
   }
@@ -118,6 +229,7 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
     }
   }
   const uint64_t r0 = record0 + group * 8;
+  if (r0 >= a.n) return;
   float xs[8], b[8];
   for (int j = 0; j < 8; ++j) {
     const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
@@ -128,13 +240,12 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
     const uint32_t q = query0 + i * 16 + col;
     if (q >= a.nq) continue;
     const float qs = a.qscales[q];
-    T* dst = static_cast<T*>(a.out) + q * a.ld;
+    float v[8];
     for (int j = 0; j < 8; ++j) {
-      if (r0 + j >= a.n) break;
-      float v = (static_cast<float>(acc[i][j >> 2][j & 3]) * qs) * xs[j];
-      if (a.bias) v += b[j];
-      dst[r0 + j] = from_f32<T>(v);
+      v[j] = (static_cast<float>(acc[i][j >> 2][j & 3]) * qs) * xs[j];
+      if (a.bias) v[j] += b[j];
     }
+    store_scores<T>(static_cast<T*>(a.out) + q * a.ld + r0, v, a.n - r0);
   }
 }
 
@@ -322,6 +433,260 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
              a.ids + static_cast<uint64_t>(row) * a.k);
 }
 
+// ---------------------------------------------------------------------------------------------- search
+// The best k of all records without the score matrix.  A pass scores every stride-th block of 32 records and lists, for
+// each query, the keys from its threshold on; the k-th best key of a coarser pass (a lower bound of the k-th best of all
+// records) is the next pass's threshold, the coarsest pass stores all its keys, and the last pass is over all records.
+// A list whose room ends loses nothing but time: its row is scanned again, alone, where the answers are selected.
+
+// The score as shine_flat_scores and then shine_flat_adjust round it.
+__device__ inline float exact_score(float sum, float qs, const PassArgs& a, uint64_t record) {
+  float v = (sum * qs) * a.scales[record];
+  if (a.tbias) v += a.tbias[record];
+  if (a.abias) v += a.abias[record];
+  return v;
+}
+
+__device__ inline uint64_t offered_key(float v, uint64_t record) {
+  return v >= -3.402823466e38f ? key_of(v, static_cast<uint32_t>(record)) : 0;
+}
+
+constexpr uint32_t kListed = 1536;  // keys a workgroup lists in LDS before they go to the queries' lists together
+
+__device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
+  const uint32_t at = atomicAdd(&a.count[query], 1u);
+  if (at < a.cap) a.keys[query * a.cap + at] = key;
+}
+
+// Per score: one fused multiply-add (two with biases) and half a maximum.  (kMagic + sum) * xs - kMagic * xs is sum * xs
+// up to 1.75 xs (the rounding of kMagic * xs is 0.75, the other roundings of numbers below 2^22 xs less than 1), and the
+// definition's own roundings of near-threshold scores are below 2^-20 of the threshold, so scores that reach the
+// threshold also reach it here once 2 qs max(xs) is added.  What passes is scored again as the definition rounds.
+template <int KC, int QT, bool BIAS>
+__global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
+  __shared__ uint64_t list_key[kListed];
+  __shared__ uint32_t list_query[kListed];
+  __shared__ uint32_t listed;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+  const Place at = place_of(query_blocks);
+  const uint32_t query0 = at.query_block * QT * 16;
+  const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
+  if (b0 >= b1) return;  // the whole workgroup
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  v4i q[QT][KC];
+  load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
+  float qs[QT], low[QT];
+  for (int i = 0; i < QT; ++i) {
+    const uint32_t r = query0 + i * 16 + col;
+    qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
+    const float thr = !a.store && r < a.nq && a.thr[r] ? key_value(a.thr[r]) : -__builtin_huge_valf();
+    // scales far from 1 may overflow in one order of products and not in another: everything passes
+    low[i] = qs[i] > 1e-18f && qs[i] < 1e18f ? thr - 0x1p-20f * fabsf(thr) : -__builtin_huge_valf();
+  }
+  Block<KC> next;
+  if (b0 + wave < b1) load_block<KC>(next, a.codes, (b0 + wave) * a.stride * 32, a.n);
+  for (uint64_t b = b0 + wave; b < b1; b += 4) {
+    const Block<KC> x = next;
+    if (b + 4 < b1) load_block<KC>(next, a.codes, (b + 4) * a.stride * 32, a.n);
+    const uint64_t word = b * a.stride, r0 = word * 32 + group * 8;
+    float xs[8], off[8], bias[8], top = 0.0f;
+    bool odd = false;
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
+      xs[j] = a.scales[r];
+      off[j] = -kMagicF * xs[j];
+      top = fmaxf(top, xs[j]);
+      odd |= xs[j] < 1e-18f && xs[j] != 0.0f;
+      if (BIAS) {
+        const float t = a.tbias ? a.tbias[r] : 0.0f, d = a.abias ? a.abias[r] : 0.0f;
+        bias[j] = (t + d) + 0x1p-21f * (fabsf(t) + fabsf(d));
+        if (a.allow && a.allow_ld == 0 && !(a.allow[word] >> (group * 8 + j) & 1u)) bias[j] = -__builtin_huge_valf();
+      }
+    }
+    const float slack = odd || !(top < 1e18f) ? __builtin_huge_valf() : 2.0f * top;
+    for (int i = 0; i < QT; ++i) {
+      float f[8], t[8];
+      sums<KC>(x, q[i], f);
+      for (int j = 0; j < 8; ++j) {
+        t[j] = fmaf(f[j], xs[j], off[j]);
+        t[j] = BIAS ? fmaf(t[j], qs[i], bias[j]) : t[j];
+      }
+      float best = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+      best = BIAS ? fmaf(qs[i], slack, best) : (best + slack) * qs[i];
+      if (best < low[i]) continue;  // a NaN passes and is refused below
+      const uint32_t query = query0 + i * 16 + col;
+      if (query >= a.nq) continue;
+      const uint64_t thr = a.store ? 0 : a.thr[query];
+      const uint32_t allowed = a.allow ? a.allow[query * a.allow_ld + word] >> (group * 8) : 0xFFu;
+      for (int j = 0; j < 8; ++j) {
+        uint64_t key = 0;
+        if (r0 + j < a.n && (allowed >> j & 1u)) key = offered_key(exact_score(f[j] - kMagicF, qs[i], a, r0 + j), r0 + j);
+        if (a.store) {
+          a.keys[query * a.cap + b * 32 + group * 8 + j] = key;
+        } else if (key && key >= thr) {  // the threshold's own record is met again
+          const uint32_t to = atomicAdd(&listed, 1u);
+          if (to < kListed) {
+            list_key[to] = key;
+            list_query[to] = query;
+          } else {
+            append(a, query, key);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t m = listed < kListed ? listed : kListed;
+  for (uint32_t i = threadIdx.x; i < m; i += 256) append(a, list_query[i], list_key[i]);
+}
+
+__device__ inline int dot_codes(const int8_t* x, const v4i* q, uint32_t pitch) {
+  int sum = 0;
+  for (uint32_t c = 0; c < pitch / 16; ++c) {
+    const v4i v = reinterpret_cast<const v4i*>(x)[c], w = q[c];
+    for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_sdot4(v[j], w[j], sum, false);
+  }
+  return sum;
+}
+
+__global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
+  __shared__ Held h;
+  __shared__ v4i query[kMaxFusedPitch / 16];
+  constexpr int N = 4;
+  const PassArgs& p = a.pass;
+  const uint32_t row = blockIdx.x;
+  if (threadIdx.x == 0) {
+    h.count = 0;
+    h.floor = 0;
+  }
+  __syncthreads();
+  const uint64_t listed = a.fixed ? a.fixed : p.count[row];
+  const uint64_t held = listed < p.cap ? listed : p.cap;
+  for (int source = 0; source < 2; ++source) {
+    const uint64_t* src = source ? a.extra + row * a.extra_ld : p.keys + row * p.cap;
+    const uint64_t count = source ? (a.extra ? a.extra_count[row] : 0) : held;
+    for (uint64_t c = 0; c < count; c += 256 * N) {
+      uint64_t key[N];
+      for (int i = 0; i < N; ++i) {
+        const uint64_t at = c + i * 256 + threadIdx.x;
+        key[i] = at < count ? src[at] : 0;
+      }
+      offer(h, a.k, key);
+    }
+  }
+  compact(h, a.k);
+  if (a.thr) {
+    // every thread has read the count: a barrier is behind each of its uses
+    if (threadIdx.x == 0) {
+      a.thr[row] = h.count == a.k ? h.key[a.k - 1] : 0;
+      p.count[row] = 0;
+    }
+    return;
+  }
+  if (listed > p.cap) {
+    // Keys were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
+    // they go, but for the extra ones, which no mask lets through.
+    if (threadIdx.x < p.pitch / 16)
+      query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
+    const uint64_t floor = h.count == a.k ? h.key[a.k - 1] : 0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      h.count = 0;
+      h.floor = floor ? floor - 1 : 0;  // the floor itself is an answer
+    }
+    __syncthreads();
+    const float qs = p.qscales[row];
+    for (uint64_t r0 = 0; r0 < p.n; r0 += 256) {
+      const uint64_t r = r0 + threadIdx.x;
+      uint64_t key[1] = {0};
+      if (r < p.n && (!p.allow || (p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u)))
+        key[0] = offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
+      offer(h, a.k, key);
+    }
+    if (a.extra)
+      for (uint64_t c = 0; c < a.extra_count[row]; c += 256) {
+        uint64_t key[1] = {c + threadIdx.x < a.extra_count[row] ? a.extra[row * a.extra_ld + c + threadIdx.x] : 0};
+        offer(h, a.k, key);
+      }
+    compact(h, a.k);
+  }
+  write_best(h, a.k, a.values + static_cast<uint64_t>(row) * a.k, a.ids + static_cast<uint64_t>(row) * a.k);
+}
+
+// The row's mask without its history: one workgroup per (row, kMaskWords words).
+constexpr uint32_t kMaskWords = 4096;
+__global__ __launch_bounds__(256) void seen_mask_kernel(SeenArgs a) {
+  __shared__ uint32_t mask[kMaskWords];
+  const uint32_t row = blockIdx.y;
+  const uint64_t w0 = static_cast<uint64_t>(blockIdx.x) * kMaskWords;
+  const uint32_t width = static_cast<uint32_t>(a.mask_ld - w0 < kMaskWords ? a.mask_ld - w0 : kMaskWords);
+  for (uint32_t i = threadIdx.x; i < width; i += 256)
+    mask[i] = a.pass.allow ? a.pass.allow[row * a.pass.allow_ld + w0 + i] : 0xFFFFFFFFu;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < a.seen_n; i += 256) {
+    const int32_t id = a.seen[row * a.seen_ld + i];
+    const int64_t w = static_cast<int64_t>(id >> 5) - static_cast<int64_t>(w0);
+    if (id >= 0 && w >= 0 && w < width) atomicAnd(&mask[w], ~(1u << (id & 31)));
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < width; i += 256) a.mask[row * a.mask_ld + w0 + i] = mask[i];
+}
+
+// The history's records, each once: the ids sorted in LDS, a run's length its count.
+__global__ __launch_bounds__(256) void seen_keys_kernel(SeenArgs a) {
+  __shared__ uint32_t ids[kMaxSeen];
+  __shared__ v4i query[kMaxFusedPitch / 16];
+  __shared__ uint32_t count;
+  const PassArgs& p = a.pass;
+  const uint32_t row = blockIdx.x;
+  uint32_t n = 2;
+  while (n < a.seen_n) n <<= 1;
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const int32_t id = i < a.seen_n ? a.seen[row * a.seen_ld + i] : -1;
+    ids[i] = id >= 0 && static_cast<uint64_t>(id) < p.n ? static_cast<uint32_t>(id) : 0xFFFFFFFFu;
+  }
+  if (threadIdx.x < p.pitch / 16)
+    query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  for (uint32_t size = 2; size <= n; size <<= 1)
+    for (uint32_t step = size >> 1; step > 0; step >>= 1) {
+      for (uint32_t i = threadIdx.x; i < n / 2; i += 256) {
+        const uint32_t lo = 2 * step * (i / step) + i % step, hi = lo + step;
+        const uint32_t x = ids[lo], y = ids[hi];
+        if ((x > y) == ((lo & size) == 0)) {
+          ids[lo] = y;
+          ids[hi] = x;
+        }
+      }
+      __syncthreads();
+    }
+  const float qs = p.qscales[row];
+  const float rep = a.repetition ? a.repetition[row] : 1.0f, f = a.frequency ? a.frequency[row] : 0.0f,
+              pres = a.presence ? a.presence[row] : 0.0f;
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const uint32_t id = ids[i];
+    if (id == 0xFFFFFFFFu || (i > 0 && ids[i - 1] == id)) continue;
+    if (p.allow && !(p.allow[row * p.allow_ld + (id >> 5)] >> (id & 31) & 1u)) continue;
+    uint32_t lo = i, hi = n;  // the run's end: ids[lo] == id, ids[hi] > id
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (ids[mid] == id) lo = mid; else hi = mid;
+    }
+    const float times = static_cast<float>(hi - i);
+    const float sum = static_cast<float>(dot_codes(p.codes + static_cast<uint64_t>(id) * p.pitch, query, p.pitch));
+    float v = (sum * qs) * p.scales[id];
+    if (p.tbias) v += p.tbias[id];
+    v = ((v > 0.0f ? v / rep : v * rep) - f * times) - pres;
+    if (p.abias) v += p.abias[id];
+    const uint64_t key = offered_key(v, id);
+    if (key) a.extra[row * a.extra_ld + atomicAdd(&count, 1u)] = key;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) a.extra_count[row] = count;
+}
+
 }  // namespace
 
 #define SHINE_BY_ELEM(elem, CALL)                 \
@@ -343,9 +708,78 @@ hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+namespace {
+// Ranges of blocks for a streaming launch: about `want` workgroups in all, whole ranges a multiple of 8 (one per XCD).
+struct Ranges {
+  uint64_t per;
+  uint32_t grid;
+};
+Ranges ranges_of(uint64_t blocks, uint32_t query_blocks, uint32_t want) {
+  uint64_t ranges = std::max<uint64_t>(1, want / query_blocks);
+  ranges = std::min(ranges, (blocks + 3) / 4);  // four waves take a block each
+  const uint64_t per = (blocks + ranges - 1) / ranges;
+  const uint64_t whole = ((blocks + per - 1) / per + 7) / 8 * 8;
+  return {per, static_cast<uint32_t>(whole * query_blocks)};
+}
+}  // namespace
+
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
+  if (a.pitch <= kStreamPitch) {
+#define SHINE_STREAM(KK, QQ)                                                                              \
+  {                                                                                                       \
+    const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                 \
+    const Ranges r = ranges_of((a.n + 31) / 32, qb, 2048);                                                \
+    hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);   \
+  }
+#define SHINE_KC(KK, BIG) \
+  if (a.nq <= 16) SHINE_STREAM(KK, 1) else if (a.nq <= 32) SHINE_STREAM(KK, 2) else SHINE_STREAM(KK, BIG)
+    SHINE_BY_ELEM(out_elem, switch (a.pitch / 64) {
+      case 1: SHINE_KC(1, 8); break;
+      case 2: SHINE_KC(2, 8); break;
+      case 3: SHINE_KC(3, 4); break;
+      default: SHINE_KC(4, 4); break;
+    });
+#undef SHINE_KC
+#undef SHINE_STREAM
+    return hipGetLastError();
+  }
   const dim3 grid(static_cast<uint32_t>((a.n + 127) / 128), (a.nq + 63) / 64);
   SHINE_BY_ELEM(out_elem, hipLaunchKernelGGL(scores_kernel<T>, grid, dim3(256), 0, s, a));
+  return hipGetLastError();
+}
+
+hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
+  const bool bias = a.tbias || a.abias || (a.allow && a.allow_ld == 0);
+#define SHINE_PASS(KK, QQ)                                                                                 \
+  {                                                                                                        \
+    const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                  \
+    const Ranges r = ranges_of(a.blocks, qb, 1024);                                                        \
+    if (bias) hipLaunchKernelGGL((pass_kernel<KK, QQ, true>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per); \
+    else hipLaunchKernelGGL((pass_kernel<KK, QQ, false>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);     \
+  }
+#define SHINE_KC(KK, BIG) \
+  if (a.nq <= 32) SHINE_PASS(KK, 2) else SHINE_PASS(KK, BIG)
+  switch (a.pitch / 64) {
+    case 1: SHINE_KC(1, 8); break;
+    case 2: SHINE_KC(2, 8); break;
+    case 3: SHINE_KC(3, 4); break;
+    case 4: SHINE_KC(4, 4); break;
+    default: return hipErrorInvalidValue;
+  }
+#undef SHINE_KC
+#undef SHINE_PASS
+  return hipGetLastError();
+}
+
+hipError_t launch_select(const SelectArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(select_kernel, dim3(a.pass.nq), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_seen(const SeenArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>((a.mask_ld + kMaskWords - 1) / kMaskWords), a.pass.nq);
+  hipLaunchKernelGGL(seen_mask_kernel, grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL(seen_keys_kernel, dim3(a.pass.nq), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -232,7 +232,7 @@ PROTOTYPES = {
     "shine_flat_adjust": (I32, [I32, P, I32, U32, U64, U64, C.POINTER(FlatAdjustment), P, U64, P]),
     "shine_flat_topk_workspace": (U64, [U32, U64, U32]),
     "shine_flat_topk": (I32, [I32, P, I32, U32, U64, U64, U32, P, P, P, U64, P]),
-    "shine_flat_search_workspace": (U64, [U32, U64, U32, U32]),
+    "shine_flat_search_workspace": (U64, [U32, U64, U32, U32, C.POINTER(FlatAdjustment)]),
     "shine_flat_search": (I32, [I32, C.POINTER(FlatTable), P, I32, U32, U64, U32, C.POINTER(FlatAdjustment), P, P, P,
                                 U64, P]),
 }

@@ -239,7 +239,7 @@ def search(table: FlatTable, queries, k: int, bias=None, allow=None, seen=None, 
     values = torch.empty((nq, k), dtype=torch.float32, device=device)
     ids = torch.empty((nq, k), dtype=torch.int32, device=device)
     lib = L.lib()
-    size = lib.shine_flat_search_workspace(nq, table.n, table.dim, k)
+    size = lib.shine_flat_search_workspace(nq, table.n, table.dim, k, a)
     ws = _workspace(size, device)
     L.check(lib.shine_flat_search(device.index, C.byref(table._c), ptr, elem, nq, ld, k, a, values.data_ptr(),
                                   ids.data_ptr(), ws.data_ptr() if size else None, size, _stream(device)))

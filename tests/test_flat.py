@@ -37,7 +37,7 @@ def test_pitch_and_workspaces():
     for dim, pitch in ((1, 64), (64, 64), (65, 128), (96, 128), (200, 256), (16384, 16384)):
         assert lib.shine_flat_pitch(dim) == pitch == flat.code_pitch(dim)
     assert lib.shine_flat_scores_workspace(7, 96) >= 7 * 128 + 7 * 4
-    assert lib.shine_flat_search_workspace(7, 1000, 96, 10) >= 7 * 128 + 7 * 4
+    assert lib.shine_flat_search_workspace(7, 1000, 96, 10, None) >= 7 * 128 + 7 * 4
 
 
 def test_quantize_refusals():
@@ -121,7 +121,7 @@ def test_search_refusals():
     refused(f(0, table(), P, 0, 4, 32, 10, None, None, P, P, big, None), "NULL")
     refused(f(0, table(), P, 0, 4, 32, 10, None, P, P + 2, P, big, None), "aligned")
     refused(f(0, table(), P, 0, 4, 32, 10, None, P, P, None, big, None), "workspace")
-    need = L.lib().shine_flat_search_workspace(4, 100, 32, 10)
+    need = L.lib().shine_flat_search_workspace(4, 100, 32, 10, None)
     refused(f(0, table(), P, 0, 4, 32, 10, None, P, P, P, need - 1, None), "workspace")
     assert f(0, table(), None, 0, 0, 32, 10, None, None, None, None, 0, None) == L.OK
 

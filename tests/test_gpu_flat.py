@@ -468,13 +468,72 @@ def test_search_of_sorted_records():
         assert torch.equal(ids.cpu(), want_i) and torch.equal(values.cpu(), want_v)
 
 
+@pytest.mark.parametrize("k", [1, 10, 256])
+@pytest.mark.parametrize("n,every", [(30000, 8), (30000, 4), (270000, 9)])
+def test_search_when_a_sample_misses_the_best(n, every, k):
+    """Every `every`-th block of 32 records is poor: a threshold taken there lets nearly all others through."""
+    x = rows(n, 32, 5) * 0.1
+    x[:, 0] = torch.where((torch.arange(n) // 32) % every == 0, -1.0, 1.0)
+    q = rows(33, 32, 6) * 0.1
+    q[:, 0] = 1
+    q[1] = -q[1]
+    a = adjustments(33, n, 3, 40, "shared", "rows")
+    flat = F()
+    table = flat.FlatTable(x.cuda())
+    values, ids = flat.search(table, q.cuda(), k)
+    want_v, want_i = topk_plain(scores32(x, q, "ip"), k)
+    assert torch.equal(ids.cpu(), want_i) and torch.equal(values.cpu(), want_v)
+    values, ids = flat.search(table, q.cuda(), k, **cuda(a))
+    v, i = flat.topk(flat.adjust(flat.scores(table, q.cuda()), **cuda(a)), k)
+    assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+@pytest.mark.parametrize("n", [8193, 131072, 400001])
+def test_search_of_many_records(n):
+    """more passes, a mask that leaves some rows few records and one row none"""
+    x, q = rows(n, 48, 7), rows(40, 48, 8)
+    a = adjustments(40, n, 3, 100, "shared", "rows")
+    a["allow"][3] = 0
+    a["allow"][4, 1:] = 0
+    a["allow"][5, 50:-50] = 0
+    flat = F()
+    for metric in ("ip", "l2"):
+        table = flat.FlatTable(x.cuda(), metric=metric)
+        s = flat.scores(table, q.cuda())
+        assert torch.equal(s.cpu(), scores32(x, q, metric))
+        for k in (1, 64, 65, 200):
+            for some in ([], ["allow"], ["allow", "bias"], list(a)):
+                b = {key: a[key].cuda() for key in some}
+                values, ids = flat.search(table, q.cuda(), k, **b)
+                v, i = flat.topk(flat.adjust(s, **b), k)
+                assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+def test_search_with_scales_far_apart():
+    """products that overflow or vanish in one order of multiplication: the answers are those of the scores"""
+    x, q = rows(9000, 32, 7), rows(40, 32, 8)
+    x *= 10.0 ** torch.linspace(-30, 30, 9000)[torch.randperm(9000, generator=torch.Generator().manual_seed(1))][:, None]
+    q *= 10.0 ** torch.linspace(-37, 37, 40)[:, None]
+    x[5], q[7] = 0, 0
+    flat = F()
+    for metric in ("ip", "l2"):
+        table = flat.FlatTable(x.cuda(), metric=metric)
+        s = flat.scores(table, q.cuda())
+        for k in (10, 200):
+            values, ids = flat.search(table, q.cuda(), k)
+            v, i = flat.topk(s, k)
+            assert torch.equal(ids, i) and torch.equal(values, v)
+
+
 def test_search_with_records_and_queries_without_a_scale():
-    x, q = rows(500, 32, 3), rows(4, 32, 4)
-    x[7, 3], x[450, 0] = math.nan, math.inf
-    q[2, 1] = math.nan
-    values, ids = F().search(F().FlatTable(x.cuda()), q.cuda(), 256)
-    assert (ids[2] == -1).all()
-    assert not ((ids == 7) | (ids == 450)).any() and (ids[[0, 1, 3]] >= 0).all() and values[[0, 1, 3]].isfinite().all()
+    for nq, n in ((4, 500), (40, 500), (40, 20000)):
+        x, q = rows(n, 32, 3), rows(nq, 32, 4)
+        x[7, 3], x[450, 0] = math.nan, math.inf
+        q[2, 1] = math.nan
+        values, ids = F().search(F().FlatTable(x.cuda()), q.cuda(), 256)
+        rest = [i for i in range(nq) if i != 2]
+        assert (ids[2] == -1).all()
+        assert not ((ids == 7) | (ids == 450)).any() and (ids[rest] >= 0).all() and values[rest].isfinite().all()
 
 
 def test_empty_tables_and_batches():
