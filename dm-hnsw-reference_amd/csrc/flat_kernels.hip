@@ -51,38 +51,77 @@ __device__ inline int code_of(float x, float scale, float inv) {
   return static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f));
 }
 
-// One group of G lanes per row, 8 components a lane and step.
-template <class T, int G>
+// V = 16 bytes of components that a lane takes in a step; components behind dim are 0
+template <class T, int V>
+__device__ inline void load_components(float (&x)[V], const T* src, uint32_t c, uint32_t dim) {
+  if (c + V <= dim) {
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(src + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = to_f32(v.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = c + i < dim ? to_f32(src[c + i]) : 0.0f;
+  }
+}
+
+// G lanes per row and S steps of 16 bytes a lane, held in registers between the maximum and the codes (S = 0: rows too wide
+// for that are read twice).
+template <class T, int G, int S>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a, uint32_t pitch) {
+  constexpr int V = 16 / sizeof(T), H = S ? S : 1;
   const uint32_t lane = threadIdx.x % G;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (256 / G) + threadIdx.x / G;
   if (row >= a.n) return;
   const T* src = static_cast<const T*>(a.rows) + row * a.ld;
+  float x[H][V];
   uint32_t top = 0;
-  for (uint32_t c = lane * 8; c < a.dim; c += G * 8)
-    for (uint32_t i = c; i < c + 8 && i < a.dim; ++i) {
-      const uint32_t bits = __float_as_uint(to_f32(src[i])) & 0x7FFFFFFFu;
-      top = bits > top ? bits : top;
+  auto raise = [&top](const float(&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  };
+  if (S) {
+#pragma unroll
+    for (int j = 0; j < H; ++j) load_components<T, V>(x[j], src, (j * G + lane) * V, a.dim);
+#pragma unroll
+    for (int j = 0; j < H; ++j) raise(x[j]);
+  } else {
+    for (uint32_t c = lane * V; c < a.dim; c += G * V) {
+      load_components<T, V>(x[0], src, c, a.dim);
+      raise(x[0]);
     }
-  for (int o = G / 2; o > 0; o >>= 1) {
-    const uint32_t other = __shfl_xor(top, o, G);
-    top = other > top ? other : top;
   }
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, G)));
   const bool finite = top < 0x7F800000u;
   const float scale = finite ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7FC00000u);
+  const bool some = finite && scale > 0.0f;
   const float inv = 1.0f / scale;
   int squares = 0;
-  for (uint32_t c = lane * 8; c < pitch; c += G * 8) {
-    uint64_t packed = 0;
-    for (uint32_t i = 0; i < 8; ++i) {
-      int code = 0;
-      if (c + i < a.dim && finite && scale > 0.0f) code = code_of(to_f32(src[c + i]), scale, inv);
+  auto write = [&](const float(&v)[V], uint32_t c) {
+    uint32_t packed[V / 4] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int code = some ? code_of(v[i], scale, inv) : 0;
       squares += code * code;
-      packed |= static_cast<uint64_t>(static_cast<uint8_t>(code)) << (8 * i);
+      packed[i / 4] |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * (i % 4));
     }
-    *reinterpret_cast<uint64_t*>(a.codes + row * pitch + c) = packed;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.codes + row * pitch + c);
+    if (V == 4) *dst = packed[0];
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[V / 4 - 1]);
+  };
+  if (S) {
+#pragma unroll
+    for (int j = 0; j < H; ++j)
+      if ((j * G + lane) * V < pitch) write(x[j], (j * G + lane) * V);
+  } else {
+    for (uint32_t c = lane * V; c < pitch; c += G * V) {
+      load_components<T, V>(x[0], src, c, a.dim);
+      write(x[0], c);
+    }
   }
-  for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
+  if (a.half_norms)
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
   if (lane == 0) {
     a.scales[row] = scale;
     if (a.half_norms) a.half_norms[row] = -0.5f * ((static_cast<float>(squares) * scale) * scale);
@@ -109,9 +148,11 @@ struct Block {  // a wave's 32 records
 template <int KC>
 __device__ inline void load_block(Block<KC>& b, const int8_t* codes, uint64_t record0, uint64_t n) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+#pragma unroll
   for (int t = 0; t < 2; ++t) {  // rows behind the last one read the last one; nobody uses their sums
     const uint64_t r = record0 + (col >> 2) * 8 + t * 4 + (col & 3);
     const int8_t* p = codes + (r < n ? r : n - 1) * (KC * 64) + group * 16;
+#pragma unroll
     for (int c = 0; c < KC; ++c) b.x[t][c] = *reinterpret_cast<const v4i*>(p + c * 64);
   }
 }
@@ -119,18 +160,23 @@ __device__ inline void load_block(Block<KC>& b, const int8_t* codes, uint64_t re
 template <int KC, int QT>
 __device__ inline void load_queries(v4i (&q)[QT][KC], const int8_t* qcodes, uint32_t query0, uint32_t nq) {
   const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t at = query0 + i * 16 + (lane & 15);
     const int8_t* p = qcodes + static_cast<uint64_t>(at < nq ? at : nq - 1) * (KC * 64) + (lane >> 4) * 16;
+#pragma unroll
     for (int c = 0; c < KC; ++c) q[i][c] = *reinterpret_cast<const v4i*>(p + c * 64);
   }
 }
 
 template <int KC>
 __device__ inline void sums(const Block<KC>& b, const v4i (&q)[KC], float (&f)[8]) {
+#pragma unroll
   for (int t = 0; t < 2; ++t) {
     v4i acc = {kMagic, kMagic, kMagic, kMagic};
+#pragma unroll
     for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.x[t][c], q[c], acc, 0, 0, 0);
+#pragma unroll
     for (int j = 0; j < 4; ++j) f[t * 4 + j] = __int_as_float(acc[j]);
   }
 }
@@ -172,6 +218,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
   v4i q[QT][KC];
   load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   float qs[QT];
+#pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t r = query0 + i * 16 + col;
     qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
@@ -188,9 +235,11 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
       xs[j] = a.scales[r];
       bias[j] = a.bias ? a.bias[r] : 0.0f;
     }
+#pragma unroll
     for (int i = 0; i < QT; ++i) {
       float v[8];
       sums<KC>(x, q[i], v);
+#pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = ((v[j] - kMagicF) * qs[i]) * xs[j];
         if (a.bias) v[j] += bias[j];
@@ -250,24 +299,26 @@ __global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- adjust
-// One workgroup per (row, kTile columns): the row's history is counted into LDS for the tile's columns (integer
-// additions: any order gives the same counts), then every column is read, changed and written once.
-constexpr uint32_t kTile = 4096;
-
-template <class T>
+// One workgroup per (row, TILE columns): the row's history is counted into LDS for the tile's columns (integer
+// additions: any order gives the same counts), then every column is read, changed and written once, 16 bytes a lane.
+// Tiles start at multiples of 32 records, so a lane's columns share a word of allowed bits.
+template <class T, int TILE>
 __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
-  __shared__ uint32_t count[kTile];
+  constexpr int V = 16 / sizeof(T);
+  __shared__ uint32_t count[TILE];
   const uint32_t row = blockIdx.y;
-  const uint64_t c0 = static_cast<uint64_t>(blockIdx.x) * kTile;
-  const uint32_t width = static_cast<uint32_t>(a.n - c0 < kTile ? a.n - c0 : kTile);
+  const uint64_t c0 = static_cast<uint64_t>(blockIdx.x) * TILE;
+  const uint32_t width = static_cast<uint32_t>(a.n - c0 < TILE ? a.n - c0 : TILE);
   const bool history = a.seen && a.seen_n;
   if (history) {
-    for (uint32_t i = threadIdx.x; i < width; i += 256) count[i] = 0;
+    for (uint32_t i = threadIdx.x * 4; i < TILE; i += 1024) *reinterpret_cast<uint4*>(&count[i]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int32_t* seen = a.seen + row * a.seen_ld;
+    const int64_t from = static_cast<int64_t>(a.first + c0);
     for (uint32_t i = threadIdx.x; i < a.seen_n; i += 256) {
-      const int64_t at = static_cast<int64_t>(seen[i]) - static_cast<int64_t>(a.first + c0);
-      if (seen[i] >= 0 && at >= 0 && at < width) atomicAdd(&count[at], 1u);
+      const int32_t id = seen[i];
+      const int64_t at = id - from;
+      if (id >= 0 && at >= 0 && at < width) atomicAdd(&count[at], 1u);
     }
     __syncthreads();
   }
@@ -275,13 +326,33 @@ __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
               p = a.presence ? a.presence[row] : 0.0f;
   const T* src = static_cast<const T*>(a.scores) + row * a.ld + c0;
   T* dst = static_cast<T*>(a.out) + row * a.out_ld + c0;
-  for (uint32_t i = threadIdx.x; i < width; i += 256) {
-    const uint64_t record = a.first + c0 + i;
-    float v = to_f32(src[i]);
-    if (history && count[i]) v = ((v > 0.0f ? v / r : v * r) - f * static_cast<float>(count[i])) - p;
-    if (a.bias) v += a.bias[row * a.bias_ld + record];
-    if (a.allow && !((a.allow[row * a.allow_ld + (record >> 5)] >> (record & 31)) & 1u)) v = -__builtin_huge_valf();
-    dst[i] = from_f32<T>(v);
+  const float* bias = a.bias ? a.bias + row * a.bias_ld + a.first + c0 : nullptr;
+  const uint32_t* allow = a.allow ? a.allow + row * a.allow_ld + ((a.first + c0) >> 5) : nullptr;
+  auto change = [&](float v, uint32_t times, float b, bool on) {
+    if (times) v = ((v > 0.0f ? v / r : v * r) - f * static_cast<float>(times)) - p;
+    if (bias) v += b;
+    return on ? v : -__builtin_huge_valf();
+  };
+#pragma unroll 2
+  for (uint32_t i = threadIdx.x * V; i < width; i += 256 * V) {
+    const uint32_t on = allow ? allow[i >> 5] >> (i & 31) : ~0u;
+    if (i + V <= width) {
+      Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src + i);
+      Vec<float, V> b{};
+      if (bias) b = *reinterpret_cast<const Vec<float, V>*>(bias + i);
+      uint32_t c[V] = {};
+      if (history)
+        for (int j = 0; j < V; j += 4) {
+          const uint4 w = *reinterpret_cast<const uint4*>(&count[i + j]);
+          c[j] = w.x, c[j + 1] = w.y, c[j + 2] = w.z, c[j + 3] = w.w;
+        }
+#pragma unroll
+      for (int j = 0; j < V; ++j) x.v[j] = from_f32<T>(change(to_f32(x.v[j]), c[j], b.v[j], on >> j & 1u));
+      *reinterpret_cast<Vec<T, V>*>(dst + i) = x;
+    } else {
+      for (uint32_t j = 0; i + j < width; ++j)
+        dst[i + j] = from_f32<T>(change(to_f32(src[i + j]), history ? count[i + j] : 0, bias ? bias[i + j] : 0.0f, on >> j & 1u));
+    }
   }
 }
 
@@ -301,20 +372,52 @@ __device__ inline int32_t key_id(uint64_t key) {
   return static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
 }
 
-constexpr uint32_t kKeys = 1024;  // keys a workgroup holds: k of them kept, the rest room for newer ones
+// A workgroup of 256 threads holds up to kKeys keys and a floor below which nothing can be an answer.  The floor comes from
+// maxima: of 256 keys, one of each thread's share, the k-th largest is no larger than the k-th largest of all, so counting for
+// each of the 256 how many are larger (256 comparisons a thread, about 1 us) raises the floor without sorting anything: of
+// 4,096 random keys about k (1 + k / 512) pass it.
+constexpr uint32_t kKeys = 1024;
 
 struct Held {
   uint64_t key[kKeys];
+  uint32_t top[256];
   uint32_t count;
-  uint64_t floor;  // the k-th best key held when the room last ran out: smaller keys are no answers
+  uint64_t floor;  // keys up to it are no answers, but for those held
 };
+
+__device__ inline void begin(Held& h, uint64_t floor = 0) {
+  if (threadIdx.x == 0) {
+    h.count = 0;
+    h.floor = floor;
+  }
+  __syncthreads();
+}
+
+// `order`: the high word of the largest key of the thread's share.  The low 8 bits give way to the thread's number, so
+// that all 256 differ.  Ends with a barrier.
+__device__ inline void raise_floor(Held& h, uint32_t order, uint32_t k) {
+  const uint32_t mine = (order & ~255u) | threadIdx.x;
+  h.top[threadIdx.x] = mine;
+  __syncthreads();
+  uint32_t larger = 0;
+#pragma unroll 8
+  for (uint32_t i = 0; i < 64; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(h.top)[i];
+    larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+  }
+  if (larger == k - 1) {
+    const uint64_t floor = static_cast<uint64_t>(mine & ~255u) << 32;
+    if (floor > h.floor) h.floor = floor;
+  }
+  __syncthreads();
+}
 
 // descending, over the first n (a power of two) keys
 __device__ inline void sort_keys(uint64_t* key, uint32_t n) {
   for (uint32_t size = 2; size <= n; size <<= 1)
     for (uint32_t step = size >> 1; step > 0; step >>= 1) {
-      for (uint32_t i = threadIdx.x; i < n / 2; i += blockDim.x) {
-        const uint32_t lo = 2 * step * (i / step) + i % step, hi = lo + step;
+      for (uint32_t i = threadIdx.x; i < n / 2; i += 256) {
+        const uint32_t lo = 2 * i - (i & (step - 1)), hi = lo + step;
         const bool up = (lo & size) != 0;
         const uint64_t x = key[lo], y = key[hi];
         if ((x < y) != up) {
@@ -326,43 +429,91 @@ __device__ inline void sort_keys(uint64_t* key, uint32_t n) {
     }
 }
 
-// Sorts what is held and keeps the best k.  All threads call it, behind a barrier; it ends with one.
-__device__ inline void compact(Held& h, uint32_t k) {
+// Makes room: raises the floor from what is held and drops what does not pass.  Where that leaves more than half (k near
+// 256, many equal values, all the best in one thread's share), sorts and keeps the best k.  All threads call it behind a
+// barrier; it ends with one.
+__device__ inline void make_room(Held& h, uint32_t k) {
   const uint32_t held = h.count < kKeys ? h.count : kKeys;
-  uint32_t n = 2;
-  while (n < held) n <<= 1;
-  for (uint32_t i = held + threadIdx.x; i < n; i += blockDim.x) h.key[i] = 0;
+  uint64_t key[kKeys / 256];
+  uint64_t best = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kKeys / 256; ++i) {
+    const uint32_t at = i * 256 + threadIdx.x;
+    key[i] = at < held ? h.key[at] : 0;
+    best = key[i] > best ? key[i] : best;
+  }
+  raise_floor(h, static_cast<uint32_t>(best >> 32), k);
+  if (threadIdx.x == 0) h.count = 0;
   __syncthreads();
-  sort_keys(h.key, n);
+  const uint64_t floor = h.floor;
+#pragma unroll
+  for (uint32_t i = 0; i < kKeys / 256; ++i)
+    if (key[i] > floor || (key[i] && key[i] == floor)) h.key[atomicAdd(&h.count, 1u)] = key[i];
+  __syncthreads();
+  const uint32_t left = h.count;
+  if (left <= kKeys / 2) return;
+  for (uint32_t i = left + threadIdx.x; i < kKeys; i += 256) h.key[i] = 0;
+  __syncthreads();
+  sort_keys(h.key, kKeys);
   if (threadIdx.x == 0) {
-    h.count = held < k ? held : k;
-    if (held >= k) h.floor = h.key[k - 1];
+    h.count = left < k ? left : k;
+    if (left >= k) h.floor = h.key[k - 1];
   }
   __syncthreads();
 }
 
-// Offers each thread's N keys (0: none).  Keys that found no room are offered again behind a compaction, which leaves
-// kKeys - k places, so every turn of the loop places some and it ends.
+// The answers: the best k of what is held, in order.  Ends with a barrier.
+__device__ inline void finish(Held& h, uint32_t k) {
+  if (h.count > 256) make_room(h, k);
+  const uint32_t held = h.count;
+  if (held <= 256) {  // each key's place is the number of larger ones
+    const uint64_t mine = threadIdx.x < held ? h.key[threadIdx.x] : 0;
+    uint32_t place = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < held; ++i) place += h.key[i] > mine;
+    __syncthreads();
+    if (threadIdx.x < held) h.key[place] = mine;
+  } else {
+    for (uint32_t i = held + threadIdx.x; i < kKeys; i += 256) h.key[i] = 0;
+    __syncthreads();
+    sort_keys(h.key, kKeys);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) h.count = held < k ? held : k;
+  __syncthreads();
+}
+
+// Offers each thread's N keys (0: none).  Keys that found no room are offered again behind make_room, which leaves half
+// of it, so every turn of the loop places some and it ends.  `first`: raise the floor from them before.
 template <int N>
-__device__ inline void offer(Held& h, uint32_t k, const uint64_t (&key)[N]) {
+__device__ inline void offer(Held& h, uint32_t k, const uint64_t (&key)[N], bool first) {
+  if (first) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = key[i] > best ? key[i] : best;
+    raise_floor(h, static_cast<uint32_t>(best >> 32), k);
+  }
   uint32_t pending = 0;
-  for (int i = 0; i < N; ++i)
-    if (key[i] > h.floor) pending |= 1u << i;
+  uint64_t floor = h.floor;
+#pragma unroll
+  for (int i = 0; i < N; ++i) pending |= (key[i] > floor ? 1u : 0u) << i;
   for (;;) {
-    for (int i = 0; i < N; ++i)
-      if (pending >> i & 1u) {
-        if (key[i] <= h.floor) {
-          pending &= ~(1u << i);
-        } else {
-          const uint32_t at = atomicAdd(&h.count, 1u);
-          if (at < kKeys) {
-            h.key[at] = key[i];
-            pending &= ~(1u << i);
+    if (pending) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (pending >> i & 1u) {
+          bool settled = key[i] <= floor;
+          if (!settled) {
+            const uint32_t at = atomicAdd(&h.count, 1u);
+            settled = at < kKeys;
+            if (settled) h.key[at] = key[i];
           }
+          if (settled) pending &= ~(1u << i);
         }
-      }
+    }
     if (!__syncthreads_or(pending != 0)) return;
-    compact(h, k);
+    make_room(h, k);
+    floor = h.floor;
   }
 }
 
@@ -378,28 +529,56 @@ __device__ inline void write_best(const Held& h, uint32_t k, T* values, int32_t*
 template <class T>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
   __shared__ Held h;
-  constexpr int N = 8;
+  constexpr int V = 16 / sizeof(T), N = 16;  // values of a load, of a thread and turn
   const uint32_t row = blockIdx.y, slice = blockIdx.x;
-  if (threadIdx.x == 0) {
-    h.count = 0;
-    h.floor = 0;
-  }
-  __syncthreads();
+  begin(h);
   const T* src = static_cast<const T*>(a.scores) + row * a.ld;
   const uint64_t per = (a.n + a.slices - 1) / a.slices, c0 = slice * per, c1 = c0 + per < a.n ? c0 + per : a.n;
   for (uint64_t c = c0; c < c1; c += 256 * N) {
-    uint64_t key[N];
-    for (int i = 0; i < N; ++i) {
-      const uint64_t at = c + i * 256 + threadIdx.x;
-      key[i] = 0;
-      if (at < c1) {
-        const float v = to_f32(src[at]);
-        if (v >= -3.402823466e38f) key[i] = key_of(v, static_cast<uint32_t>(a.first + at));
+    float v[N];
+    float best = -__builtin_huge_valf();
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+      const uint64_t at = c + i * 256 + threadIdx.x * V;
+      if (at + V <= c1) {
+        const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src + at);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i + j] = to_f32(x.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i + j] = at + j < c1 ? to_f32(src[at + j]) : -__builtin_huge_valf();
       }
     }
-    offer(h, a.k, key);
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = fmaxf(best, v[i]);  // a NaN is no maximum
+    if (c == c0) raise_floor(h, best >= -3.402823466e38f ? static_cast<uint32_t>(key_of(best, 0) >> 32) : 0, a.k);
+    uint64_t floor = h.floor;
+    float low = floor ? key_value(floor) : -3.402823466e38f;
+    uint32_t pending = 0;
+    if (best >= low)
+#pragma unroll
+      for (int i = 0; i < N; ++i) pending |= (v[i] >= low ? 1u : 0u) << i;
+    for (;;) {  // as offer() does
+      if (pending) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (pending >> i & 1u) {
+            const uint64_t key = key_of(v[i], static_cast<uint32_t>(a.first + c + (i / V) * V * 256 + threadIdx.x * V + i % V));
+            bool settled = key <= floor;
+            if (!settled) {
+              const uint32_t at = atomicAdd(&h.count, 1u);
+              settled = at < kKeys;
+              if (settled) h.key[at] = key;
+            }
+            if (settled) pending &= ~(1u << i);
+          }
+      }
+      if (!__syncthreads_or(pending != 0)) break;
+      make_room(h, a.k);
+      floor = h.floor;
+    }
   }
-  compact(h, a.k);
+  finish(h, a.k);
   if (to_keys) {
     uint64_t* out = a.keys + (static_cast<uint64_t>(row) * a.key_ld + slice) * a.k;
     for (uint32_t i = threadIdx.x; i < a.k; i += 256) out[i] = i < h.count ? h.key[i] : 0;
@@ -409,26 +588,27 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
   }
 }
 
+// All threads call it behind a barrier.
+__device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* src, uint64_t count) {
+  constexpr int N = 8;
+  for (uint64_t c = 0; c < count; c += 256 * N) {
+    uint64_t key[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t at = c + i * 256 + threadIdx.x;
+      key[i] = at < count ? src[at] : 0;
+    }
+    offer(h, k, key, c == 0);
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
   __shared__ Held h;
-  constexpr int N = 4;
   const uint32_t row = blockIdx.x;
-  if (threadIdx.x == 0) {
-    h.count = 0;
-    h.floor = 0;
-  }
-  __syncthreads();
-  const uint64_t* src = a.keys + row * a.count;
-  for (uint64_t c = 0; c < a.count; c += 256 * N) {
-    uint64_t key[N];
-    for (int i = 0; i < N; ++i) {
-      const uint64_t at = c + i * 256 + threadIdx.x;
-      key[i] = at < a.count ? src[at] : 0;
-    }
-    offer(h, a.k, key);
-  }
-  compact(h, a.k);
+  begin(h);
+  offer_list(h, a.k, a.keys + row * a.count, a.count);
+  finish(h, a.k);
   write_best(h, a.k, static_cast<T*>(a.values) + static_cast<uint64_t>(row) * a.k,
              a.ids + static_cast<uint64_t>(row) * a.k);
 }
@@ -477,6 +657,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   v4i q[QT][KC];
   load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   float qs[QT], low[QT];
+#pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t r = query0 + i * 16 + col;
     qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
@@ -505,32 +686,48 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
       }
     }
     const float slack = odd || !(top < 1e18f) ? __builtin_huge_valf() : 2.0f * top;
+#pragma unroll
     for (int i = 0; i < QT; ++i) {
       float f[8], t[8];
       sums<KC>(x, q[i], f);
+#pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[j] = fmaf(f[j], xs[j], off[j]);
         t[j] = BIAS ? fmaf(t[j], qs[i], bias[j]) : t[j];
       }
       float best = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
       best = BIAS ? fmaf(qs[i], slack, best) : (best + slack) * qs[i];
-      if (best < low[i]) continue;  // a NaN passes and is refused below
-      const uint32_t query = query0 + i * 16 + col;
-      if (query >= a.nq) continue;
-      const uint64_t thr = a.store ? 0 : a.thr[query];
-      const uint32_t allowed = a.allow ? a.allow[query * a.allow_ld + word] >> (group * 8) : 0xFFu;
-      for (int j = 0; j < 8; ++j) {
-        uint64_t key = 0;
-        if (r0 + j < a.n && (allowed >> j & 1u)) key = offered_key(exact_score(f[j] - kMagicF, qs[i], a, r0 + j), r0 + j);
-        if (a.store) {
-          a.keys[query * a.cap + b * 32 + group * 8 + j] = key;
-        } else if (key && key >= thr) {  // the threshold's own record is met again
-          const uint32_t to = atomicAdd(&listed, 1u);
-          if (to < kListed) {
-            list_key[to] = key;
-            list_query[to] = query;
-          } else {
-            append(a, query, key);
+      if (!(best < low[i])) {  // a NaN passes and is refused below
+        const uint32_t query = query0 + i * 16 + col;
+        uint32_t maybe = query < a.nq ? 0xFFu : 0u;
+        if (maybe && a.allow) maybe &= a.allow[query * a.allow_ld + word] >> (group * 8);
+        if (r0 + 8 > a.n) maybe &= r0 < a.n ? 0xFFu >> (8 - (a.n - r0)) : 0u;
+        const uint64_t thr = !a.store && maybe ? a.thr[query] : 0;
+        if (a.store && query < a.nq) {
+          uint64_t* to = a.keys + query * a.cap + b * 32 + group * 8;
+          for (uint32_t j = 0; j < 8; ++j) to[j] = 0;
+        }
+        while (maybe) {
+          const uint32_t j = __builtin_ctz(maybe);
+          maybe &= maybe - 1;
+          float sum = f[0], rough = t[0];
+#pragma unroll
+          for (uint32_t e = 1; e < 8; ++e) {
+            sum = j == e ? f[e] : sum;
+            rough = j == e ? t[e] : rough;
+          }
+          if ((BIAS ? fmaf(qs[i], slack, rough) : (rough + slack) * qs[i]) < low[i]) continue;
+          const uint64_t key = offered_key(exact_score(sum - kMagicF, qs[i], a, r0 + j), r0 + j);
+          if (a.store) {
+            a.keys[query * a.cap + b * 32 + group * 8 + j] = key;
+          } else if (key && key >= thr) {  // the threshold's own record is met again
+            const uint32_t to = atomicAdd(&listed, 1u);
+            if (to < kListed) {
+              list_key[to] = key;
+              list_query[to] = query;
+            } else {
+              append(a, query, key);
+            }
           }
         }
       }
@@ -553,31 +750,15 @@ __device__ inline int dot_codes(const int8_t* x, const v4i* q, uint32_t pitch) {
 __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
   __shared__ Held h;
   __shared__ v4i query[kMaxFusedPitch / 16];
-  constexpr int N = 4;
   const PassArgs& p = a.pass;
   const uint32_t row = blockIdx.x;
-  if (threadIdx.x == 0) {
-    h.count = 0;
-    h.floor = 0;
-  }
-  __syncthreads();
+  begin(h);
   const uint64_t listed = a.fixed ? a.fixed : p.count[row];
   const uint64_t held = listed < p.cap ? listed : p.cap;
-  for (int source = 0; source < 2; ++source) {
-    const uint64_t* src = source ? a.extra + row * a.extra_ld : p.keys + row * p.cap;
-    const uint64_t count = source ? (a.extra ? a.extra_count[row] : 0) : held;
-    for (uint64_t c = 0; c < count; c += 256 * N) {
-      uint64_t key[N];
-      for (int i = 0; i < N; ++i) {
-        const uint64_t at = c + i * 256 + threadIdx.x;
-        key[i] = at < count ? src[at] : 0;
-      }
-      offer(h, a.k, key);
-    }
-  }
-  compact(h, a.k);
+  offer_list(h, a.k, p.keys + row * p.cap, held);
+  if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
+  finish(h, a.k);  // every thread has read the row's count: there is a barrier in between
   if (a.thr) {
-    // every thread has read the count: a barrier is behind each of its uses
     if (threadIdx.x == 0) {
       a.thr[row] = h.count == a.k ? h.key[a.k - 1] : 0;
       p.count[row] = 0;
@@ -586,30 +767,22 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
   }
   if (listed > p.cap) {
     // Keys were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
-    // they go, but for the extra ones, which no mask lets through.
+    // they go; the history's records, which no mask lets through, are offered again.
     if (threadIdx.x < p.pitch / 16)
       query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
-    const uint64_t floor = h.count == a.k ? h.key[a.k - 1] : 0;
+    const uint64_t floor = h.count == a.k ? h.key[a.k - 1] - 1 : 0;  // the k-th best itself is an answer
     __syncthreads();
-    if (threadIdx.x == 0) {
-      h.count = 0;
-      h.floor = floor ? floor - 1 : 0;  // the floor itself is an answer
-    }
-    __syncthreads();
+    begin(h, floor);
     const float qs = p.qscales[row];
     for (uint64_t r0 = 0; r0 < p.n; r0 += 256) {
       const uint64_t r = r0 + threadIdx.x;
       uint64_t key[1] = {0};
       if (r < p.n && (!p.allow || (p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u)))
         key[0] = offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
-      offer(h, a.k, key);
+      offer(h, a.k, key, false);
     }
-    if (a.extra)
-      for (uint64_t c = 0; c < a.extra_count[row]; c += 256) {
-        uint64_t key[1] = {c + threadIdx.x < a.extra_count[row] ? a.extra[row * a.extra_ld + c + threadIdx.x] : 0};
-        offer(h, a.k, key);
-      }
-    compact(h, a.k);
+    if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
+    finish(h, a.k);
   }
   write_best(h, a.k, a.values + static_cast<uint64_t>(row) * a.k, a.ids + static_cast<uint64_t>(row) * a.k);
 }
@@ -697,14 +870,24 @@ __global__ __launch_bounds__(256) void seen_keys_kernel(SeenArgs a) {
     default: return hipErrorInvalidValue;         \
   }
 
-hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s) {
-  const uint32_t pitch = code_pitch(a.dim);
-#define SHINE_GROUP(GG)                                                                                    \
-  hipLaunchKernelGGL((quantize_kernel<T, GG>), dim3(static_cast<uint32_t>((a.n + 256 / GG - 1) / (256 / GG))), \
+template <class T>
+void quantize_by_width(const QuantizeArgs& a, hipStream_t s) {
+  const uint32_t pitch = code_pitch(a.dim), steps = pitch * sizeof(T) / 16;  // 16-byte steps of a row
+#define SHINE_GROUP(GG, SS)                                                                                    \
+  hipLaunchKernelGGL((quantize_kernel<T, GG, SS>), dim3(static_cast<uint32_t>((a.n + 256 / GG - 1) / (256 / GG))), \
                      dim3(256), 0, s, a, pitch)
-  SHINE_BY_ELEM(elem, if (pitch <= 64) SHINE_GROUP(8); else if (pitch <= 128) SHINE_GROUP(16);
-                else if (pitch <= 256) SHINE_GROUP(32); else SHINE_GROUP(64));
+  if (steps <= 8) SHINE_GROUP(8, 1);
+  else if (steps <= 16) SHINE_GROUP(16, 1);
+  else if (steps <= 32) SHINE_GROUP(32, 1);
+  else if (steps <= 64) SHINE_GROUP(64, 1);
+  else if (steps <= 128) SHINE_GROUP(64, 2);
+  else if (steps <= 256) SHINE_GROUP(64, 4);
+  else SHINE_GROUP(64, 0);
 #undef SHINE_GROUP
+}
+
+hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s) {
+  SHINE_BY_ELEM(elem, quantize_by_width<T>(a, s));
   return hipGetLastError();
 }
 
@@ -784,8 +967,12 @@ hipError_t launch_seen(const SeenArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>((a.n + kTile - 1) / kTile), a.nq);
-  SHINE_BY_ELEM(elem, hipLaunchKernelGGL(adjust_kernel<T>, grid, dim3(256), 0, s, a));
+  // wide tiles read the history less often, narrow ones spread a small call over more of the GPU
+  const bool wide = a.nq * ((a.n + 8191) / 8192) >= 512;
+  const uint64_t tile = wide ? 8192 : 2048;
+  const dim3 grid(static_cast<uint32_t>((a.n + tile - 1) / tile), a.nq);
+  SHINE_BY_ELEM(elem, if (wide) hipLaunchKernelGGL((adjust_kernel<T, 8192>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((adjust_kernel<T, 2048>), grid, dim3(256), 0, s, a));
   return hipGetLastError();
 }
 
