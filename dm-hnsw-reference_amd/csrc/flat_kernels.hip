@@ -619,33 +619,58 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
 // records) is the next pass's threshold, the coarsest pass stores all its keys, and the last pass is over all records.
 // A list whose room ends loses nothing but time: its row is scanned again, alone, where the answers are selected.
 
-// The score as shine_flat_scores and then shine_flat_adjust round it.
-__device__ inline float exact_score(float sum, float qs, const PassArgs& a, uint64_t record) {
-  float v = (sum * qs) * a.scales[record];
-  if (a.tbias) v += a.tbias[record];
-  if (a.abias) v += a.abias[record];
+// The score as shine_flat_scores and then shine_flat_adjust round it; tb and ab count where the biases are given.
+__device__ inline float exact_score(float sum, float qs, float xs, const PassArgs& a, float tb, float ab) {
+  float v = (sum * qs) * xs;
+  if (a.tbias) v += tb;
+  if (a.abias) v += ab;
   return v;
+}
+__device__ inline float exact_score(float sum, float qs, const PassArgs& a, uint64_t record) {
+  return exact_score(sum, qs, a.scales[record], a, a.tbias ? a.tbias[record] : 0.0f, a.abias ? a.abias[record] : 0.0f);
 }
 
 __device__ inline uint64_t offered_key(float v, uint64_t record) {
   return v >= -3.402823466e38f ? key_of(v, static_cast<uint32_t>(record)) : 0;
 }
 
-constexpr uint32_t kListed = 1536;  // keys a workgroup lists in LDS before they go to the queries' lists together
+// Keys that a workgroup lists in LDS.  They go to the queries' lists together, with one addition to each query's count:
+// additions to one address from all over the GPU are served one after another.
+constexpr uint32_t kListed = 4096;
 
 __device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
   const uint32_t at = atomicAdd(&a.count[query], 1u);
   if (at < a.cap) a.keys[query * a.cap + at] = key;
 }
 
+// Between a wave's own writes to LDS and its lanes' reads of them (a wave's LDS accesses are in order: no wait)
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// What a wave knows of its 32 records, beside their codes.
+template <int QUERIES>
+struct Beside {
+  float xs[32], rough[32], tb[32], ab[32];  // rough: the biases' sum, raised by more than its roundings
+  uint32_t allow[QUERIES];                  // each query's word of its mask
+};
+
 // Per score: one fused multiply-add (two with biases) and half a maximum.  (kMagic + sum) * xs - kMagic * xs is sum * xs
 // up to 1.75 xs (the rounding of kMagic * xs is 0.75, the other roundings of numbers below 2^22 xs less than 1), and the
 // definition's own roundings of near-threshold scores are below 2^-20 of the threshold, so scores that reach the
-// threshold also reach it here once 2 qs max(xs) is added.  What passes is scored again as the definition rounds.
-template <int KC, int QT, bool BIAS>
+// threshold also reach it here once 2 qs max(xs) is added.  What passes is scored again as the definition rounds, from
+// LDS alone: a load from memory there would wait for the next block's codes, which are on their way.
+//
+// The next block is fetched while this one is scored, with no branch around its loads (what is not given is read from the
+// scales and not used): behind a branch the loaded registers would be copied, and the copy would wait for the loads.
+template <int KC, int QT, bool BIAS, bool ROWS, bool STORE>
 __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
-  __shared__ uint64_t list_key[kListed];
-  __shared__ uint32_t list_query[kListed];
+  __shared__ Beside<QT * 16> beside[4];
+  __shared__ uint64_t thr_key[QT * 16];
+  __shared__ uint64_t list_key[STORE ? 1 : kListed];
+  __shared__ uint32_t list_place[STORE ? 1 : kListed];  // the query's number in the workgroup, and the key's among its keys << 8
+  __shared__ uint32_t found[QT * 16], base[QT * 16];
   __shared__ uint32_t listed;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
   const Place at = place_of(query_blocks);
@@ -653,43 +678,93 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
   if (b0 >= b1) return;  // the whole workgroup
   if (threadIdx.x == 0) listed = 0;
-  __syncthreads();
+  if (threadIdx.x < QT * 16) {
+    thr_key[threadIdx.x] = !STORE && query0 + threadIdx.x < a.nq ? a.thr[query0 + threadIdx.x] : 0;
+    found[threadIdx.x] = 0;
+  }
   v4i q[QT][KC];
   load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   float qs[QT], low[QT];
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t r = query0 + i * 16 + col;
     qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
-    const float thr = !a.store && r < a.nq && a.thr[r] ? key_value(a.thr[r]) : -__builtin_huge_valf();
+    const uint64_t key = thr_key[i * 16 + col];
+    const float thr = key ? key_value(key) : -__builtin_huge_valf();
     // scales far from 1 may overflow in one order of products and not in another: everything passes
     low[i] = qs[i] > 1e-18f && qs[i] < 1e18f ? thr - 0x1p-20f * fabsf(thr) : -__builtin_huge_valf();
   }
+  // the next block: its codes, and lane l's part of what is beside record l (lanes 32 .. 63: of record l - 32)
+  constexpr int MASKS = (QT * 16 + 63) / 64;  // queries whose mask words a lane fetches
+  const float* tbias = a.tbias ? a.tbias : a.scales;
+  const float* abias = a.abias ? a.abias : a.scales;
+  const bool has_allow = a.allow, shared = !ROWS && has_allow;
+  const uint32_t* allow_base = has_allow ? a.allow : reinterpret_cast<const uint32_t*>(a.scales);
+  const uint32_t* allow_row[MASKS];
+#pragma unroll
+  for (int i = 0; i < MASKS; ++i) {
+    const uint32_t r = query0 + i * 64 + lane;
+    allow_row[i] = allow_base + (has_allow && ROWS ? (r < a.nq ? r : a.nq - 1) * a.allow_ld : 0);
+  }
   Block<KC> next;
-  if (b0 + wave < b1) load_block<KC>(next, a.codes, (b0 + wave) * a.stride * 32, a.n);
+  float next_xs, next_tb = 0.0f, next_ab = 0.0f;
+  uint32_t next_allow[MASKS];
+  auto fetch = [&](uint64_t b) {
+    const uint64_t word = b * a.stride, r = word * 32 + (lane & 31), at = r < a.n ? r : a.n - 1;
+    load_block<KC>(next, a.codes, word * 32, a.n);
+    next_xs = a.scales[at];
+    if (BIAS) {
+      next_tb = tbias[at];
+      next_ab = abias[at];
+    }
+#pragma unroll
+    for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][has_allow ? word : 0];
+  };
+  const uint64_t last = b1 - 1;
+  fetch(b0 + wave < b1 ? b0 + wave : last);
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
     const Block<KC> x = next;
-    if (b + 4 < b1) load_block<KC>(next, a.codes, (b + 4) * a.stride * 32, a.n);
-    const uint64_t word = b * a.stride, r0 = word * 32 + group * 8;
-    float xs[8], off[8], bias[8], top = 0.0f;
-    bool odd = false;
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
-      xs[j] = a.scales[r];
-      off[j] = -kMagicF * xs[j];
-      top = fmaxf(top, xs[j]);
-      odd |= xs[j] < 1e-18f && xs[j] != 0.0f;
+    const uint64_t word = b * a.stride;
+    uint32_t live = ~0u;  // records of the block that are there and that the shared mask allows
+    if (word * 32 + 32 > a.n) live >>= 32 - static_cast<uint32_t>(a.n - word * 32);
+    if (shared) live &= next_allow[0];
+    Beside<QT * 16>& s = beside[wave];
+    if (lane < 32) {
+      s.xs[lane] = next_xs;
       if (BIAS) {
-        const float t = a.tbias ? a.tbias[r] : 0.0f, d = a.abias ? a.abias[r] : 0.0f;
-        bias[j] = (t + d) + 0x1p-21f * (fabsf(t) + fabsf(d));
-        if (a.allow && a.allow_ld == 0 && !(a.allow[word] >> (group * 8 + j) & 1u)) bias[j] = -__builtin_huge_valf();
+        if (!a.tbias) next_tb = 0.0f;
+        if (!a.abias) next_ab = 0.0f;
+        s.rough[lane] = live >> lane & 1u ? (next_tb + next_ab) + 0x1p-21f * (fabsf(next_tb) + fabsf(next_ab)) : -__builtin_huge_valf();
+        s.tb[lane] = next_tb;
+        s.ab[lane] = next_ab;
       }
     }
-    const float slack = odd || !(top < 1e18f) ? __builtin_huge_valf() : 2.0f * top;
+    if (ROWS) {
+#pragma unroll
+      for (int i = 0; i < MASKS; ++i)
+        if (i * 64 + lane < QT * 16) s.allow[i * 64 + lane] = has_allow ? next_allow[i] : ~0u;
+    }
+    const bool odd = __any((next_xs < 1e-18f && next_xs != 0.0f) || next_xs >= 1e18f);
+    wave_sync();
+    fetch(b + 4 < b1 ? b + 4 : last);
+    float xs[8], off[8], bias[8], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      xs[j] = s.xs[group * 8 + j];
+      off[j] = -kMagicF * xs[j];
+      top = fmaxf(top, xs[j]);
+      if (BIAS) bias[j] = s.rough[group * 8 + j];
+    }
+    const float slack = odd ? __builtin_huge_valf() : 2.0f * top;
+    float ahead[8];  // the next tile's sums: the matrix unit works on them while this tile's are looked at
+    sums<KC>(x, q[0], ahead);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       float f[8], t[8];
-      sums<KC>(x, q[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = ahead[j];
+      if (i + 1 < QT) sums<KC>(x, q[i + 1 < QT ? i + 1 : 0], ahead);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[j] = fmaf(f[j], xs[j], off[j]);
@@ -697,34 +772,41 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
       }
       float best = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
       best = BIAS ? fmaf(qs[i], slack, best) : (best + slack) * qs[i];
-      if (!(best < low[i])) {  // a NaN passes and is refused below
-        const uint32_t query = query0 + i * 16 + col;
-        uint32_t maybe = query < a.nq ? 0xFFu : 0u;
-        if (maybe && a.allow) maybe &= a.allow[query * a.allow_ld + word] >> (group * 8);
-        if (r0 + 8 > a.n) maybe &= r0 < a.n ? 0xFFu >> (8 - (a.n - r0)) : 0u;
-        const uint64_t thr = !a.store && maybe ? a.thr[query] : 0;
-        if (a.store && query < a.nq) {
-          uint64_t* to = a.keys + query * a.cap + b * 32 + group * 8;
-          for (uint32_t j = 0; j < 8; ++j) to[j] = 0;
-        }
-        while (maybe) {
-          const uint32_t j = __builtin_ctz(maybe);
-          maybe &= maybe - 1;
-          float sum = f[0], rough = t[0];
+      const uint32_t query = query0 + i * 16 + col;
+      if (STORE) {
+        if (query < a.nq) {
+          ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + group * 8);
 #pragma unroll
-          for (uint32_t e = 1; e < 8; ++e) {
-            sum = j == e ? f[e] : sum;
-            rough = j == e ? t[e] : rough;
+          for (int j = 0; j < 8; j += 2) {
+            uint64_t key[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t r = group * 8 + j + e;
+              const float v = exact_score(f[j + e] - kMagicF, qs[i], xs[j + e], a, BIAS ? s.tb[r] : 0.0f, BIAS ? s.ab[r] : 0.0f);
+              key[e] = (ROWS ? live & s.allow[i * 16 + col] : live) >> r & 1u ? offered_key(v, word * 32 + r) : 0;
+            }
+            to[j / 2] = make_ulonglong2(key[0], key[1]);
           }
-          if ((BIAS ? fmaf(qs[i], slack, rough) : (rough + slack) * qs[i]) < low[i]) continue;
-          const uint64_t key = offered_key(exact_score(sum - kMagicF, qs[i], a, r0 + j), r0 + j);
-          if (a.store) {
-            a.keys[query * a.cap + b * 32 + group * 8 + j] = key;
-          } else if (key && key >= thr) {  // the threshold's own record is met again
+        }
+      } else if (!(best < low[i])) {  // a NaN passes and is refused below
+        const float under = BIAS ? fmaf(-qs[i], slack, low[i]) : low[i];
+        uint32_t maybe = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) maybe |= ((BIAS ? t[j] : (t[j] + slack) * qs[i]) < under ? 0u : 1u) << j;
+        maybe &= query < a.nq ? (ROWS ? live & s.allow[i * 16 + col] : live) >> (group * 8) : 0u;
+        while (maybe) {
+          const uint32_t j = __builtin_ctz(maybe), r = group * 8 + j;
+          maybe &= maybe - 1;
+          float sum = f[0];
+#pragma unroll
+          for (uint32_t e = 1; e < 8; ++e) sum = j == e ? f[e] : sum;
+          const float v = exact_score(sum - kMagicF, qs[i], s.xs[r], a, BIAS ? s.tb[r] : 0.0f, BIAS ? s.ab[r] : 0.0f);
+          const uint64_t key = offered_key(v, word * 32 + r);
+          if (key && key >= thr_key[i * 16 + col]) {  // the threshold's own record is met again
             const uint32_t to = atomicAdd(&listed, 1u);
             if (to < kListed) {
               list_key[to] = key;
-              list_query[to] = query;
+              list_place[to] = (i * 16 + col) | atomicAdd(&found[i * 16 + col], 1u) << 8;
             } else {
               append(a, query, key);
             }
@@ -732,10 +814,19 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
         }
       }
     }
+    wave_sync();
   }
+  if (STORE) return;
+  __syncthreads();
+  const uint32_t t = threadIdx.x;
+  if (t < QT * 16 && found[t]) base[t] = atomicAdd(&a.count[query0 + t], found[t]);
   __syncthreads();
   const uint32_t m = listed < kListed ? listed : kListed;
-  for (uint32_t i = threadIdx.x; i < m; i += 256) append(a, list_query[i], list_key[i]);
+  for (uint32_t i = t; i < m; i += 256) {
+    const uint32_t mine = list_place[i] & 255u;
+    const uint64_t to = static_cast<uint64_t>(base[mine]) + (list_place[i] >> 8);
+    if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = list_key[i];
+  }
 }
 
 __device__ inline int dot_codes(const int8_t* x, const v4i* q, uint32_t pitch) {
@@ -932,13 +1023,18 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
-  const bool bias = a.tbias || a.abias || (a.allow && a.allow_ld == 0);
+  const bool rows = a.allow && a.allow_ld, bias = a.tbias || a.abias || (a.allow && !rows);
+#define SHINE_FOR(KK, QQ, BB, RR, SS)                                                                      \
+  if (bias == BB && rows == RR && a.store == SS)                                                           \
+    hipLaunchKernelGGL((pass_kernel<KK, QQ, BB, RR, SS>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
 #define SHINE_PASS(KK, QQ)                                                                                 \
   {                                                                                                        \
     const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                  \
     const Ranges r = ranges_of(a.blocks, qb, 1024);                                                        \
-    if (bias) hipLaunchKernelGGL((pass_kernel<KK, QQ, true>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per); \
-    else hipLaunchKernelGGL((pass_kernel<KK, QQ, false>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);     \
+    SHINE_FOR(KK, QQ, true, true, true) SHINE_FOR(KK, QQ, true, true, false)                               \
+    SHINE_FOR(KK, QQ, true, false, true) SHINE_FOR(KK, QQ, true, false, false)                             \
+    SHINE_FOR(KK, QQ, false, true, true) SHINE_FOR(KK, QQ, false, true, false)                             \
+    SHINE_FOR(KK, QQ, false, false, true) SHINE_FOR(KK, QQ, false, false, false)                           \
   }
 #define SHINE_KC(KK, BIG) \
   if (a.nq <= 32) SHINE_PASS(KK, 2) else SHINE_PASS(KK, BIG)
@@ -951,6 +1047,7 @@ hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
   }
 #undef SHINE_KC
 #undef SHINE_PASS
+#undef SHINE_FOR
   return hipGetLastError();
 }
 
