@@ -169,7 +169,7 @@ SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const 
   if (p.fused) {
     p.keys = take(8 * p.cap * p.rows);
     p.thr = take(8ull * p.rows);
-    p.count = take(4ull * p.rows);
+    p.count = take(4ull * F::kCountStride * p.rows);
     if (seen_n) {
       p.mask = take(4 * p.words * p.rows);
       p.extra = take(8ull * seen_n * p.rows);

@@ -38,6 +38,8 @@ struct ScoresArgs {
   uint64_t ld;   // in elements
 };
 
+constexpr uint32_t kCountStride = 32;  // queries' counts lie in memory lines of their own: all XCDs add to them
+
 // One pass of a fused search over every `stride`-th block of 32 records.
 struct PassArgs {
   const int8_t* qcodes;
@@ -54,7 +56,7 @@ struct PassArgs {
   uint64_t stride;
   bool store;             // every key at keys[q * cap + 32 * block + i]; else those from thr on, appended
   const uint64_t* thr;    // per query; key 0: none
-  uint32_t* count;        // per query: keys offered to its list (may pass cap; the list then holds cap of them)
+  uint32_t* count;        // query q's at q * kCountStride: keys offered to its list (may pass cap; the list then holds cap of them)
   uint64_t* keys;
   uint64_t cap;
 };

@@ -145,15 +145,19 @@ struct Block {  // a wave's 32 records
   v4i x[2][KC];
 };
 
+// The wave's number, in a scalar register: what follows from it alone is computed once for the wave
+__device__ inline uint32_t wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 template <int KC>
 __device__ inline void load_block(Block<KC>& b, const int8_t* codes, uint64_t record0, uint64_t n) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+  const int8_t* p = codes + record0 * (KC * 64);
+  const uint32_t last = n - record0 < 32 ? static_cast<uint32_t>(n - record0) - 1 : 31;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {  // rows behind the last one read the last one; nobody uses their sums
-    const uint64_t r = record0 + (col >> 2) * 8 + t * 4 + (col & 3);
-    const int8_t* p = codes + (r < n ? r : n - 1) * (KC * 64) + group * 16;
+    const uint32_t at = min((col >> 2) * 8 + t * 4 + (col & 3), last) * (KC * 64) + group * 16;
 #pragma unroll
-    for (int c = 0; c < KC; ++c) b.x[t][c] = *reinterpret_cast<const v4i*>(p + c * 64);
+    for (int c = 0; c < KC; ++c) b.x[t][c] = *reinterpret_cast<const v4i*>(p + at + c * 64);
   }
 }
 
@@ -169,11 +173,18 @@ __device__ inline void load_queries(v4i (&q)[QT][KC], const int8_t* qcodes, uint
   }
 }
 
+// kMagic four times, in registers of its own that the compiler does not fill anew for every product
+__device__ inline v4i magic_start() {
+  v4i m = {kMagic, kMagic, kMagic, kMagic};
+  asm volatile("" : "+v"(m));
+  return m;
+}
+
 template <int KC>
-__device__ inline void sums(const Block<KC>& b, const v4i (&q)[KC], float (&f)[8]) {
+__device__ inline void sums(const Block<KC>& b, const v4i (&q)[KC], const v4i& start, float (&f)[8]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    v4i acc = {kMagic, kMagic, kMagic, kMagic};
+    v4i acc = start;
 #pragma unroll
     for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.x[t][c], q[c], acc, 0, 0, 0);
 #pragma unroll
@@ -209,7 +220,7 @@ __device__ inline void store_scores(T* dst, const float (&v)[8], uint64_t left) 
 
 template <class T, int KC, int QT>
 __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per_range) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
   const Place at = place_of(query_blocks);
   const uint32_t query0 = at.query_block * QT * 16;
   const uint64_t blocks = (a.n + 31) / 32, b0 = at.range * per_range,
@@ -223,6 +234,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
     const uint32_t r = query0 + i * 16 + col;
     qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
   }
+  const v4i start = magic_start();
   Block<KC> next;
   load_block<KC>(next, a.codes, (b0 + wave) * 32, a.n);
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
@@ -238,7 +250,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       float v[8];
-      sums<KC>(x, q[i], v);
+      sums<KC>(x, q[i], start, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = ((v[j] - kMagicF) * qs[i]) * xs[j];
@@ -639,7 +651,7 @@ __device__ inline uint64_t offered_key(float v, uint64_t record) {
 constexpr uint32_t kListed = 4096;
 
 __device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
-  const uint32_t at = atomicAdd(&a.count[query], 1u);
+  const uint32_t at = atomicAdd(&a.count[query * kCountStride], 1u);
   if (at < a.cap) a.keys[query * a.cap + at] = key;
 }
 
@@ -672,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   __shared__ uint32_t list_place[STORE ? 1 : kListed];  // the query's number in the workgroup, and the key's among its keys << 8
   __shared__ uint32_t found[QT * 16], base[QT * 16];
   __shared__ uint32_t listed;
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
   const Place at = place_of(query_blocks);
   const uint32_t query0 = at.query_block * QT * 16;
   const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
@@ -721,6 +733,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
 #pragma unroll
     for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][has_allow ? word : 0];
   };
+  const v4i start = magic_start();
   const uint64_t last = b1 - 1;
   fetch(b0 + wave < b1 ? b0 + wave : last);
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
@@ -758,13 +771,13 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
     }
     const float slack = odd ? __builtin_huge_valf() : 2.0f * top;
     float ahead[8];  // the next tile's sums: the matrix unit works on them while this tile's are looked at
-    sums<KC>(x, q[0], ahead);
+    sums<KC>(x, q[0], start, ahead);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       float f[8], t[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = ahead[j];
-      if (i + 1 < QT) sums<KC>(x, q[i + 1 < QT ? i + 1 : 0], ahead);
+      if (i + 1 < QT) sums<KC>(x, q[i + 1 < QT ? i + 1 : 0], start, ahead);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[j] = fmaf(f[j], xs[j], off[j]);
@@ -819,7 +832,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   if (STORE) return;
   __syncthreads();
   const uint32_t t = threadIdx.x;
-  if (t < QT * 16 && found[t]) base[t] = atomicAdd(&a.count[query0 + t], found[t]);
+  if (t < QT * 16 && found[t]) base[t] = atomicAdd(&a.count[(query0 + t) * kCountStride], found[t]);
   __syncthreads();
   const uint32_t m = listed < kListed ? listed : kListed;
   for (uint32_t i = t; i < m; i += 256) {
@@ -844,15 +857,17 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
   const PassArgs& p = a.pass;
   const uint32_t row = blockIdx.x;
   begin(h);
-  const uint64_t listed = a.fixed ? a.fixed : p.count[row];
+  const uint64_t listed = a.fixed ? a.fixed : p.count[row * kCountStride];
   const uint64_t held = listed < p.cap ? listed : p.cap;
   offer_list(h, a.k, p.keys + row * p.cap, held);
   if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
   finish(h, a.k);  // every thread has read the row's count: there is a barrier in between
   if (a.thr) {
     if (threadIdx.x == 0) {
-      a.thr[row] = h.count == a.k ? h.key[a.k - 1] : 0;
-      p.count[row] = 0;
+      // a finer pass need not meet the coarser one's records again: where it finds fewer than k, that one's bound stays
+      if (h.count == a.k) a.thr[row] = h.key[a.k - 1];
+      else if (a.fixed) a.thr[row] = 0;
+      p.count[row * kCountStride] = 0;
     }
     return;
   }
@@ -1022,6 +1037,7 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+constexpr uint32_t kPassGroups = 512;  // two workgroups a CU
 hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
   const bool rows = a.allow && a.allow_ld, bias = a.tbias || a.abias || (a.allow && !rows);
 #define SHINE_FOR(KK, QQ, BB, RR, SS)                                                                      \
@@ -1030,7 +1046,7 @@ hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
 #define SHINE_PASS(KK, QQ)                                                                                 \
   {                                                                                                        \
     const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                  \
-    const Ranges r = ranges_of(a.blocks, qb, 1024);                                                        \
+    const Ranges r = ranges_of(a.blocks, qb, kPassGroups);                                                        \
     SHINE_FOR(KK, QQ, true, true, true) SHINE_FOR(KK, QQ, true, true, false)                               \
     SHINE_FOR(KK, QQ, true, false, true) SHINE_FOR(KK, QQ, true, false, false)                             \
     SHINE_FOR(KK, QQ, false, true, true) SHINE_FOR(KK, QQ, false, true, false)                             \
