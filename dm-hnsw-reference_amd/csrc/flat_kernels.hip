@@ -1,6 +1,5 @@
 // Flat scoring kernels for gfx950 (include/shine_gpu.h shine_flat_*): 8-bit row quantisation, the scaled 8-bit matrix
 // product of a query batch with a record table, score adjustments, and top-k.
-#include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -21,7 +20,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec {
 
 __device__ inline float to_f32(float x) { return x; }
 __device__ inline float to_f32(__half x) { return __half2float(x); }
-__device__ inline float to_f32(__hip_bfloat16 x) { return __bfloat162float(x); }
+__device__ inline float to_f32(__bf16 x) { return static_cast<float>(x); }
 template <class T>
 __device__ inline T from_f32(float x);
 template <>
@@ -29,7 +28,7 @@ __device__ inline float from_f32<float>(float x) { return x; }
 template <>
 __device__ inline __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <>
-__device__ inline __hip_bfloat16 from_f32<__hip_bfloat16>(float x) { return __float2bfloat16(x); }
+__device__ inline __bf16 from_f32<__bf16>(float x) { return static_cast<__bf16>(x); }
 
 // ---------------------------------------------------------------------------------------------- quantisation
 // scale = f32(max|x| / 127); code = the integer nearest to x / scale in real arithmetic, halves to even.  The quotient
@@ -148,14 +147,22 @@ struct Block {  // a wave's 32 records
 // The wave's number, in a scalar register: what follows from it alone is computed once for the wave
 __device__ inline uint32_t wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-template <int KC>
+// Between a wave's own writes to LDS and its lanes' reads of them (a wave's LDS accesses are in order: no wait)
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// PAIRED: a lane's eight sums are neighbours (above); else tile t holds records 16 t .. 16 t + 15 and a lane four neighbours
+// of each tile: the better order for writing 32-bit scores, 64 bytes of a row an instruction.
+template <int KC, bool PAIRED = true>
 __device__ inline void load_block(Block<KC>& b, const int8_t* codes, uint64_t record0, uint64_t n) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
   const int8_t* p = codes + record0 * (KC * 64);
   const uint32_t last = n - record0 < 32 ? static_cast<uint32_t>(n - record0) - 1 : 31;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {  // rows behind the last one read the last one; nobody uses their sums
-    const uint32_t at = min((col >> 2) * 8 + t * 4 + (col & 3), last) * (KC * 64) + group * 16;
+    const uint32_t at = min(PAIRED ? (col >> 2) * 8 + t * 4 + (col & 3) : t * 16 + col, last) * (KC * 64) + group * 16;
 #pragma unroll
     for (int c = 0; c < KC; ++c) b.x[t][c] = *reinterpret_cast<const v4i*>(p + at + c * 64);
   }
@@ -204,109 +211,290 @@ __device__ inline Place place_of(uint32_t query_blocks) {
 
 // ---------------------------------------------------------------------------------------------- scores
 // out[i][j] = (float(sum_k qc[i][k] * xc[j][k]) * qscale[i]) * scale[j] (+ bias[j])
-template <class T>
-__device__ inline void store_scores(T* dst, const float (&v)[8], uint64_t left) {
-  if (left >= 8) {
-    constexpr int N = 16 / sizeof(T);
-    for (int h = 0; h < 8 / N; ++h) {
-      Vec<T, N> o;
-      for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>(v[h * N + j]);
-      *reinterpret_cast<Vec<T, N>*>(dst + h * N) = o;
-    }
-  } else {
-    for (uint32_t j = 0; j < left; ++j) dst[j] = from_f32<T>(v[j]);
-  }
+template <class T, int N>
+__device__ inline void store_scores(T* dst, const float* v) {
+  Vec<T, N> o;
+#pragma unroll
+  for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>(v[j]);
+  *reinterpret_cast<Vec<T, N>*>(dst) = o;
 }
 
+// Where a lane's j-th sum of a block belongs, and the writing of all eight to a row, from the block's first record on.
+template <class T>
+struct Order {
+  static constexpr bool kPaired = sizeof(T) == 2;
+  __device__ static uint32_t record(uint32_t group, int j) {
+    return kPaired ? group * 8 + j : (j >> 2) * 16 + group * 4 + (j & 3);
+  }
+  __device__ static void store(T* row, uint32_t group, const float (&v)[8]) {
+    if (kPaired) {
+      store_scores<T, 8>(row + group * 8, v);
+    } else {
+      store_scores<T, 4>(row + group * 4, v);
+      store_scores<T, 4>(row + 16 + group * 4, v + 4);
+    }
+  }
+  __device__ static void store(T* row, uint32_t group, const float (&v)[8], uint32_t left) {  // the row's last `left` records
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (record(group, j) < left) row[record(group, j)] = from_f32<T>(v[j]);
+  }
+};
+
+// The next block's codes, scales and biases are asked for before this block's scores are written, and no branch is around
+// the writes: memory accesses end in order, so what waits for a load must know how many writes are behind it.  Lanes
+// whose query is behind the last one hold the last one and write its scores once more; the block that the records end in
+// comes last, on its own.
 template <class T, int KC, int QT>
 __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per_range) {
+  __shared__ float beside[4][2][32];  // each wave's records' scales and biases
   const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
   const Place at = place_of(query_blocks);
   const uint32_t query0 = at.query_block * QT * 16;
-  const uint64_t blocks = (a.n + 31) / 32, b0 = at.range * per_range,
+  const uint64_t blocks = (a.n + 31) / 32, whole = a.n / 32, b0 = at.range * per_range,
                  b1 = b0 + per_range < blocks ? b0 + per_range : blocks;
   if (b0 + wave >= b1) return;
   v4i q[QT][KC];
   load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   float qs[QT];
+  T* to[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const uint32_t r = query0 + i * 16 + col;
-    qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
+    const uint32_t r = min(query0 + i * 16 + col, a.nq - 1);
+    qs[i] = a.qscales[r];
+    to[i] = static_cast<T*>(a.out) + r * a.ld;
   }
   const v4i start = magic_start();
+  const float* biases = a.bias ? a.bias : a.scales;
   Block<KC> next;
-  load_block<KC>(next, a.codes, (b0 + wave) * 32, a.n);
-  for (uint64_t b = b0 + wave; b < b1; b += 4) {
-    const Block<KC> x = next;
-    if (b + 4 < b1) load_block<KC>(next, a.codes, (b + 4) * 32, a.n);
-    const uint64_t r0 = b * 32 + group * 8;
-    float xs[8], bias[8];
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
-      xs[j] = a.scales[r];
-      bias[j] = a.bias ? a.bias[r] : 0.0f;
+  float next_xs, next_bias;
+  auto fetch = [&](uint64_t b) {
+    load_block<KC, Order<T>::kPaired>(next, a.codes, b * 32, a.n);
+    const uint64_t r = b * 32 + (lane & 31), from = r < a.n ? r : a.n - 1;
+    next_xs = a.scales[from];
+    next_bias = biases[from];
+  };
+  Block<KC> x;
+  auto stage = [&] {  // what was fetched is next to be scored: here, and not where the compiler would first need it
+    x = next;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) asm volatile("" : "+v"(x.x[t][c]));
+    if (lane < 32) {
+      beside[wave][0][lane] = next_xs;
+      beside[wave][1][lane] = a.bias ? next_bias : -0.0f;  // adding -0 changes nothing
     }
+    wave_sync();
+  };
+  float xs[8], bias[8];
+  auto look = [&] {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      xs[j] = beside[wave][0][Order<T>::record(group, j)];
+      bias[j] = beside[wave][1][Order<T>::record(group, j)];
+    }
+    wave_sync();
+  };
+  auto score = [&](int i, float(&v)[8]) {
+    sums<KC>(x, q[i], start, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = ((v[j] - kMagicF) * qs[i]) * xs[j] + bias[j];
+  };
+  uint64_t b = b0 + wave;
+  fetch(b);
+  stage();
+  for (; b < b1 && b < whole; b += 4) {
+    look();
+    fetch(b + 4 < b1 ? b + 4 : b1 - 1);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       float v[8];
-      sums<KC>(x, q[i], start, v);
+      score(i, v);
+      Order<T>::store(to[i] + b * 32, group, v);
+    }
+    stage();  // at the end: at the start, where the first block's loads have no writes behind them, it would wait for all
+  }
+  if (b < b1) {
+    look();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = ((v[j] - kMagicF) * qs[i]) * xs[j];
-        if (a.bias) v[j] += bias[j];
-      }
-      const uint32_t row = query0 + i * 16 + col;
-      if (row < a.nq && r0 < a.n) store_scores<T>(static_cast<T*>(a.out) + row * a.ld + r0, v, a.n - r0);
+    for (int i = 0; i < QT; ++i) {
+      float v[8];
+      score(i, v);
+      Order<T>::store(to[i] + b * 32, group, v, static_cast<uint32_t>(a.n - b * 32));
     }
   }
 }
 
-// Rows of any width.
+// Wider rows: tiles of 256 records x 128 queries, four waves of 128 x 64 each, 64 codes of every row a step.  A step's codes go
+// through LDS (a wave reads 12 fragments for 32 matrix instructions) in two buffers; the step after the next is on its way in
+// registers meanwhile.  A row's four 16-byte pieces are rotated by its number, so that the 8 rows that one LDS cycle serves
+// lie in different banks.
+constexpr uint32_t kTileRecords = 256, kTileQueries = 128;
+
+struct WideTile {
+  int8_t x[2][kTileRecords * 64], q[2][kTileQueries * 64];
+};
+
+__device__ inline uint32_t record_piece(uint32_t row, uint32_t piece) {  // rows met together: 0 .. 3 and 8 .. 11 (+ 4)
+  return row * 64 + (piece ^ ((row >> 1 & 1) | (row >> 2 & 2))) * 16;
+}
+__device__ inline uint32_t query_piece(uint32_t row, uint32_t piece) { return row * 64 + (piece ^ (row >> 1 & 3)) * 16; }
+
+// acc[i][t]: query tile i (16 queries) of the wave's four, record tile t of its eight (two to a block of 32)
+template <bool PAIRED>
+__device__ inline void wide_sums(WideTile& w, const int8_t* codes, uint64_t n, const int8_t* qcodes, uint32_t nq, uint32_t pitch,
+                                 uint64_t record0, uint32_t query0, v4i (&acc)[4][8]) {
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
+  const int8_t* xbase = codes + record0 * pitch;
+  const int8_t* qbase = qcodes + static_cast<uint64_t>(query0) * pitch;
+  const uint32_t xlast = static_cast<uint32_t>(min(n - record0, static_cast<uint64_t>(kTileRecords))) - 1,
+                 qlast = min(nq - query0, kTileQueries) - 1;
+  const uint32_t row = threadIdx.x >> 2, piece = threadIdx.x & 3;  // this thread brings piece `piece` of rows row + 64 j
+  uint32_t xat[4], qat[2];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) xat[j] = min(row + 64 * j, xlast) * pitch + piece * 16;  // behind the last row: the last row
+#pragma unroll
+  for (uint32_t j = 0; j < 2; ++j) qat[j] = min(row + 64 * j, qlast) * pitch + piece * 16;
+  v4i xr[4], qr[2];
+  auto fetch = [&](uint32_t c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xr[j] = *reinterpret_cast<const v4i*>(xbase + xat[j] + c);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) qr[j] = *reinterpret_cast<const v4i*>(qbase + qat[j] + c);
+  };
+  auto put = [&](uint32_t buffer) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(&w.x[buffer][record_piece(row + 64 * j, piece)]) = xr[j];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) *reinterpret_cast<v4i*>(&w.q[buffer][query_piece(row + 64 * j, piece)]) = qr[j];
+  };
+  const uint32_t x0 = (wave & 1) * 128, q0 = (wave >> 1) * 64;
+  uint32_t xlds[8], qlds[4];
+#pragma unroll
+  for (uint32_t t = 0; t < 8; ++t) xlds[t] = record_piece(x0 + (t >> 1) * 32 + (PAIRED ? (col >> 2) * 8 + (t & 1) * 4 + (col & 3) : (t & 1) * 16 + col), group);
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) qlds[i] = query_piece(q0 + i * 16 + col, group);
+  fetch(0);
+  put(0);
+  if (pitch > 64) fetch(64);
+  __syncthreads();
+  for (uint32_t c = 0, buffer = 0; c < pitch; c += 64, buffer ^= 1) {
+    v4i xf[8], qf[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const v4i*>(&w.q[buffer][qlds[i]]);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) xf[t] = *reinterpret_cast<const v4i*>(&w.x[buffer][xlds[t]]);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[t], qf[i], acc[i][t], 0, 0, 0);
+    if (c + 64 < pitch) {
+      put(buffer ^ 1);  // everyone read it before the last barrier
+      if (c + 128 < pitch) fetch(c + 128);
+      __syncthreads();
+    }
+  }
+}
+
 template <class T>
-__global__ __launch_bounds__(256) void scores_kernel(ScoresArgs a) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t record0 = (static_cast<uint64_t>(blockIdx.x) * 4 + wave) * 32;
-  const uint32_t query0 = blockIdx.y * 64;
-  if (record0 >= a.n) return;
-  const uint32_t col = lane & 15, group = lane >> 4;
-  const int8_t* qp[4];
-  const int8_t* xp[2];
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t q = query0 + i * 16 + col;
-    qp[i] = a.qcodes + static_cast<uint64_t>(q < a.nq ? q : a.nq - 1) * a.pitch + group * 16;
+__global__ __launch_bounds__(256, 2) void scores_wide_kernel(ScoresArgs a, uint32_t query_blocks, uint32_t record_blocks) {
+  __shared__ WideTile w;
+  __shared__ float scales[kTileRecords], biases[kTileRecords], qscales[kTileQueries];
+  const Place at = place_of(query_blocks);
+  if (at.range >= record_blocks) return;
+  const uint64_t record0 = static_cast<uint64_t>(at.range) * kTileRecords;
+  const uint32_t query0 = at.query_block * kTileQueries;
+  {
+    const uint64_t r = min(record0 + threadIdx.x, a.n - 1);
+    scales[threadIdx.x] = a.scales[r];
+    biases[threadIdx.x] = a.bias ? a.bias[r] : -0.0f;  // adding -0 changes nothing
+    if (threadIdx.x < kTileQueries) qscales[threadIdx.x] = a.qscales[min(query0 + threadIdx.x, a.nq - 1)];
   }
-  for (int t = 0; t < 2; ++t) {
-    const uint64_t r = record0 + (col >> 2) * 8 + t * 4 + (col & 3);
-    xp[t] = a.codes + (r < a.n ? r : a.n - 1) * a.pitch + group * 16;
-  }
-  v4i acc[4][2] = {};
-  for (uint32_t c = 0; c < a.pitch; c += 64) {
-    v4i x[2];
-    for (int t = 0; t < 2; ++t) x[t] = *reinterpret_cast<const v4i*>(xp[t] + c);
+  v4i acc[4][8] = {};
+  wide_sums<Order<T>::kPaired>(w, a.codes, a.n, a.qcodes, a.nq, a.pitch, record0, query0, acc);
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
+  const bool whole = record0 + kTileRecords <= a.n;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t at0 = (wave & 1) * 128 + p * 32;
+    const uint64_t r0 = record0 + at0;
+    float xs[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      xs[j] = scales[at0 + Order<T>::record(group, j)];
+      b[j] = biases[at0 + Order<T>::record(group, j)];
+    }
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const v4i q = *reinterpret_cast<const v4i*>(qp[i] + c);
+      const uint32_t q = (wave >> 1) * 64 + i * 16 + col;
+      const float qs = qscales[q];
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (static_cast<float>(acc[i][p * 2 + (j >> 2)][j & 3]) * qs) * xs[j] + b[j];
+      // queries behind the last one are the last one: its scores are written once more
+      T* row = static_cast<T*>(a.out) + min(query0 + q, a.nq - 1) * a.ld + r0;
+      if (whole) Order<T>::store(row, group, v);
+      else if (r0 < a.n) Order<T>::store(row, group, v, static_cast<uint32_t>(min(a.n - r0, static_cast<uint64_t>(32))));
+    }
+  }
+}
+
+// Wide rows, few queries: every wave 32 records, the queries' codes from the caches.
+template <class T, int QT>
+__global__ __launch_bounds__(256) void scores_few_kernel(ScoresArgs a) {
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+  const uint64_t record0 = (static_cast<uint64_t>(blockIdx.x) * 4 + wave_number()) * 32;
+  if (record0 >= a.n) return;
+  const uint32_t last = static_cast<uint32_t>(min(a.n - record0, 32ul)) - 1;
+  const int8_t* xbase = a.codes + record0 * a.pitch;
+  uint32_t xat[2], qat[QT];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) xat[t] = min(Order<T>::kPaired ? (col >> 2) * 8 + t * 4 + (col & 3) : t * 16 + col, last) * a.pitch + group * 16;
+#pragma unroll
+  for (int i = 0; i < QT; ++i) qat[i] = min(i * 16 + col, a.nq - 1) * a.pitch + group * 16;
+  v4i acc[QT][2] = {};
+  auto step = [&](const v4i(&x)[2], uint32_t c) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      const v4i q = *reinterpret_cast<const v4i*>(a.qcodes + qat[i] + c);
+#pragma unroll
       for (int t = 0; t < 2; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t], q, acc[i][t], 0, 0, 0);
     }
+  };
+  uint32_t c = 0;
+  for (; c + 256 <= a.pitch; c += 256) {  // four steps' records are asked for together
+    v4i x[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) x[k][t] = *reinterpret_cast<const v4i*>(xbase + xat[t] + c + k * 64);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) step(x[k], c + k * 64);
   }
-  const uint64_t r0 = record0 + group * 8;
-  if (r0 >= a.n) return;
+  for (; c < a.pitch; c += 64) {
+    v4i x[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) x[t] = *reinterpret_cast<const v4i*>(xbase + xat[t] + c);
+    step(x, c);
+  }
   float xs[8], b[8];
+#pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const uint64_t r = r0 + j < a.n ? r0 + j : a.n - 1;
+    const uint64_t r = min(record0 + Order<T>::record(group, j), a.n - 1);
     xs[j] = a.scales[r];
-    b[j] = a.bias ? a.bias[r] : 0.0f;
+    b[j] = a.bias ? a.bias[r] : -0.0f;
   }
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t q = query0 + i * 16 + col;
-    if (q >= a.nq) continue;
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const uint32_t q = min(i * 16 + col, a.nq - 1);  // behind the last query: the last one once more
     const float qs = a.qscales[q];
     float v[8];
-    for (int j = 0; j < 8; ++j) {
-      v[j] = (static_cast<float>(acc[i][j >> 2][j & 3]) * qs) * xs[j];
-      if (a.bias) v[j] += b[j];
-    }
-    store_scores<T>(static_cast<T*>(a.out) + q * a.ld + r0, v, a.n - r0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (static_cast<float>(acc[i][j >> 2][j & 3]) * qs) * xs[j] + b[j];
+    T* row = static_cast<T*>(a.out) + q * a.ld + record0;
+    if (last == 31) Order<T>::store(row, group, v);
+    else Order<T>::store(row, group, v, last + 1);
   }
 }
 
@@ -345,25 +533,39 @@ __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
     if (bias) v += b;
     return on ? v : -__builtin_huge_valf();
   };
-#pragma unroll 2
-  for (uint32_t i = threadIdx.x * V; i < width; i += 256 * V) {
-    const uint32_t on = allow ? allow[i >> 5] >> (i & 31) : ~0u;
-    if (i + V <= width) {
-      Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src + i);
-      Vec<float, V> b{};
-      if (bias) b = *reinterpret_cast<const Vec<float, V>*>(bias + i);
-      uint32_t c[V] = {};
-      if (history)
-        for (int j = 0; j < V; j += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(&count[i + j]);
-          c[j] = w.x, c[j + 1] = w.y, c[j + 2] = w.z, c[j + 3] = w.w;
-        }
+  // kTogether steps' scores are asked for before any is written: memory accesses end in order
+  constexpr uint32_t kTogether = TILE / (256 * V) < 4 ? TILE / (256 * V) : 4;
+  for (uint32_t i0 = threadIdx.x * V; i0 < width; i0 += 256 * V * kTogether) {
+    Vec<T, V> x[kTogether];
+    Vec<float, V> b[kTogether] = {};
+    uint32_t on[kTogether];
 #pragma unroll
-      for (int j = 0; j < V; ++j) x.v[j] = from_f32<T>(change(to_f32(x.v[j]), c[j], b.v[j], on >> j & 1u));
-      *reinterpret_cast<Vec<T, V>*>(dst + i) = x;
-    } else {
-      for (uint32_t j = 0; i + j < width; ++j)
-        dst[i + j] = from_f32<T>(change(to_f32(src[i + j]), history ? count[i + j] : 0, bias ? bias[i + j] : 0.0f, on >> j & 1u));
+    for (uint32_t h = 0; h < kTogether; ++h) {
+      const uint32_t i = i0 + h * 256 * V;
+      on[h] = allow && i < width ? allow[i >> 5] >> (i & 31) : ~0u;
+      if (i + V <= width) {
+        x[h] = *reinterpret_cast<const Vec<T, V>*>(src + i);
+        if (bias) b[h] = *reinterpret_cast<const Vec<float, V>*>(bias + i);
+      }
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < kTogether; ++h) {
+      const uint32_t i = i0 + h * 256 * V;
+      if (i + V <= width) {
+        uint32_t c[V] = {};
+        if (history)
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&count[i + j]);
+            c[j] = w.x, c[j + 1] = w.y, c[j + 2] = w.z, c[j + 3] = w.w;
+          }
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[h].v[j] = from_f32<T>(change(to_f32(x[h].v[j]), c[j], b[h].v[j], on[h] >> j & 1u));
+        *reinterpret_cast<Vec<T, V>*>(dst + i) = x[h];
+      } else {
+        for (uint32_t j = 0; i + j < width; ++j)
+          dst[i + j] = from_f32<T>(change(to_f32(src[i + j]), history ? count[i + j] : 0, bias ? bias[i + j] : 0.0f, on[h] >> j & 1u));
+      }
     }
   }
 }
@@ -653,12 +855,6 @@ constexpr uint32_t kListed = 4096;
 __device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
   const uint32_t at = atomicAdd(&a.count[query * kCountStride], 1u);
   if (at < a.cap) a.keys[query * a.cap + at] = key;
-}
-
-// Between a wave's own writes to LDS and its lanes' reads of them (a wave's LDS accesses are in order: no wait)
-__device__ inline void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 }
 
 // What a wave knows of its 32 records, beside their codes.
@@ -972,7 +1168,7 @@ __global__ __launch_bounds__(256) void seen_keys_kernel(SeenArgs a) {
   switch (elem) {                                 \
     case kF32: { using T = float; CALL; break; }  \
     case kF16: { using T = __half; CALL; break; } \
-    case kBF16: { using T = __hip_bfloat16; CALL; break; } \
+    case kBF16: { using T = __bf16; CALL; break; } \
     default: return hipErrorInvalidValue;         \
   }
 
@@ -1013,27 +1209,31 @@ Ranges ranges_of(uint64_t blocks, uint32_t query_blocks, uint32_t want) {
 }  // namespace
 
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
-  if (a.pitch <= kStreamPitch) {
-#define SHINE_STREAM(KK, QQ)                                                                              \
+  // Up to 32 queries: streams of any number of workgroups, the more the better where the table's bytes count (1 x 4M x 128:
+  // 107 us with 4096, 113 with 512).  More: rows of 128 codes stream in 512 workgroups (1024 x 100,000 x 96: 46 us with bf16
+  // scores, 117 with f32; in tiles 56 and 109), wider ones go in tiles (1024 x 100,000 x 200: 66 and 123 us; streamed, with
+  // 64 queries a wave, 66 and 158).
+  if (a.pitch <= (a.nq <= 32 ? kStreamPitch : 128)) {
+#define SHINE_STREAM(KK, QQ, WANT)                                                                        \
   {                                                                                                       \
     const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                 \
-    const Ranges r = ranges_of((a.n + 31) / 32, qb, 2048);                                                \
+    const Ranges r = ranges_of((a.n + 31) / 32, qb, WANT);                                                \
     hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);   \
   }
-#define SHINE_KC(KK, BIG) \
-  if (a.nq <= 16) SHINE_STREAM(KK, 1) else if (a.nq <= 32) SHINE_STREAM(KK, 2) else SHINE_STREAM(KK, BIG)
     SHINE_BY_ELEM(out_elem, switch (a.pitch / 64) {
-      case 1: SHINE_KC(1, 8); break;
-      case 2: SHINE_KC(2, 8); break;
-      case 3: SHINE_KC(3, 4); break;
-      default: SHINE_KC(4, 4); break;
+      case 1: if (a.nq <= 16) SHINE_STREAM(1, 1, 4096) else if (a.nq <= 32) SHINE_STREAM(1, 2, 2048) else SHINE_STREAM(1, 8, 512) break;
+      case 2: if (a.nq <= 16) SHINE_STREAM(2, 1, 4096) else if (a.nq <= 32) SHINE_STREAM(2, 2, 2048) else SHINE_STREAM(2, 8, 512) break;
+      case 3: if (a.nq <= 16) SHINE_STREAM(3, 1, 4096) else SHINE_STREAM(3, 2, 2048) break;
+      default: if (a.nq <= 16) SHINE_STREAM(4, 1, 4096) else SHINE_STREAM(4, 2, 2048) break;
     });
-#undef SHINE_KC
 #undef SHINE_STREAM
     return hipGetLastError();
   }
-  const dim3 grid(static_cast<uint32_t>((a.n + 127) / 128), (a.nq + 63) / 64);
-  SHINE_BY_ELEM(out_elem, hipLaunchKernelGGL(scores_kernel<T>, grid, dim3(256), 0, s, a));
+  const uint32_t few = static_cast<uint32_t>((a.n + 127) / 128), qb = (a.nq + kTileQueries - 1) / kTileQueries,
+                 rb = static_cast<uint32_t>((a.n + kTileRecords - 1) / kTileRecords);
+  SHINE_BY_ELEM(out_elem, if (a.nq <= 16) hipLaunchKernelGGL((scores_few_kernel<T, 1>), dim3(few), dim3(256), 0, s, a);
+                else if (a.nq <= 32) hipLaunchKernelGGL((scores_few_kernel<T, 2>), dim3(few), dim3(256), 0, s, a);
+                else hipLaunchKernelGGL(scores_wide_kernel<T>, dim3((rb + 7) / 8 * 8 * qb), dim3(256), 0, s, a, qb, rb));
   return hipGetLastError();
 }
 
