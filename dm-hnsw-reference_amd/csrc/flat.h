@@ -87,6 +87,7 @@ struct SeenArgs {
   uint32_t* extra_count;
   uint64_t extra_ld;
 };
+constexpr uint32_t kMaxHistory = 65535;    // longest history (its counts are 16-bit numbers)
 constexpr uint32_t kMaxSeen = 4096;       // longest history of a fused search (its ids are sorted in LDS)
 constexpr uint32_t kMaxFusedPitch = 256;  // widest rows of a fused search (the queries' codes stay in registers)
 

@@ -499,46 +499,28 @@ __global__ __launch_bounds__(256) void scores_few_kernel(ScoresArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- adjust
-// One workgroup per (row, TILE columns): the row's history is counted into LDS for the tile's columns (integer
-// additions: any order gives the same counts), then every column is read, changed and written once, 16 bytes a lane.
-// Tiles start at multiples of 32 records, so a lane's columns share a word of allowed bits.
+// One workgroup per (row, TILE columns).  The row's history is counted in LDS for the tile's columns, in 16 bits beside a bit
+// for each column that is met (integer additions: any order gives the same counts).  Then every column is read, changed
+// and written once, 16 bytes a lane.  Tiles start at multiples of 32 records, so a lane's columns share a word of allowed
+// bits and one of met ones.
+// A batch of loads is asked for before anything of it is written (memory accesses end in order), the first one before the
+// history is counted.
 template <class T, int TILE>
 __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
   constexpr int V = 16 / sizeof(T);
-  __shared__ uint32_t count[TILE];
+  constexpr uint32_t kSteps = TILE / (256 * V), kTogether = kSteps < 4 ? kSteps : 4;
+  __shared__ uint32_t count[TILE / 2], met[TILE / 32];
   const uint32_t row = blockIdx.y;
   const uint64_t c0 = static_cast<uint64_t>(blockIdx.x) * TILE;
   const uint32_t width = static_cast<uint32_t>(a.n - c0 < TILE ? a.n - c0 : TILE);
-  const bool history = a.seen && a.seen_n;
-  if (history) {
-    for (uint32_t i = threadIdx.x * 4; i < TILE; i += 1024) *reinterpret_cast<uint4*>(&count[i]) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    const int32_t* seen = a.seen + row * a.seen_ld;
-    const int64_t from = static_cast<int64_t>(a.first + c0);
-    for (uint32_t i = threadIdx.x; i < a.seen_n; i += 256) {
-      const int32_t id = seen[i];
-      const int64_t at = id - from;
-      if (id >= 0 && at >= 0 && at < width) atomicAdd(&count[at], 1u);
-    }
-    __syncthreads();
-  }
-  const float r = a.repetition ? a.repetition[row] : 1.0f, f = a.frequency ? a.frequency[row] : 0.0f,
-              p = a.presence ? a.presence[row] : 0.0f;
   const T* src = static_cast<const T*>(a.scores) + row * a.ld + c0;
   T* dst = static_cast<T*>(a.out) + row * a.out_ld + c0;
   const float* bias = a.bias ? a.bias + row * a.bias_ld + a.first + c0 : nullptr;
   const uint32_t* allow = a.allow ? a.allow + row * a.allow_ld + ((a.first + c0) >> 5) : nullptr;
-  auto change = [&](float v, uint32_t times, float b, bool on) {
-    if (times) v = ((v > 0.0f ? v / r : v * r) - f * static_cast<float>(times)) - p;
-    if (bias) v += b;
-    return on ? v : -__builtin_huge_valf();
-  };
-  // kTogether steps' scores are asked for before any is written: memory accesses end in order
-  constexpr uint32_t kTogether = TILE / (256 * V) < 4 ? TILE / (256 * V) : 4;
-  for (uint32_t i0 = threadIdx.x * V; i0 < width; i0 += 256 * V * kTogether) {
-    Vec<T, V> x[kTogether];
-    Vec<float, V> b[kTogether] = {};
-    uint32_t on[kTogether];
+  Vec<T, V> x[kTogether];
+  Vec<float, V> b[kTogether] = {};
+  uint32_t on[kTogether];
+  auto fetch = [&](uint32_t i0) {
 #pragma unroll
     for (uint32_t h = 0; h < kTogether; ++h) {
       const uint32_t i = i0 + h * 256 * V;
@@ -548,25 +530,69 @@ __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
         if (bias) b[h] = *reinterpret_cast<const Vec<float, V>*>(bias + i);
       }
     }
+  };
+  const bool history = a.seen && a.seen_n;
+  constexpr uint32_t kIds = 8;
+  const int32_t* seen = history ? a.seen + row * a.seen_ld : nullptr;
+  const uint32_t from = static_cast<uint32_t>(a.first + c0);
+  int32_t id[kIds];
+  if (history)
+#pragma unroll
+    for (uint32_t j = 0; j < kIds; ++j) id[j] = threadIdx.x + 256 * j < a.seen_n ? seen[threadIdx.x + 256 * j] : -1;
+  fetch(threadIdx.x * V);
+  const float r = a.repetition ? a.repetition[row] : 1.0f, f = a.frequency ? a.frequency[row] : 0.0f,
+              p = a.presence ? a.presence[row] : 0.0f;
+  if (history) {
+    for (uint32_t i = threadIdx.x * 4; i < TILE / 2; i += 1024) *reinterpret_cast<uint4*>(&count[i]) = make_uint4(0, 0, 0, 0);
+    for (uint32_t i = threadIdx.x; i < TILE / 32; i += 256) met[i] = 0;
+    __syncthreads();
+    auto meet = [&](int32_t id) {
+      const uint32_t at = static_cast<uint32_t>(id) - from;  // ids before the tile and -1 wrap to more than 2^31
+      if (at < width) {
+        atomicAdd(&count[at >> 1], 1u << (at & 1) * 16);
+        atomicOr(&met[at >> 5], 1u << (at & 31));
+      }
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < kIds; ++j) meet(id[j]);
+    for (uint32_t i = threadIdx.x + 256 * kIds; i < a.seen_n; i += 256) meet(seen[i]);
+    __syncthreads();
+  }
+  auto times = [&](uint32_t i) { return count[i >> 1] >> (i & 1) * 16 & 0xFFFFu; };
+  auto penalised = [&](float v, uint32_t times) {
+    return ((v > 0.0f ? v / r : v * r) - f * static_cast<float>(times)) - p;
+  };
+  auto finish = [&](float v, float b, bool on) {
+    if (bias) v += b;
+    return on ? v : -__builtin_huge_valf();
+  };
+  for (uint32_t i0 = threadIdx.x * V;;) {
 #pragma unroll
     for (uint32_t h = 0; h < kTogether; ++h) {
       const uint32_t i = i0 + h * 256 * V;
       if (i + V <= width) {
-        uint32_t c[V] = {};
-        if (history)
+        float v[V];
 #pragma unroll
-          for (int j = 0; j < V; j += 4) {
-            const uint4 w = *reinterpret_cast<const uint4*>(&count[i + j]);
-            c[j] = w.x, c[j + 1] = w.y, c[j + 2] = w.z, c[j + 3] = w.w;
-          }
+        for (int j = 0; j < V; ++j) v[j] = to_f32(x[h].v[j]);
+        const uint32_t some = history ? met[i >> 5] >> (i & 31) & ((1u << V) - 1) : 0;
+        if (some)
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[h].v[j] = from_f32<T>(change(to_f32(x[h].v[j]), c[j], b[h].v[j], on[h] >> j & 1u));
+          for (int j = 0; j < V; ++j)
+            if (some >> j & 1u) v[j] = penalised(v[j], times(i + j));
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[h].v[j] = from_f32<T>(finish(v[j], b[h].v[j], on[h] >> j & 1u));
         *reinterpret_cast<Vec<T, V>*>(dst + i) = x[h];
       } else {
-        for (uint32_t j = 0; i + j < width; ++j)
-          dst[i + j] = from_f32<T>(change(to_f32(src[i + j]), history ? count[i + j] : 0, bias ? bias[i + j] : 0.0f, on[h] >> j & 1u));
+        for (uint32_t j = 0; i + j < width; ++j) {
+          float v = to_f32(src[i + j]);
+          if (history && met[(i + j) >> 5] >> ((i + j) & 31) & 1u) v = penalised(v, times(i + j));
+          dst[i + j] = from_f32<T>(finish(v, bias ? bias[i + j] : 0.0f, on[h] >> j & 1u));
+        }
       }
     }
+    i0 += 256 * V * kTogether;
+    if (i0 >= width) break;
+    fetch(i0);
   }
 }
 
@@ -740,51 +766,74 @@ __device__ inline void write_best(const Held& h, uint32_t k, T* values, int32_t*
   }
 }
 
+// A turn takes 16 values a thread; the next turn's are on their way meanwhile.  The floor is raised from the threads' largest
+// values after turns 1, 4, 16, ...: fewer and fewer values then pass it.
 template <class T>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
   __shared__ Held h;
-  constexpr int V = 16 / sizeof(T), N = 16;  // values of a load, of a thread and turn
+  constexpr int V = 16 / sizeof(T), N = 16, L = N / V;  // values of a load, values and loads of a turn
+  constexpr float kLowest = -3.402823466e38f;
   const uint32_t row = blockIdx.y, slice = blockIdx.x;
   begin(h);
   const T* src = static_cast<const T*>(a.scores) + row * a.ld;
   const uint64_t per = (a.n + a.slices - 1) / a.slices, c0 = slice * per, c1 = c0 + per < a.n ? c0 + per : a.n;
-  for (uint64_t c = c0; c < c1; c += 256 * N) {
-    float v[N];
-    float best = -__builtin_huge_valf();
+  Vec<T, V> next[L];
+  auto fetch = [&](uint64_t c) {
+    if (c + 256 * N <= c1) {
 #pragma unroll
-    for (int i = 0; i < N; i += V) {
-      const uint64_t at = c + i * 256 + threadIdx.x * V;
-      if (at + V <= c1) {
-        const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src + at);
+      for (int i = 0; i < L; ++i) next[i] = *reinterpret_cast<const Vec<T, V>*>(src + c + i * 256 * V + threadIdx.x * V);
+    } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i + j] = to_f32(x.v[j]);
-      } else {
+      for (int i = 0; i < L; ++i) {
+        const uint64_t at = c + i * 256 * V + threadIdx.x * V;
+        if (at + V <= c1) {
+          next[i] = *reinterpret_cast<const Vec<T, V>*>(src + at);
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i + j] = at + j < c1 ? to_f32(src[at + j]) : -__builtin_huge_valf();
+          for (int j = 0; j < V; ++j) next[i].v[j] = at + j < c1 ? src[at + j] : from_f32<T>(-__builtin_huge_valf());
+        }
       }
     }
+  };
+  if (c0 < c1) fetch(c0);
+  float best = -__builtin_huge_valf();
+  uint32_t until = 1, turns = 1;
+  for (uint64_t c = c0; c < c1; c += 256 * N) {
+    float v[N], top[N / 4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = fmaxf(best, v[i]);  // a NaN is no maximum
-    if (c == c0) raise_floor(h, best >= -3.402823466e38f ? static_cast<uint32_t>(key_of(best, 0) >> 32) : 0, a.k);
+    for (int i = 0; i < N; ++i) v[i] = to_f32(next[i / V].v[i % V]);
+    if (c + 256 * N < c1) fetch(c + 256 * N);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)  // a NaN is no maximum
+      top[i] = fmaxf(fmaxf(v[i * 4], v[i * 4 + 1]), fmaxf(v[i * 4 + 2], v[i * 4 + 3]));
+    best = fmaxf(best, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    if (--until == 0) {
+      raise_floor(h, best >= kLowest ? static_cast<uint32_t>(key_of(best, 0) >> 32) : 0, a.k);
+      until = turns * 3;
+      turns *= 4;
+    }
     uint64_t floor = h.floor;
-    float low = floor ? key_value(floor) : -3.402823466e38f;
+    float low = floor ? key_value(floor) : kLowest;
     uint32_t pending = 0;
-    if (best >= low)
 #pragma unroll
-      for (int i = 0; i < N; ++i) pending |= (v[i] >= low ? 1u : 0u) << i;
+    for (int i = 0; i < N; ++i) pending |= (v[i] >= low ? 1u : 0u) << i;
     for (;;) {  // as offer() does
       if (pending) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (pending >> i & 1u) {
-            const uint64_t key = key_of(v[i], static_cast<uint32_t>(a.first + c + (i / V) * V * 256 + threadIdx.x * V + i % V));
-            bool settled = key <= floor;
-            if (!settled) {
-              const uint32_t at = atomicAdd(&h.count, 1u);
-              settled = at < kKeys;
-              if (settled) h.key[at] = key;
-            }
-            if (settled) pending &= ~(1u << i);
+        for (int g = 0; g < N; g += 4)
+          if (pending >> g & 15u) {
+#pragma unroll
+            for (int i = g; i < g + 4; ++i)
+              if (pending >> i & 1u) {
+                const uint64_t key = key_of(v[i], static_cast<uint32_t>(a.first + c + (i / V) * V * 256 + threadIdx.x * V + i % V));
+                bool settled = key <= floor;
+                if (!settled) {
+                  const uint32_t at = atomicAdd(&h.count, 1u);
+                  settled = at < kKeys;
+                  if (settled) h.key[at] = key;
+                }
+                if (settled) pending &= ~(1u << i);
+              }
           }
       }
       if (!__syncthreads_or(pending != 0)) break;

@@ -462,7 +462,7 @@ typedef struct shine_flat_adjustment {
   uint64_t allow_ld;
   const int32_t* seen;     /* seen[i * seen_ld + 0 .. seen_n - 1]: record ids, repeats counted, others (-1) skipped */
   uint64_t seen_ld;
-  uint32_t seen_n;
+  uint32_t seen_n;         /* <= 65535 */
   uint32_t reserved0;
   const float* repetition; /* one number per row, > 0 (1: none) */
   const float* frequency;  /* one per row */

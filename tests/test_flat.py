@@ -87,6 +87,7 @@ def test_adjust_refusals():
     refused(f(0, P, 0, 4, 100, 100, adjustment(allow=P, allow_ld=3), P, 100, None), "allow row stride")
     refused(f(0, P, 0, 4, 100, 100, adjustment(seen_n=3), P, 100, None), "seen is NULL")
     refused(f(0, P, 0, 4, 100, 100, adjustment(seen=P, seen_n=3, seen_ld=2), P, 100, None), "seen row stride")
+    refused(f(0, P, 0, 4, 100, 100, adjustment(seen=P, seen_n=65536, seen_ld=65536), P, 100, None), "65535")
     refused(f(0, P, 0, 4, 100, 100, adjustment(bias=P + 2), P, 100, None), "4-byte")
     assert f(0, None, 0, 0, 100, 100, adjustment(), None, 100, None) == L.OK
     assert f(0, None, 0, 4, 0, 0, adjustment(), None, 0, None) == L.OK

@@ -320,6 +320,22 @@ def test_adjust_special_values(dtype):
     assert (ids[2] == -1).all() and (values[2] == NEG).all()
 
 
+def test_adjust_longest_history():
+    """65,535 ids of one record, beside one that shares its count's word and one met once"""
+    s = rows(2, 9000, 4)
+    seen = torch.full((2, 65535), 4098, dtype=torch.int32)
+    seen[1, :30000] = 4099
+    seen[1, 7] = 8999
+    arg = dict(seen=seen, frequency=torch.tensor([1e-3, 1.0]))
+    want, err = adjust64(s, **arg)
+    close(F().adjust(s.cuda(), **cuda(arg)), want, err, torch.float32)
+    table = F().FlatTable(rows(9000, 16, 1).cuda())
+    q = rows(2, 16, 2).cuda()
+    values, ids = F().search(table, q, 20, **cuda(arg))
+    v, i = F().topk(F().adjust(F().scores(table, q), **cuda(arg)), 20)
+    assert torch.equal(ids, i) and torch.equal(values, v)
+
+
 def test_adjust_strides():
     whole = rows(7, 999, 3).cuda()
     s = whole[1:5, 3:903]
