@@ -906,167 +906,238 @@ __device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
   if (at < a.cap) a.keys[query * a.cap + at] = key;
 }
 
+// Whether a score reaches the threshold is left to the matrix unit as well.  With the query's scale q and threshold l, the
+// record's scale x and bias b,
+//   (sum * q) * x + b >= l   <=>   sum + (b / x) (1 / q) - (1 / x) (l / q) >= 0,
+// a product of four numbers of the record with four of the query, added to a sum that is already there: kMagic + sum is a
+// float (kMagic's), so one 32x32x8 bf16 instruction takes it as its start and leaves the margin in units of the integer
+// sum, negative where the score fails.  Per score that leaves half a maximum to the vector unit, where scaling takes two
+// fused multiply-adds (1024 x 1M x 128: FIXME us a pass against 244).  A number goes in as two bf16 (2^-17 of it is
+// lost), a product as three; the margin is raised by kSlack counts and 2^-13 of its terms, more than this, the roundings of
+// the additions and those of the definition come to.  What passes is scored again as the definition rounds.
+//
+// The terms of a record, and what they meet in a query:
+//   1        -kMagic
+//   u hi     v hi      u = b / x, v = 1 / q
+//   u hi     v lo
+//   u lo     v hi
+//   w hi     y hi      w = 1 / x, y = -l / q
+//   w hi     y lo
+//   w lo     y hi
+//   slack    v hi
+constexpr int kSlack = 16;
+constexpr float kSumZero = kMagicF + kSlack;  // what a sum of 0 reads as
+
+struct Two {
+  __bf16 hi, lo;
+  __device__ explicit Two(float x) : hi(static_cast<__bf16>(x)), lo(static_cast<__bf16>(x - static_cast<float>(hi))) {}
+};
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+struct __attribute__((aligned(16))) Terms {
+  __bf16 t[8];
+};
+
+// A record for which the margin says nothing always passes (scales and biases whose quotients may overflow), one that is no
+// answer never does: its terms are u = +-1e20 alone.
+constexpr float kNear = 1e9f, kSure = 1e20f;
+__device__ inline Terms record_terms(float x, float b, bool on, float low_most) {
+  if (x == 0.0f) x = 1.0f;  // its codes and so its sums are 0, whatever they are scaled by
+  const bool none = !on || x != x || b != b || b == -__builtin_huge_valf();
+  const bool plain = x > 1.0f / kNear && x < kNear && fabsf(b) < kNear;
+  const float w = plain && !none ? 1.0f / x : 0.0f, u = none ? -kSure : plain ? b * w : kSure;
+  const float slack = plain && !none ? 0x1p-13f * (fabsf(u) + low_most * w) : 0.0f;
+  const Two a(u), c(w);
+  return {{static_cast<__bf16>(1.0f), a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(slack)}};
+}
+// `open`: no threshold to hold to.  Queries for which the margin says nothing meet nothing: every sum passes.
+__device__ inline bool query_plain(float q, float low) { return q > 1.0f / kNear && q < kNear && fabsf(low) < 1e15f; }
+__device__ inline Terms query_terms(float q, float low, bool there) {
+  const float zero = 0.0f;
+  if (!there || q != q) return {{static_cast<__bf16>(-2.0f * kMagicF), static_cast<__bf16>(zero)}};
+  if (!query_plain(q, low)) return {{static_cast<__bf16>(zero)}};
+  const Two v(1.0f / q), y(-low / q);
+  return {{static_cast<__bf16>(-kMagicF), v.hi, v.lo, v.hi, y.hi, y.lo, y.hi, v.hi}};
+}
+
 // What a wave knows of its 32 records, beside their codes.
 template <int QUERIES>
 struct Beside {
-  float xs[32], rough[32], tb[32], ab[32];  // rough: the biases' sum, raised by more than its roundings
-  uint32_t allow[QUERIES];                  // each query's word of its mask
+  Terms terms[32];
+  float xs[32], tb[32], ab[32];
+  uint32_t allow[QUERIES];  // each query's word of its mask
 };
 
-// Per score: one fused multiply-add (two with biases) and half a maximum.  (kMagic + sum) * xs - kMagic * xs is sum * xs
-// up to 1.75 xs (the rounding of kMagic * xs is 0.75, the other roundings of numbers below 2^22 xs less than 1), and the
-// definition's own roundings of near-threshold scores are below 2^-20 of the threshold, so scores that reach the
-// threshold also reach it here once 2 qs max(xs) is added.  What passes is scored again as the definition rounds, from
-// LDS alone: a load from memory there would wait for the next block's codes, which are on their way.
-//
-// The next block is fetched while this one is scored, with no branch around its loads (what is not given is read from the
-// scales and not used): behind a branch the loaded registers would be copied, and the copy would wait for the loads.
-template <int KC, int QT, bool BIAS, bool ROWS, bool STORE>
+// A wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32 queries: sum v
+// (0 .. 15) of lane l is of record 8 (v / 4) + 4 (l / 32) + v % 4 and query l % 32.  The next block is fetched while this one is
+// scored, with no branch around its loads (what is not given is read from the scales and not used): behind a branch the
+// loaded registers would be copied, and the copy would wait for the loads.  What passes is looked up in LDS alone: a load
+// from memory there would wait for the next block's codes as well.
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <int KC, int QT, bool ROWS, bool STORE>
 __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
-  __shared__ Beside<QT * 16> beside[4];
-  __shared__ uint64_t thr_key[QT * 16];
+  constexpr uint32_t kQueries = QT * 32;
+  constexpr int C = KC * 2;  // 32-byte steps of a row
+  __shared__ Beside<kQueries> beside[4];
+  __shared__ float qscale[kQueries], lowest[kQueries];
   __shared__ uint64_t list_key[STORE ? 1 : kListed];
-  __shared__ uint32_t list_place[STORE ? 1 : kListed];  // the query's number in the workgroup, and the key's among its keys << 8
-  __shared__ uint32_t found[QT * 16], base[QT * 16];
+  __shared__ uint32_t list_place[STORE ? 1 : kListed];  // the query's number in the workgroup, later the key's among its keys << 8
+  __shared__ uint32_t found[kQueries], base[kQueries];
   __shared__ uint32_t listed;
-  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 31, half = lane >> 5;
   const Place at = place_of(query_blocks);
-  const uint32_t query0 = at.query_block * QT * 16;
+  const uint32_t query0 = at.query_block * kQueries;
   const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
   if (b0 >= b1) return;  // the whole workgroup
   if (threadIdx.x == 0) listed = 0;
-  if (threadIdx.x < QT * 16) {
-    thr_key[threadIdx.x] = !STORE && query0 + threadIdx.x < a.nq ? a.thr[query0 + threadIdx.x] : 0;
+  if (threadIdx.x < kQueries) {
+    const uint32_t r = min(query0 + threadIdx.x, a.nq - 1);
+    const uint64_t key = STORE ? 0 : a.thr[r];
+    const float thr = key ? fminf(key_value(key), 3.4028e38f) : -__builtin_huge_valf();  // an infinite one as the largest
+    qscale[threadIdx.x] = a.qscales[r];
+    lowest[threadIdx.x] = thr - 0x1p-20f * fabsf(thr);
     found[threadIdx.x] = 0;
   }
-  v4i q[QT][KC];
-  load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
-  float qs[QT], low[QT];
-  __syncthreads();
+  v4i q[QT][C];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const uint32_t r = query0 + i * 16 + col;
-    qs[i] = a.qscales[r < a.nq ? r : a.nq - 1];
-    const uint64_t key = thr_key[i * 16 + col];
-    const float thr = key ? key_value(key) : -__builtin_huge_valf();
-    // scales far from 1 may overflow in one order of products and not in another: everything passes
-    low[i] = qs[i] > 1e-18f && qs[i] < 1e18f ? thr - 0x1p-20f * fabsf(thr) : -__builtin_huge_valf();
+    const int8_t* p = a.qcodes + static_cast<uint64_t>(min(query0 + i * 32 + col, a.nq - 1)) * (KC * 64) + half * 16;
+#pragma unroll
+    for (int c = 0; c < C; ++c) q[i][c] = *reinterpret_cast<const v4i*>(p + c * 32);
   }
-  // the next block: its codes, and lane l's part of what is beside record l (lanes 32 .. 63: of record l - 32)
-  constexpr int MASKS = (QT * 16 + 63) / 64;  // queries whose mask words a lane fetches
+  __syncthreads();
+  v4s qterms[QT];
+  float low_most = 0.0f;
+  if (!STORE) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      const uint32_t mine = i * 32 + col;
+      const Terms t = query_terms(qscale[mine], lowest[mine], query0 + mine < a.nq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qterms[i][e] = __builtin_bit_cast(short, half ? t.t[4 + e] : t.t[e]);
+      if (query_plain(qscale[mine], lowest[mine])) low_most = fmaxf(low_most, fabsf(lowest[mine]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low_most = fmaxf(low_most, __shfl_xor(low_most, o));
+  }
+  // the next block: its codes, and lane l's part of what is beside record l % 32
+  constexpr int MASKS = (kQueries + 63) / 64;  // queries whose mask words a lane fetches
   const float* tbias = a.tbias ? a.tbias : a.scales;
   const float* abias = a.abias ? a.abias : a.scales;
   const bool has_allow = a.allow, shared = !ROWS && has_allow;
   const uint32_t* allow_base = has_allow ? a.allow : reinterpret_cast<const uint32_t*>(a.scales);
   const uint32_t* allow_row[MASKS];
 #pragma unroll
-  for (int i = 0; i < MASKS; ++i) {
-    const uint32_t r = query0 + i * 64 + lane;
-    allow_row[i] = allow_base + (has_allow && ROWS ? (r < a.nq ? r : a.nq - 1) * a.allow_ld : 0);
-  }
-  Block<KC> next;
-  float next_xs, next_tb = 0.0f, next_ab = 0.0f;
+  for (int i = 0; i < MASKS; ++i) allow_row[i] = allow_base + (ROWS ? min(query0 + i * 64 + lane, a.nq - 1) * a.allow_ld : 0);
+  const uint64_t last = b1 - 1;
+  v4i next[C];
+  float next_xs, next_tb, next_ab;
   uint32_t next_allow[MASKS];
   auto fetch = [&](uint64_t b) {
-    const uint64_t word = b * a.stride, r = word * 32 + (lane & 31), at = r < a.n ? r : a.n - 1;
-    load_block<KC>(next, a.codes, word * 32, a.n);
-    next_xs = a.scales[at];
-    if (BIAS) {
-      next_tb = tbias[at];
-      next_ab = abias[at];
-    }
+    const uint64_t word = min(b, last) * a.stride, r0 = word * 32;
+    const uint32_t mine = min(col, static_cast<uint32_t>(min(a.n - r0, static_cast<uint64_t>(32))) - 1);
+    const int8_t* p = a.codes + r0 * (KC * 64);
+#pragma unroll
+    for (int c = 0; c < C; ++c) next[c] = *reinterpret_cast<const v4i*>(p + mine * (KC * 64) + half * 16 + c * 32);
+    next_xs = (a.scales + r0)[mine];
+    next_tb = (tbias + r0)[mine];
+    next_ab = (abias + r0)[mine];
 #pragma unroll
     for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][has_allow ? word : 0];
   };
-  const v4i start = magic_start();
-  const uint64_t last = b1 - 1;
-  fetch(b0 + wave < b1 ? b0 + wave : last);
+  v16i start;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) start[v] = kMagic + kSlack;
+  asm volatile("" : "+v"(start));  // registers of its own, not filled anew for every product
+  fetch(b0 + wave);
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
-    const Block<KC> x = next;
+    v4i x[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = next[c];
     const uint64_t word = b * a.stride;
     uint32_t live = ~0u;  // records of the block that are there and that the shared mask allows
     if (word * 32 + 32 > a.n) live >>= 32 - static_cast<uint32_t>(a.n - word * 32);
     if (shared) live &= next_allow[0];
-    Beside<QT * 16>& s = beside[wave];
-    if (lane < 32) {
+    Beside<kQueries>& s = beside[wave];
+    if (half == 0) {
+      const float tb = a.tbias ? next_tb : 0.0f, ab = a.abias ? next_ab : 0.0f;
+      if (!STORE) s.terms[lane] = record_terms(next_xs, tb + ab, live >> lane & 1u, low_most);
       s.xs[lane] = next_xs;
-      if (BIAS) {
-        if (!a.tbias) next_tb = 0.0f;
-        if (!a.abias) next_ab = 0.0f;
-        s.rough[lane] = live >> lane & 1u ? (next_tb + next_ab) + 0x1p-21f * (fabsf(next_tb) + fabsf(next_ab)) : -__builtin_huge_valf();
-        s.tb[lane] = next_tb;
-        s.ab[lane] = next_ab;
-      }
+      s.tb[lane] = tb;
+      s.ab[lane] = ab;
     }
     if (ROWS) {
 #pragma unroll
       for (int i = 0; i < MASKS; ++i)
-        if (i * 64 + lane < QT * 16) s.allow[i * 64 + lane] = has_allow ? next_allow[i] : ~0u;
+        if (i * 64 + lane < kQueries) s.allow[i * 64 + lane] = next_allow[i];
     }
-    const bool odd = __any((next_xs < 1e-18f && next_xs != 0.0f) || next_xs >= 1e18f);
     wave_sync();
-    fetch(b + 4 < b1 ? b + 4 : last);
-    float xs[8], off[8], bias[8], top = 0.0f;
+    fetch(b + 4);
+    v4s xterms;
+    if (!STORE) xterms = *reinterpret_cast<const v4s*>(&s.terms[col].t[half * 4]);
+    auto products = [&](const v4i(&q)[C], v16i& sum) {
+      sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[0], q[0], start, 0, 0, 0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      xs[j] = s.xs[group * 8 + j];
-      off[j] = -kMagicF * xs[j];
-      top = fmaxf(top, xs[j]);
-      if (BIAS) bias[j] = s.rough[group * 8 + j];
-    }
-    const float slack = odd ? __builtin_huge_valf() : 2.0f * top;
-    float ahead[8];  // the next tile's sums: the matrix unit works on them while this tile's are looked at
-    sums<KC>(x, q[0], start, ahead);
+      for (int c = 1; c < C; ++c) sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[c], q[c], sum, 0, 0, 0);
+    };
+    // the bits of `words` that are of this lane's records, sum v's in bit v
+    auto of_lane = [&](uint32_t words) {
+      words >>= half * 4;
+      return (words & 15u) | (words >> 4 & 0xF0u) | (words >> 8 & 0xF00u) | (words >> 12 & 0xF000u);
+    };
+    v16i ahead;  // the next tile's sums: the matrix unit works on them while this tile's are looked at
+    products(q[0], ahead);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      float f[8], t[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = ahead[j];
-      if (i + 1 < QT) sums<KC>(x, q[i + 1 < QT ? i + 1 : 0], start, ahead);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        t[j] = fmaf(f[j], xs[j], off[j]);
-        t[j] = BIAS ? fmaf(t[j], qs[i], bias[j]) : t[j];
-      }
-      float best = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
-      best = BIAS ? fmaf(qs[i], slack, best) : (best + slack) * qs[i];
-      const uint32_t query = query0 + i * 16 + col;
+      const v16i sum = ahead;
+      v16f margin;
+      if (!STORE) margin = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(xterms, qterms[i], __builtin_bit_cast(v16f, sum), 0, 0, 0);
+      if (i + 1 < QT) products(q[i + 1 < QT ? i + 1 : 0], ahead);
+      const uint32_t mine = i * 32 + col, query = query0 + mine;
       if (STORE) {
         if (query < a.nq) {
-          ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + group * 8);
+          ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + half * 4);
+          const uint32_t on = ROWS ? live & s.allow[mine] : live;
+          const float qs = qscale[mine];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
+          for (int v = 0; v < 16; v += 2) {
             uint64_t key[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t r = group * 8 + j + e;
-              const float v = exact_score(f[j + e] - kMagicF, qs[i], xs[j + e], a, BIAS ? s.tb[r] : 0.0f, BIAS ? s.ab[r] : 0.0f);
-              key[e] = (ROWS ? live & s.allow[i * 16 + col] : live) >> r & 1u ? offered_key(v, word * 32 + r) : 0;
+              const uint32_t r = (v >> 2) * 8 + half * 4 + (v & 3) + e;
+              const float score = exact_score(__int_as_float(sum[v + e]) - kSumZero, qs, s.xs[r], a, s.tb[r], s.ab[r]);
+              key[e] = on >> r & 1u ? offered_key(score, word * 32 + r) : 0;
             }
-            to[j / 2] = make_ulonglong2(key[0], key[1]);
+            to[(v >> 2) * 4 + (v & 3) / 2] = make_ulonglong2(key[0], key[1]);
           }
         }
-      } else if (!(best < low[i])) {  // a NaN passes and is refused below
-        const float under = BIAS ? fmaf(-qs[i], slack, low[i]) : low[i];
-        uint32_t maybe = 0;
+      } else {
+        int some = -1;  // negative as long as all margins are: a float's sign is its bits' as an integer
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) maybe |= ((BIAS ? t[j] : (t[j] + slack) * qs[i]) < under ? 0u : 1u) << j;
-        maybe &= query < a.nq ? (ROWS ? live & s.allow[i * 16 + col] : live) >> (group * 8) : 0u;
-        while (maybe) {
-          const uint32_t j = __builtin_ctz(maybe), r = group * 8 + j;
-          maybe &= maybe - 1;
-          float sum = f[0];
+        for (int v = 0; v < 16; ++v) some = max(some, __float_as_int(margin[v]));
+        if (some >= 0) {
+          uint32_t maybe = 0;
 #pragma unroll
-          for (uint32_t e = 1; e < 8; ++e) sum = j == e ? f[e] : sum;
-          const float v = exact_score(sum - kMagicF, qs[i], s.xs[r], a, BIAS ? s.tb[r] : 0.0f, BIAS ? s.ab[r] : 0.0f);
-          const uint64_t key = offered_key(v, word * 32 + r);
-          if (key && key >= thr_key[i * 16 + col]) {  // the threshold's own record is met again
-            const uint32_t to = atomicAdd(&listed, 1u);
-            if (to < kListed) {
-              list_key[to] = key;
-              list_place[to] = (i * 16 + col) | atomicAdd(&found[i * 16 + col], 1u) << 8;
-            } else {
-              append(a, query, key);
+          for (uint32_t v = 0; v < 16; ++v) maybe |= (__float_as_int(margin[v]) >= 0 ? 1u : 0u) << v;
+          maybe &= query < a.nq ? of_lane(ROWS ? live & s.allow[mine] : live) : 0u;
+          while (maybe) {
+            const uint32_t v = __builtin_ctz(maybe), r = (v >> 2) * 8 + half * 4 + (v & 3);
+            maybe &= maybe - 1;
+            int bits = sum[0];
+#pragma unroll
+            for (uint32_t e = 1; e < 16; ++e) bits = v == e ? sum[e] : bits;
+            const float score = exact_score(__int_as_float(bits) - kSumZero, qscale[mine], s.xs[r], a, s.tb[r], s.ab[r]);
+            const uint64_t key = offered_key(score, word * 32 + r);
+            if (key && score >= lowest[mine]) {  // from a little below the threshold on: the selection sees to the rest
+              const uint32_t to = atomicAdd(&listed, 1u);
+              if (to < kListed) {
+                list_key[to] = key;
+                list_place[to] = mine;
+              } else {
+                append(a, query, key);
+              }
             }
           }
         }
@@ -1076,10 +1147,11 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   }
   if (STORE) return;
   __syncthreads();
-  const uint32_t t = threadIdx.x;
-  if (t < QT * 16 && found[t]) base[t] = atomicAdd(&a.count[(query0 + t) * kCountStride], found[t]);
+  const uint32_t t = threadIdx.x, m = listed < kListed ? listed : kListed;
+  for (uint32_t i = t; i < m; i += 256) list_place[i] |= atomicAdd(&found[list_place[i]], 1u) << 8;
   __syncthreads();
-  const uint32_t m = listed < kListed ? listed : kListed;
+  if (t < kQueries && found[t]) base[t] = atomicAdd(&a.count[(query0 + t) * kCountStride], found[t]);
+  __syncthreads();
   for (uint32_t i = t; i < m; i += 256) {
     const uint32_t mine = list_place[i] & 255u;
     const uint64_t to = static_cast<uint64_t>(base[mine]) + (list_place[i] >> 8);
@@ -1288,26 +1360,24 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
 
 constexpr uint32_t kPassGroups = 512;  // two workgroups a CU
 hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
-  const bool rows = a.allow && a.allow_ld, bias = a.tbias || a.abias || (a.allow && !rows);
-#define SHINE_FOR(KK, QQ, BB, RR, SS)                                                                      \
-  if (bias == BB && rows == RR && a.store == SS)                                                           \
-    hipLaunchKernelGGL((pass_kernel<KK, QQ, BB, RR, SS>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+  const bool rows = a.allow && a.allow_ld;
+#define SHINE_FOR(KK, QQ, RR, SS)                                                                          \
+  if (rows == RR && a.store == SS)                                                                         \
+    hipLaunchKernelGGL((pass_kernel<KK, QQ, RR, SS>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
 #define SHINE_PASS(KK, QQ)                                                                                 \
   {                                                                                                        \
-    const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                  \
-    const Ranges r = ranges_of(a.blocks, qb, kPassGroups);                                                        \
-    SHINE_FOR(KK, QQ, true, true, true) SHINE_FOR(KK, QQ, true, true, false)                               \
-    SHINE_FOR(KK, QQ, true, false, true) SHINE_FOR(KK, QQ, true, false, false)                             \
-    SHINE_FOR(KK, QQ, false, true, true) SHINE_FOR(KK, QQ, false, true, false)                             \
-    SHINE_FOR(KK, QQ, false, false, true) SHINE_FOR(KK, QQ, false, false, false)                           \
+    const uint32_t qb = (a.nq + QQ * 32 - 1) / (QQ * 32);                                                  \
+    const Ranges r = ranges_of(a.blocks, qb, kPassGroups);                                                 \
+    SHINE_FOR(KK, QQ, true, true) SHINE_FOR(KK, QQ, true, false)                                           \
+    SHINE_FOR(KK, QQ, false, true) SHINE_FOR(KK, QQ, false, false)                                         \
   }
 #define SHINE_KC(KK, BIG) \
-  if (a.nq <= 32) SHINE_PASS(KK, 2) else SHINE_PASS(KK, BIG)
+  if (a.nq <= 32) SHINE_PASS(KK, 1) else SHINE_PASS(KK, BIG)
   switch (a.pitch / 64) {
-    case 1: SHINE_KC(1, 8); break;
-    case 2: SHINE_KC(2, 8); break;
-    case 3: SHINE_KC(3, 4); break;
-    case 4: SHINE_KC(4, 4); break;
+    case 1: SHINE_KC(1, 4); break;
+    case 2: SHINE_KC(2, 4); break;
+    case 3: SHINE_KC(3, 2); break;
+    case 4: SHINE_KC(4, 2); break;
     default: return hipErrorInvalidValue;
   }
 #undef SHINE_KC
