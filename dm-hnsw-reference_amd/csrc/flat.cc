@@ -115,7 +115,7 @@ struct SearchPlan {
   uint32_t chunks, slices;
   uint32_t passes;     // fused
   uint64_t stride[kMaxPasses], cap, words;
-  uint64_t codes, scales, scores, keys, thr, count, mask, extra, extra_count, total;  // offsets into the workspace
+  uint64_t codes, scales, scores, keys, terms, query_terms, limit, count, mask, extra, extra_count, total;  // offsets into the workspace
 };
 
 // Fused passes cost less than the score matrix once it is larger than the table: from 17 queries on.  A bias for each row
@@ -169,7 +169,9 @@ SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const 
   p.scales = take(4ull * p.rows);
   if (p.fused) {
     p.keys = take(8 * p.cap * p.rows);
-    p.thr = take(8ull * p.rows);
+    if (p.passes > 1) p.terms = take(F::kTermBytes * 32ull * p.words);
+    p.query_terms = take(static_cast<uint64_t>(F::kTermBytes) * p.rows);
+    p.limit = take(4ull * p.rows);
     p.count = take(4ull * F::kCountStride * p.rows);
     if (seen_n) {
       p.mask = take(4 * p.words * p.rows);
@@ -195,7 +197,9 @@ hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const sh
   pass.nq = m;
   pass.pitch = F::code_pitch(t.dim);
   pass.n = t.n;
-  pass.thr = reinterpret_cast<uint64_t*>(ws + p.thr);
+  pass.record_terms = ws + p.terms;
+  pass.query_terms = ws + p.query_terms;
+  pass.limit = reinterpret_cast<int32_t*>(ws + p.limit);
   pass.count = reinterpret_cast<uint32_t*>(ws + p.count);
   pass.keys = reinterpret_cast<uint64_t*>(ws + p.keys);
   pass.cap = p.cap;
@@ -227,18 +231,19 @@ hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const sh
       sel.extra_ld = seen.extra_ld;
     }
   }
+  if (p.passes > 1 && q == 0)  // the records' terms are the same for all blocks of rows
+    if (hipError_t e = F::launch_terms(pass, s); e != hipSuccess) return e;
   const uint64_t* extra = sel.extra;
   for (uint32_t i = 0; i < p.passes; ++i) {
     const bool last = i + 1 == p.passes;
     pass.stride = p.stride[i];
     pass.blocks = (p.words + pass.stride - 1) / pass.stride;
-    pass.store = i == 0;
-    if (hipError_t e = F::launch_pass(pass, s); e != hipSuccess) return e;
+    if (hipError_t e = i ? F::launch_pass(pass, s) : F::launch_sample(pass, s); e != hipSuccess) return e;
     sel.pass = pass;
     sel.k = k;
     sel.fixed = i == 0 ? pass.blocks * 32 : 0;
     sel.extra = last ? extra : nullptr;
-    sel.thr = last ? nullptr : const_cast<uint64_t*>(pass.thr);
+    sel.last = last;
     sel.values = values;
     sel.ids = ids;
     if (hipError_t e = F::launch_select(sel, s); e != hipSuccess) return e;

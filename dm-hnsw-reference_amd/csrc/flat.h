@@ -39,6 +39,7 @@ struct ScoresArgs {
 };
 
 constexpr uint32_t kCountStride = 32;  // queries' counts lie in memory lines of their own: all XCDs add to them
+constexpr uint32_t kTermBytes = 16;    // of a record or a query in the threshold test
 
 // One pass of a fused search over every `stride`-th block of 32 records.
 struct PassArgs {
@@ -54,22 +55,26 @@ struct PassArgs {
   uint64_t n;
   uint64_t blocks;        // ceil(ceil(n / 32) / stride): blocks of this pass
   uint64_t stride;
-  bool store;             // every key at keys[q * cap + 32 * block + i]; else those from thr on, appended
-  const uint64_t* thr;    // per query; key 0: none
-  uint32_t* count;        // query q's at q * kCountStride: keys offered to its list (may pass cap; the list then holds cap of them)
+  // the coarsest pass: every key at keys[q * cap + 32 * block + i]
   uint64_t* keys;
   uint64_t cap;
+  // the others: what may reach the threshold is listed at keys[q * cap + 0 .. count - 1] as a record (low word: the first one)
+  // and 16 bits, v for record 8 (v / 4) + v % 4 behind it
+  const void* record_terms;  // of all records, whole blocks
+  void* query_terms;
+  int32_t* limit;            // per query
+  uint32_t* count;           // query q's at q * kCountStride (may pass cap; the list then holds cap entries)
 };
 
-// Selection from a search's lists: the k-th best key (thr) between passes, the answers behind the last one.
+// Selection from a search's lists: the k-th best key between passes, the answers behind the last one.
 struct SelectArgs {
-  PassArgs pass;          // what a row whose list overflowed is scanned again with (answers only)
+  PassArgs pass;          // what a row's scores are computed with
   uint32_t k;
-  uint64_t fixed;         // keys of every list, or 0: count[q]
+  uint64_t fixed;         // keys of every list, or 0: count[q] entries
   const uint64_t* extra;  // nullable: extra_count[q] more keys at extra + q * extra_ld
   const uint32_t* extra_count;
   uint64_t extra_ld;
-  uint64_t* thr;          // not nullptr: write the k-th best key and clear count
+  bool last;              // write the answers; else thr, limit and query_terms, and clear count
   float* values;
   int32_t* ids;
 };
@@ -133,6 +138,8 @@ uint32_t topk_slices(uint32_t nq, uint64_t n);
 
 hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s);
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s);
+hipError_t launch_terms(const PassArgs& a, hipStream_t s);  // record_terms, as allow (shared), scales and biases have them
+hipError_t launch_sample(const PassArgs& a, hipStream_t s);
 hipError_t launch_pass(const PassArgs& a, hipStream_t s);
 hipError_t launch_select(const SelectArgs& a, hipStream_t s);
 hipError_t launch_seen(const SeenArgs& a, hipStream_t s);

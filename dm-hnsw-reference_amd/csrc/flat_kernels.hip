@@ -897,34 +897,27 @@ __device__ inline uint64_t offered_key(float v, uint64_t record) {
   return v >= -3.402823466e38f ? key_of(v, static_cast<uint32_t>(record)) : 0;
 }
 
-// Keys that a workgroup lists in LDS.  They go to the queries' lists together, with one addition to each query's count:
-// additions to one address from all over the GPU are served one after another.
-constexpr uint32_t kListed = 4096;
-
-__device__ inline void append(const PassArgs& a, uint32_t query, uint64_t key) {
-  const uint32_t at = atomicAdd(&a.count[query * kCountStride], 1u);
-  if (at < a.cap) a.keys[query * a.cap + at] = key;
-}
-
 // Whether a score reaches the threshold is left to the matrix unit as well.  With the query's scale q and threshold l, the
 // record's scale x and bias b,
 //   (sum * q) * x + b >= l   <=>   sum + (b / x) (1 / q) - (1 / x) (l / q) >= 0,
 // a product of four numbers of the record with four of the query, added to a sum that is already there: kMagic + sum is a
 // float (kMagic's), so one 32x32x8 bf16 instruction takes it as its start and leaves the margin in units of the integer
-// sum, negative where the score fails.  Per score that leaves half a maximum to the vector unit, where scaling takes two
+// sum.  Per score that leaves half a maximum to the vector unit, where scaling takes two
 // fused multiply-adds (1024 x 1M x 128: FIXME us a pass against 244).  A number goes in as two bf16 (2^-17 of it is
 // lost), a product as three; the margin is raised by kSlack counts and 2^-13 of its terms, more than this, the roundings of
 // the additions and those of the definition come to.  What passes is scored again as the definition rounds.
 //
 // The terms of a record, and what they meet in a query:
-//   1        -kMagic
-//   u hi     v hi      u = b / x, v = 1 / q
-//   u hi     v lo
-//   u lo     v hi
-//   w hi     y hi      w = 1 / x, y = -l / q
-//   w hi     y lo
-//   w lo     y hi
-//   slack    v hi
+//   u hi          v hi      u = b / x, v = 1 / q
+//   u hi          v lo
+//   u lo          v hi
+//   w hi          y hi      w = 1 / x, y = -l / q
+//   w hi          y lo
+//   w lo          y hi
+//   2^-13 |u|     v hi
+//   2^-13 w       |y hi|
+// The margin still has kMagic in it: the score fails where it is below kMagic, for floats of which some are positive and for
+// their bits as integers alike.
 constexpr int kSlack = 16;
 constexpr float kSumZero = kMagicF + kSlack;  // what a sum of 0 reads as
 
@@ -933,275 +926,336 @@ struct Two {
   __device__ explicit Two(float x) : hi(static_cast<__bf16>(x)), lo(static_cast<__bf16>(x - static_cast<float>(hi))) {}
 };
 typedef short v4s __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 struct __attribute__((aligned(16))) Terms {
   __bf16 t[8];
 };
 
 // A record for which the margin says nothing always passes (scales and biases whose quotients may overflow), one that is no
-// answer never does: its terms are u = +-1e20 alone.
+// answer never does: its terms are u = +-1e20 alone.  The reciprocals are within 2^-22.
 constexpr float kNear = 1e9f, kSure = 1e20f;
-__device__ inline Terms record_terms(float x, float b, bool on, float low_most) {
-  if (x == 0.0f) x = 1.0f;  // its codes and so its sums are 0, whatever they are scaled by
-  const bool none = !on || x != x || b != b || b == -__builtin_huge_valf();
-  const bool plain = x > 1.0f / kNear && x < kNear && fabsf(b) < kNear;
-  const float w = plain && !none ? 1.0f / x : 0.0f, u = none ? -kSure : plain ? b * w : kSure;
-  const float slack = plain && !none ? 0x1p-13f * (fabsf(u) + low_most * w) : 0.0f;
+__device__ inline Terms record_terms(float x, float b, bool on) {
+  x = x == 0.0f ? 1.0f : x;  // its codes and so its sums are 0, whatever they are scaled by
+  const bool plain = on && x > 1.0f / kNear && x < kNear && fabsf(b) < kNear;
+  const bool none = !on || x != x || !(b > -__builtin_huge_valf());
+  const float w = plain ? __builtin_amdgcn_rcpf(x) : 0.0f, u = plain ? b * w : none ? -kSure : kSure;
   const Two a(u), c(w);
-  return {{static_cast<__bf16>(1.0f), a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(slack)}};
+  return {{a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(plain ? 0x1p-13f * fabsf(u) : 0.0f), static_cast<__bf16>(0x1p-13f * w)}};
 }
-// `open`: no threshold to hold to.  Queries for which the margin says nothing meet nothing: every sum passes.
+// Queries for which the margin says nothing (no threshold yet, scales or thresholds whose quotients may overflow) have no
+// terms, and a limit that every margin reaches; those that are not there or have no scale one that none does.
 __device__ inline bool query_plain(float q, float low) { return q > 1.0f / kNear && q < kNear && fabsf(low) < 1e15f; }
-__device__ inline Terms query_terms(float q, float low, bool there) {
-  const float zero = 0.0f;
-  if (!there || q != q) return {{static_cast<__bf16>(-2.0f * kMagicF), static_cast<__bf16>(zero)}};
-  if (!query_plain(q, low)) return {{static_cast<__bf16>(zero)}};
+__device__ inline Terms query_terms(float q, float low) {
+  if (!query_plain(q, low)) return {{static_cast<__bf16>(0.0f)}};
   const Two v(1.0f / q), y(-low / q);
-  return {{static_cast<__bf16>(-kMagicF), v.hi, v.lo, v.hi, y.hi, y.lo, y.hi, v.hi}};
+  return {{v.hi, v.lo, v.hi, y.hi, y.lo, y.hi, v.hi, static_cast<__bf16>(fabsf(static_cast<float>(y.hi)))}};
+}
+__device__ inline int query_limit(float q, float low, bool there) {
+  return !there || q != q ? 0x7FFFFFFF : query_plain(q, low) ? kMagic : -0x7FFFFFFF - 1;
 }
 
-// What a wave knows of its 32 records, beside their codes.
-template <int QUERIES>
-struct Beside {
-  Terms terms[32];
-  float xs[32], tb[32], ab[32];
-  uint32_t allow[QUERIES];  // each query's word of its mask
-};
+__global__ __launch_bounds__(256) void terms_kernel(PassArgs a, Terms* out) {
+  const uint64_t r = blockIdx.x * 256ull + threadIdx.x;
+  if (r >= (a.n + 31) / 32 * 32) return;
+  const uint64_t at = min(r, a.n - 1);
+  const bool on = r < a.n && (!a.allow || a.allow_ld || (a.allow[r >> 5] >> (r & 31) & 1u));
+  out[r] = record_terms(a.scales[at], (a.tbias ? a.tbias[at] : 0.0f) + (a.abias ? a.abias[at] : 0.0f), on);
+}
 
-// A wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32 queries: sum v
-// (0 .. 15) of lane l is of record 8 (v / 4) + 4 (l / 32) + v % 4 and query l % 32.  The next block is fetched while this one is
-// scored, with no branch around its loads (what is not given is read from the scales and not used): behind a branch the
-// loaded registers would be copied, and the copy would wait for the loads.  What passes is looked up in LDS alone: a load
-// from memory there would wait for the next block's codes as well.
+// Both passes: a wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32
+// queries: sum v (0 .. 15) of lane l is of record 8 (v / 4) + 4 (l / 32) + v % 4 and query l % 32.  The next block is fetched while
+// this one is scored, with no branch around its loads: behind a branch the loaded registers would be copied, and the copy
+// would wait for the loads.
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-template <int KC, int QT, bool ROWS, bool STORE>
-__global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
-  constexpr uint32_t kQueries = QT * 32;
-  constexpr int C = KC * 2;  // 32-byte steps of a row
-  __shared__ Beside<kQueries> beside[4];
-  __shared__ float qscale[kQueries], lowest[kQueries];
-  __shared__ uint64_t list_key[STORE ? 1 : kListed];
-  __shared__ uint32_t list_place[STORE ? 1 : kListed];  // the query's number in the workgroup, later the key's among its keys << 8
-  __shared__ uint32_t found[kQueries], base[kQueries];
-  __shared__ uint32_t listed;
-  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 31, half = lane >> 5;
-  const Place at = place_of(query_blocks);
-  const uint32_t query0 = at.query_block * kQueries;
-  const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
-  if (b0 >= b1) return;  // the whole workgroup
-  if (threadIdx.x == 0) listed = 0;
-  if (threadIdx.x < kQueries) {
-    const uint32_t r = min(query0 + threadIdx.x, a.nq - 1);
-    const uint64_t key = STORE ? 0 : a.thr[r];
-    const float thr = key ? fminf(key_value(key), 3.4028e38f) : -__builtin_huge_valf();  // an infinite one as the largest
-    qscale[threadIdx.x] = a.qscales[r];
-    lowest[threadIdx.x] = thr - 0x1p-20f * fabsf(thr);
-    found[threadIdx.x] = 0;
-  }
-  v4i q[QT][C];
+template <int C, int QT>
+__device__ inline void load_tile_queries(v4i (&q)[QT][C], const PassArgs& a, uint32_t query0) {
+  const uint32_t col = threadIdx.x & 31, half = threadIdx.x >> 5 & 1;
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const int8_t* p = a.qcodes + static_cast<uint64_t>(min(query0 + i * 32 + col, a.nq - 1)) * (KC * 64) + half * 16;
+    const int8_t* p = a.qcodes + static_cast<uint64_t>(min(query0 + i * 32 + col, a.nq - 1)) * (C * 32) + half * 16;
 #pragma unroll
     for (int c = 0; c < C; ++c) q[i][c] = *reinterpret_cast<const v4i*>(p + c * 32);
   }
-  __syncthreads();
-  v4s qterms[QT];
-  float low_most = 0.0f;
-  if (!STORE) {
+}
+__device__ inline uint32_t records_of(const PassArgs& a, uint64_t word) {
+  return static_cast<uint32_t>(min(a.n - word * 32, static_cast<uint64_t>(32)));
+}
+template <int C>
+__device__ inline void load_tile_block(v4i (&x)[C], const PassArgs& a, uint64_t word) {
+  const uint32_t col = threadIdx.x & 31, half = threadIdx.x >> 5 & 1;
+  const uint32_t at = min(col, records_of(a, word) - 1) * (C * 32) + half * 16;  // behind the last record: the last one
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-      const uint32_t mine = i * 32 + col;
-      const Terms t = query_terms(qscale[mine], lowest[mine], query0 + mine < a.nq);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qterms[i][e] = __builtin_bit_cast(short, half ? t.t[4 + e] : t.t[e]);
-      if (query_plain(qscale[mine], lowest[mine])) low_most = fmaxf(low_most, fabsf(lowest[mine]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) low_most = fmaxf(low_most, __shfl_xor(low_most, o));
-  }
-  // the next block: its codes, and lane l's part of what is beside record l % 32
-  constexpr int MASKS = (kQueries + 63) / 64;  // queries whose mask words a lane fetches
-  const float* tbias = a.tbias ? a.tbias : a.scales;
-  const float* abias = a.abias ? a.abias : a.scales;
-  const bool has_allow = a.allow, shared = !ROWS && has_allow;
-  const uint32_t* allow_base = has_allow ? a.allow : reinterpret_cast<const uint32_t*>(a.scales);
-  const uint32_t* allow_row[MASKS];
-#pragma unroll
-  for (int i = 0; i < MASKS; ++i) allow_row[i] = allow_base + (ROWS ? min(query0 + i * 64 + lane, a.nq - 1) * a.allow_ld : 0);
-  const uint64_t last = b1 - 1;
-  v4i next[C];
-  float next_xs, next_tb, next_ab;
-  uint32_t next_allow[MASKS];
-  auto fetch = [&](uint64_t b) {
-    const uint64_t word = min(b, last) * a.stride, r0 = word * 32;
-    const uint32_t mine = min(col, static_cast<uint32_t>(min(a.n - r0, static_cast<uint64_t>(32))) - 1);
-    const int8_t* p = a.codes + r0 * (KC * 64);
-#pragma unroll
-    for (int c = 0; c < C; ++c) next[c] = *reinterpret_cast<const v4i*>(p + mine * (KC * 64) + half * 16 + c * 32);
-    next_xs = (a.scales + r0)[mine];
-    next_tb = (tbias + r0)[mine];
-    next_ab = (abias + r0)[mine];
-#pragma unroll
-    for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][has_allow ? word : 0];
-  };
+  for (int c = 0; c < C; ++c) x[c] = *reinterpret_cast<const v4i*>(a.codes + word * (32 * C * 32) + at + c * 32);
+}
+__device__ inline v16i sums_start() {  // registers of its own, not filled anew for every product
   v16i start;
 #pragma unroll
   for (int v = 0; v < 16; ++v) start[v] = kMagic + kSlack;
-  asm volatile("" : "+v"(start));  // registers of its own, not filled anew for every product
-  fetch(b0 + wave);
+  asm volatile("" : "+v"(start));
+  return start;
+}
+template <int C>
+__device__ inline v16i tile_sums(const v4i (&x)[C], const v4i (&q)[C], const v16i& start) {
+  v16i sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[0], q[0], start, 0, 0, 0);
+#pragma unroll
+  for (int c = 1; c < C; ++c) sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[c], q[c], sum, 0, 0, 0);
+  return sum;
+}
+
+// The coarsest pass: a few thousand records of every query, all of whose keys are stored.
+template <int KC, int QT>
+__global__ __launch_bounds__(256, 2) void sample_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
+  constexpr int C = KC * 2;
+  __shared__ float beside[4][3][32];
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 31, half = lane >> 5;
+  const Place at = place_of(query_blocks);
+  const uint32_t query0 = at.query_block * QT * 32;
+  const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks;
+  if (b0 + wave >= b1) return;
+  v4i q[QT][C];
+  load_tile_queries<C, QT>(q, a, query0);
+  float qs[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) qs[i] = a.qscales[min(query0 + i * 32 + col, a.nq - 1)];
+  const v16i start = sums_start();
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
+    const uint64_t word = b * a.stride, mine = word * 32 + min(col, records_of(a, word) - 1);
     v4i x[C];
+    load_tile_block<C>(x, a, word);
+    uint32_t allow[QT];
 #pragma unroll
-    for (int c = 0; c < C; ++c) x[c] = next[c];
-    const uint64_t word = b * a.stride;
-    uint32_t live = ~0u;  // records of the block that are there and that the shared mask allows
-    if (word * 32 + 32 > a.n) live >>= 32 - static_cast<uint32_t>(a.n - word * 32);
-    if (shared) live &= next_allow[0];
-    Beside<kQueries>& s = beside[wave];
+    for (int i = 0; i < QT; ++i)
+      allow[i] = a.allow ? a.allow[min(query0 + i * 32 + col, a.nq - 1) * a.allow_ld + word] : ~0u;
     if (half == 0) {
-      const float tb = a.tbias ? next_tb : 0.0f, ab = a.abias ? next_ab : 0.0f;
-      if (!STORE) s.terms[lane] = record_terms(next_xs, tb + ab, live >> lane & 1u, low_most);
-      s.xs[lane] = next_xs;
-      s.tb[lane] = tb;
-      s.ab[lane] = ab;
-    }
-    if (ROWS) {
-#pragma unroll
-      for (int i = 0; i < MASKS; ++i)
-        if (i * 64 + lane < kQueries) s.allow[i * 64 + lane] = next_allow[i];
+      beside[wave][0][col] = a.scales[mine];
+      beside[wave][1][col] = a.tbias ? a.tbias[mine] : 0.0f;
+      beside[wave][2][col] = a.abias ? a.abias[mine] : 0.0f;
     }
     wave_sync();
-    fetch(b + 4);
-    v4s xterms;
-    if (!STORE) xterms = *reinterpret_cast<const v4s*>(&s.terms[col].t[half * 4]);
-    auto products = [&](const v4i(&q)[C], v16i& sum) {
-      sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[0], q[0], start, 0, 0, 0);
-#pragma unroll
-      for (int c = 1; c < C; ++c) sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[c], q[c], sum, 0, 0, 0);
-    };
-    // the bits of `words` that are of this lane's records, sum v's in bit v
-    auto of_lane = [&](uint32_t words) {
-      words >>= half * 4;
-      return (words & 15u) | (words >> 4 & 0xF0u) | (words >> 8 & 0xF00u) | (words >> 12 & 0xF000u);
-    };
-    v16i ahead;  // the next tile's sums: the matrix unit works on them while this tile's are looked at
-    products(q[0], ahead);
+    const uint32_t there = records_of(a, word) == 32 ? ~0u : (1u << records_of(a, word)) - 1;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      const v16i sum = ahead;
-      v16f margin;
-      if (!STORE) margin = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(xterms, qterms[i], __builtin_bit_cast(v16f, sum), 0, 0, 0);
-      if (i + 1 < QT) products(q[i + 1 < QT ? i + 1 : 0], ahead);
-      const uint32_t mine = i * 32 + col, query = query0 + mine;
-      if (STORE) {
-        if (query < a.nq) {
-          ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + half * 4);
-          const uint32_t on = ROWS ? live & s.allow[mine] : live;
-          const float qs = qscale[mine];
+      const uint32_t query = query0 + i * 32 + col;
+      const v16i sum = tile_sums<C>(x, q[i], start);
+      if (query < a.nq) {
+        ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + half * 4);
+        const uint32_t on = there & allow[i];
 #pragma unroll
-          for (int v = 0; v < 16; v += 2) {
-            uint64_t key[2];
+        for (int v = 0; v < 16; v += 2) {
+          uint64_t key[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t r = (v >> 2) * 8 + half * 4 + (v & 3) + e;
-              const float score = exact_score(__int_as_float(sum[v + e]) - kSumZero, qs, s.xs[r], a, s.tb[r], s.ab[r]);
-              key[e] = on >> r & 1u ? offered_key(score, word * 32 + r) : 0;
-            }
-            to[(v >> 2) * 4 + (v & 3) / 2] = make_ulonglong2(key[0], key[1]);
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t r = (v >> 2) * 8 + half * 4 + (v & 3) + e;
+            const float score = exact_score(__int_as_float(sum[v + e]) - kSumZero, qs[i], beside[wave][0][r], a,
+                                            beside[wave][1][r], beside[wave][2][r]);
+            key[e] = on >> r & 1u ? offered_key(score, word * 32 + r) : 0;
           }
-        }
-      } else {
-        int some = -1;  // negative as long as all margins are: a float's sign is its bits' as an integer
-#pragma unroll
-        for (int v = 0; v < 16; ++v) some = max(some, __float_as_int(margin[v]));
-        if (some >= 0) {
-          uint32_t maybe = 0;
-#pragma unroll
-          for (uint32_t v = 0; v < 16; ++v) maybe |= (__float_as_int(margin[v]) >= 0 ? 1u : 0u) << v;
-          maybe &= query < a.nq ? of_lane(ROWS ? live & s.allow[mine] : live) : 0u;
-          while (maybe) {
-            const uint32_t v = __builtin_ctz(maybe), r = (v >> 2) * 8 + half * 4 + (v & 3);
-            maybe &= maybe - 1;
-            int bits = sum[0];
-#pragma unroll
-            for (uint32_t e = 1; e < 16; ++e) bits = v == e ? sum[e] : bits;
-            const float score = exact_score(__int_as_float(bits) - kSumZero, qscale[mine], s.xs[r], a, s.tb[r], s.ab[r]);
-            const uint64_t key = offered_key(score, word * 32 + r);
-            if (key && score >= lowest[mine]) {  // from a little below the threshold on: the selection sees to the rest
-              const uint32_t to = atomicAdd(&listed, 1u);
-              if (to < kListed) {
-                list_key[to] = key;
-                list_place[to] = mine;
-              } else {
-                append(a, query, key);
-              }
-            }
-          }
+          to[(v >> 2) * 4 + (v & 3) / 2] = make_ulonglong2(key[0], key[1]);
         }
       }
     }
     wave_sync();
   }
-  if (STORE) return;
-  __syncthreads();
-  const uint32_t t = threadIdx.x, m = listed < kListed ? listed : kListed;
-  for (uint32_t i = t; i < m; i += 256) list_place[i] |= atomicAdd(&found[list_place[i]], 1u) << 8;
-  __syncthreads();
-  if (t < kQueries && found[t]) base[t] = atomicAdd(&a.count[(query0 + t) * kCountStride], found[t]);
-  __syncthreads();
-  for (uint32_t i = t; i < m; i += 256) {
-    const uint32_t mine = list_place[i] & 255u;
-    const uint64_t to = static_cast<uint64_t>(base[mine]) + (list_place[i] >> 8);
-    if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = list_key[i];
-  }
 }
 
+// The other passes: which records may reach the threshold.  A wave lists them in LDS, without their scores (the selection
+// computes those: here it would keep the matrix unit waiting), and hands the list on when it runs full, with one addition
+// to each query's count: additions to one address from all over the GPU are served one after another.
+template <int KC, int QT, bool ROWS>
+__global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
+  constexpr uint32_t kQueries = QT * 32, kList = 512, kFull = kList - QT * 64;  // a block adds at most 64 entries a tile
+  constexpr int C = KC * 2;
+  struct Own {  // each wave's
+    uint64_t list[kList];  // first record | bits << 32 | query << 48
+    uint32_t found[kQueries], base[kQueries];
+    uint32_t allow[ROWS ? kQueries : 1];
+  };
+  __shared__ Own owns[4];
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 31, half = lane >> 5;
+  Own& own = owns[wave];
+  const Place at = place_of(query_blocks);
+  const uint32_t query0 = at.query_block * kQueries;
+  const uint64_t b0 = at.range * per_range, b1 = b0 + per_range < a.blocks ? b0 + per_range : a.blocks, last = b1 - 1;
+  if (b0 + wave >= b1) return;
+  v4i q[QT][C];
+  load_tile_queries<C, QT>(q, a, query0);
+  v4s qterms[QT];
+  int limit[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const uint32_t query = query0 + i * 32 + col, r = min(query, a.nq - 1);
+    qterms[i] = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.query_terms)[r].t[half * 4]);
+    limit[i] = query < a.nq ? a.limit[r] : 0x7FFFFFFF;
+  }
+  for (uint32_t i = lane; i < kQueries; i += 64) own.found[i] = 0;
+  constexpr int MASKS = (kQueries + 63) / 64;  // queries whose mask words a lane fetches
+  const uint32_t* allow_row[MASKS];
+#pragma unroll
+  for (int i = 0; i < MASKS; ++i) allow_row[i] = a.allow + (ROWS ? min(query0 + i * 64 + lane, a.nq - 1) * a.allow_ld : 0);
+  v4i next[C];
+  v4s next_terms;
+  uint32_t next_allow[MASKS];
+  auto fetch = [&](uint64_t b) {
+    const uint64_t word = min(b, last) * a.stride;
+    load_tile_block<C>(next, a, word);
+    next_terms = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.record_terms)[word * 32 + col].t[half * 4]);
+    if (ROWS)
+#pragma unroll
+      for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][word];
+  };
+  uint32_t listed = 0;
+  auto hand_on = [&] {
+    wave_sync();
+    uint32_t place[kList / 64];
+#pragma unroll
+    for (uint32_t i = 0; i < kList / 64; ++i)
+      if (i * 64 + lane < listed) place[i] = atomicAdd(&own.found[own.list[i * 64 + lane] >> 48], 1u);
+    wave_sync();
+    for (uint32_t i = lane; i < kQueries; i += 64) {
+      if (own.found[i]) own.base[i] = atomicAdd(&a.count[(query0 + i) * kCountStride], own.found[i]);
+      own.found[i] = 0;
+    }
+    wave_sync();
+#pragma unroll
+    for (uint32_t i = 0; i < kList / 64; ++i)
+      if (i * 64 + lane < listed) {
+        const uint64_t entry = own.list[i * 64 + lane];
+        const uint32_t mine = static_cast<uint32_t>(entry >> 48);
+        const uint64_t to = static_cast<uint64_t>(own.base[mine]) + place[i];
+        if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = entry & 0xFFFFFFFFFFFFull;
+      }
+    wave_sync();
+    listed = 0;
+  };
+  const v16i start = sums_start();
+  fetch(b0 + wave);
+  for (uint64_t b = b0 + wave; b < b1; b += 4) {
+    v4i x[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = next[c];
+    const v4s terms = next_terms;
+    const uint64_t word = b * a.stride;
+    if (ROWS) {
+      wave_sync();
+#pragma unroll
+      for (int i = 0; i < MASKS; ++i)
+        if (i * 64 + lane < kQueries) own.allow[i * 64 + lane] = next_allow[i];
+      wave_sync();
+    }
+    fetch(b + 4);
+    v16i ahead = tile_sums<C>(x, q[0], start);  // the matrix unit works on the next tile while this one is looked at
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      const v16f margin = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(terms, qterms[i], __builtin_bit_cast(v16f, ahead), 0, 0, 0);
+      if (i + 1 < QT) ahead = tile_sums<C>(x, q[i + 1 < QT ? i + 1 : 0], start);
+      int most = -0x7FFFFFFF - 1;  // as integers, floats' bits keep their order but for the negative ones among themselves
+#pragma unroll
+      for (int v = 0; v < 16; ++v) most = max(most, __float_as_int(margin[v]));
+      if (__any(most >= limit[i])) {
+        uint32_t maybe = 0;
+#pragma unroll
+        for (uint32_t v = 0; v < 16; ++v) maybe |= (__float_as_int(margin[v]) >= limit[i] ? 1u : 0u) << v;
+        if (ROWS) {
+          const uint32_t w = own.allow[i * 32 + col] >> (half * 4);
+          maybe &= (w & 15u) | (w >> 4 & 0xF0u) | (w >> 8 & 0xF00u) | (w >> 12 & 0xF000u);
+        }
+        const uint64_t who = __ballot(maybe != 0);
+        if (maybe)
+          own.list[listed + __popcll(who & ((1ull << lane) - 1))] =
+              (word * 32 + half * 4) | static_cast<uint64_t>(maybe) << 32 | static_cast<uint64_t>(i * 32 + col) << 48;
+        listed += __popcll(who);
+      }
+    }
+    if (listed > kFull) hand_on();
+  }
+  if (listed) hand_on();
+}
+
+// Rows of whole 64-byte steps; a step's four loads are asked for together.
 __device__ inline int dot_codes(const int8_t* x, const v4i* q, uint32_t pitch) {
   int sum = 0;
-  for (uint32_t c = 0; c < pitch / 16; ++c) {
-    const v4i v = reinterpret_cast<const v4i*>(x)[c], w = q[c];
-    for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_sdot4(v[j], w[j], sum, false);
+  for (uint32_t c = 0; c < pitch / 64; ++c) {
+    v4i v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = reinterpret_cast<const v4i*>(x)[c * 4 + e];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_sdot4(v[e][j], q[c * 4 + e][j], sum, false);
   }
   return sum;
 }
 
 __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
+  constexpr uint32_t kEntries = 256;
   __shared__ Held h;
   __shared__ v4i query[kMaxFusedPitch / 16];
+  __shared__ uint32_t records[kEntries * 16], n_records;
   const PassArgs& p = a.pass;
   const uint32_t row = blockIdx.x;
+  if (threadIdx.x < p.pitch / 16)
+    query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
   begin(h);
-  const uint64_t listed = a.fixed ? a.fixed : p.count[row * kCountStride];
-  const uint64_t held = listed < p.cap ? listed : p.cap;
-  offer_list(h, a.k, p.keys + row * p.cap, held);
+  const float qs = p.qscales[row];
+  auto key_at = [&](uint64_t r) -> uint64_t {  // a query without a threshold lists what is behind the end or masked, too
+    if (r >= p.n || (p.allow && !(p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u))) return 0;
+    return offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
+  };
+  const uint64_t listed = a.fixed ? a.fixed : p.count[row * kCountStride], held = listed < p.cap ? listed : p.cap;
+  const uint64_t* list = p.keys + row * p.cap;
+  if (a.fixed) {
+    offer_list(h, a.k, list, held);
+  } else {
+    for (uint64_t c = 0; c < held; c += kEntries) {
+      if (threadIdx.x == 0) n_records = 0;
+      __syncthreads();
+      if (c + threadIdx.x < held) {
+        const uint64_t entry = list[c + threadIdx.x];
+        const uint32_t first = static_cast<uint32_t>(entry);
+        uint32_t bits = static_cast<uint32_t>(entry >> 32);
+        uint32_t to = atomicAdd(&n_records, __popc(bits));
+        while (bits) {
+          const uint32_t v = __builtin_ctz(bits);
+          bits &= bits - 1;
+          records[to++] = first + (v >> 2) * 8 + (v & 3);
+        }
+      }
+      __syncthreads();
+      const uint32_t m = n_records;
+      for (uint32_t i = 0; i < m; i += 512) {
+        uint64_t key[2];
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) key[e] = i + e * 256 + threadIdx.x < m ? key_at(records[i + e * 256 + threadIdx.x]) : 0;
+        offer(h, a.k, key, c == 0 && i == 0);
+      }
+    }
+  }
   if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
   finish(h, a.k);  // every thread has read the row's count: there is a barrier in between
-  if (a.thr) {
+  if (!a.last) {
     if (threadIdx.x == 0) {
       // a finer pass need not meet the coarser one's records again: where it finds fewer than k, that one's bound stays
-      if (h.count == a.k) a.thr[row] = h.key[a.k - 1];
-      else if (a.fixed) a.thr[row] = 0;
+      if (h.count == a.k || a.fixed) {
+        const uint64_t key = h.count == a.k ? h.key[a.k - 1] : 0;
+        const float thr = key ? fminf(key_value(key), 3.4028e38f) : -__builtin_huge_valf();  // an infinite one as the largest
+        const float low = thr - 0x1p-20f * fabsf(thr);
+        static_cast<Terms*>(p.query_terms)[row] = query_terms(qs, low);
+        p.limit[row] = query_limit(qs, low, true);
+      }
       p.count[row * kCountStride] = 0;
     }
     return;
   }
   if (listed > p.cap) {
-    // Keys were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
+    // Entries were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
     // they go; the history's records, which no mask lets through, are offered again.
-    if (threadIdx.x < p.pitch / 16)
-      query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
     const uint64_t floor = h.count == a.k ? h.key[a.k - 1] - 1 : 0;  // the k-th best itself is an answer
     __syncthreads();
     begin(h, floor);
-    const float qs = p.qscales[row];
     for (uint64_t r0 = 0; r0 < p.n; r0 += 256) {
       const uint64_t r = r0 + threadIdx.x;
-      uint64_t key[1] = {0};
-      if (r < p.n && (!p.allow || (p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u)))
-        key[0] = offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
+      const uint64_t key[1] = {key_at(r)};
       offer(h, a.k, key, false);
     }
     if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
@@ -1358,31 +1412,52 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+hipError_t launch_terms(const PassArgs& a, hipStream_t s) {
+  const uint64_t records = (a.n + 31) / 32 * 32;
+  hipLaunchKernelGGL(terms_kernel, dim3(static_cast<uint32_t>((records + 255) / 256)), dim3(256), 0, s, a,
+                     static_cast<Terms*>(const_cast<void*>(a.record_terms)));
+  return hipGetLastError();
+}
+
+namespace {
 constexpr uint32_t kPassGroups = 512;  // two workgroups a CU
-hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
-  const bool rows = a.allow && a.allow_ld;
-#define SHINE_FOR(KK, QQ, RR, SS)                                                                          \
-  if (rows == RR && a.store == SS)                                                                         \
-    hipLaunchKernelGGL((pass_kernel<KK, QQ, RR, SS>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
-#define SHINE_PASS(KK, QQ)                                                                                 \
-  {                                                                                                        \
-    const uint32_t qb = (a.nq + QQ * 32 - 1) / (QQ * 32);                                                  \
-    const Ranges r = ranges_of(a.blocks, qb, kPassGroups);                                                 \
-    SHINE_FOR(KK, QQ, true, true) SHINE_FOR(KK, QQ, true, false)                                           \
-    SHINE_FOR(KK, QQ, false, true) SHINE_FOR(KK, QQ, false, false)                                         \
-  }
-#define SHINE_KC(KK, BIG) \
-  if (a.nq <= 32) SHINE_PASS(KK, 1) else SHINE_PASS(KK, BIG)
+
+template <int KC, int QT>
+void sample_with(const PassArgs& a, hipStream_t s) {
+  const uint32_t qb = (a.nq + QT * 32 - 1) / (QT * 32);
+  const Ranges r = ranges_of(a.blocks, qb, kPassGroups);
+  hipLaunchKernelGGL((sample_kernel<KC, QT>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+}
+template <int KC, int QT>
+void pass_with(const PassArgs& a, hipStream_t s) {
+  const uint32_t qb = (a.nq + QT * 32 - 1) / (QT * 32);
+  const Ranges r = ranges_of(a.blocks, qb, kPassGroups);
+  if (a.allow && a.allow_ld) hipLaunchKernelGGL((pass_kernel<KC, QT, true>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+  else hipLaunchKernelGGL((pass_kernel<KC, QT, false>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+}
+}  // namespace
+
+hipError_t launch_sample(const PassArgs& a, hipStream_t s) {
+  const bool few = a.nq <= 32;
   switch (a.pitch / 64) {
-    case 1: SHINE_KC(1, 4); break;
-    case 2: SHINE_KC(2, 4); break;
-    case 3: SHINE_KC(3, 2); break;
-    case 4: SHINE_KC(4, 2); break;
+    case 1: few ? sample_with<1, 1>(a, s) : sample_with<1, 4>(a, s); break;
+    case 2: few ? sample_with<2, 1>(a, s) : sample_with<2, 4>(a, s); break;
+    case 3: few ? sample_with<3, 1>(a, s) : sample_with<3, 2>(a, s); break;
+    case 4: few ? sample_with<4, 1>(a, s) : sample_with<4, 2>(a, s); break;
     default: return hipErrorInvalidValue;
   }
-#undef SHINE_KC
-#undef SHINE_PASS
-#undef SHINE_FOR
+  return hipGetLastError();
+}
+
+hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
+  const bool few = a.nq <= 32;
+  switch (a.pitch / 64) {
+    case 1: few ? pass_with<1, 1>(a, s) : pass_with<1, 4>(a, s); break;
+    case 2: few ? pass_with<2, 1>(a, s) : pass_with<2, 4>(a, s); break;
+    case 3: few ? pass_with<3, 1>(a, s) : pass_with<3, 2>(a, s); break;
+    case 4: few ? pass_with<4, 1>(a, s) : pass_with<4, 2>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 
