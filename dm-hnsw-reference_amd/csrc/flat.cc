@@ -241,7 +241,7 @@ hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const sh
     if (hipError_t e = i ? F::launch_pass(pass, s) : F::launch_sample(pass, s); e != hipSuccess) return e;
     sel.pass = pass;
     sel.k = k;
-    sel.fixed = i == 0 ? pass.blocks * 32 : 0;
+    sel.sample = i == 0;
     sel.extra = last ? extra : nullptr;
     sel.last = last;
     sel.values = values;

@@ -58,19 +58,18 @@ struct PassArgs {
   // the coarsest pass: every key at keys[q * cap + 32 * block + i]
   uint64_t* keys;
   uint64_t cap;
-  // the others: what may reach the threshold is listed at keys[q * cap + 0 .. count - 1] as a record (low word: the first one)
-  // and 16 bits, v for record 8 (v / 4) + v % 4 behind it
+  // the others: the keys of what reaches the threshold, or lies a little below it, at keys[q * cap + 0 .. count - 1]
   const void* record_terms;  // of all records, whole blocks
   void* query_terms;
   int32_t* limit;            // per query
-  uint32_t* count;           // query q's at q * kCountStride (may pass cap; the list then holds cap entries)
+  uint32_t* count;           // query q's at q * kCountStride (may pass cap; the list then holds cap keys)
 };
 
 // Selection from a search's lists: the k-th best key between passes, the answers behind the last one.
 struct SelectArgs {
   PassArgs pass;          // what a row's scores are computed with
   uint32_t k;
-  uint64_t fixed;         // keys of every list, or 0: count[q] entries
+  bool sample;            // every list holds `blocks` x 32 keys; else count[q]
   const uint64_t* extra;  // nullable: extra_count[q] more keys at extra + q * extra_ld
   const uint32_t* extra_count;
   uint64_t extra_ld;

@@ -854,13 +854,20 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
 // All threads call it behind a barrier.
 __device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* src, uint64_t count) {
   constexpr int N = 8;
-  for (uint64_t c = 0; c < count; c += 256 * N) {
-    uint64_t key[N];
+  uint64_t next[N];
+  auto fetch = [&](uint64_t c) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint64_t at = c + i * 256 + threadIdx.x;
-      key[i] = at < count ? src[at] : 0;
+      next[i] = at < count ? src[at] : 0;
     }
+  };
+  if (count) fetch(0);
+  for (uint64_t c = 0; c < count; c += 256 * N) {
+    uint64_t key[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] = next[i];
+    if (c + 256 * N < count) fetch(c + 256 * N);
     offer(h, k, key, c == 0);
   }
 }
@@ -1059,15 +1066,17 @@ __global__ __launch_bounds__(256, 2) void sample_kernel(PassArgs a, uint32_t que
   }
 }
 
-// The other passes: which records may reach the threshold.  A wave lists them in LDS, without their scores (the selection
-// computes those: here it would keep the matrix unit waiting), and hands the list on when it runs full, with one addition
-// to each query's count: additions to one address from all over the GPU are served one after another.
+// The other passes: the keys of what reaches the threshold.  A wave lists them in LDS and hands its list on when it runs full,
+// with one addition to each query's count: additions to one address from all over the GPU are served one after another.
+// What a score needs beside its sum is in registers, a record's in lane r % 32: a load from memory would wait for the next
+// block's codes, which are on their way.
 template <int KC, int QT, bool ROWS>
 __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
-  constexpr uint32_t kQueries = QT * 32, kList = 512, kFull = kList - QT * 64;  // a block adds at most 64 entries a tile
+  constexpr uint32_t kQueries = QT * 32, kList = 512, kFull = kList - 64;  // a turn of the listing adds at most 64 keys
   constexpr int C = KC * 2;
   struct Own {  // each wave's
-    uint64_t list[kList];  // first record | bits << 32 | query << 48
+    uint64_t key[kList];
+    uint32_t query[kList];
     uint32_t found[kQueries], base[kQueries];
     uint32_t allow[ROWS ? kQueries : 1];
   };
@@ -1082,27 +1091,37 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   load_tile_queries<C, QT>(q, a, query0);
   v4s qterms[QT];
   int limit[QT];
+  float qs[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t query = query0 + i * 32 + col, r = min(query, a.nq - 1);
     qterms[i] = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.query_terms)[r].t[half * 4]);
     limit[i] = query < a.nq ? a.limit[r] : 0x7FFFFFFF;
+    qs[i] = a.qscales[r];
   }
   for (uint32_t i = lane; i < kQueries; i += 64) own.found[i] = 0;
   constexpr int MASKS = (kQueries + 63) / 64;  // queries whose mask words a lane fetches
   const uint32_t* allow_row[MASKS];
 #pragma unroll
   for (int i = 0; i < MASKS; ++i) allow_row[i] = a.allow + (ROWS ? min(query0 + i * 64 + lane, a.nq - 1) * a.allow_ld : 0);
+  const float* tbias = a.tbias ? a.tbias : a.scales;
+  const float* abias = a.abias ? a.abias : a.scales;
+  const uint32_t* shared_allow = a.allow ? a.allow : reinterpret_cast<const uint32_t*>(a.scales);
+  const bool shared = !ROWS && a.allow;
   v4i next[C];
   v4s next_terms;
+  float next_xs, next_tb, next_ab;
   uint32_t next_allow[MASKS];
   auto fetch = [&](uint64_t b) {
     const uint64_t word = min(b, last) * a.stride;
     load_tile_block<C>(next, a, word);
     next_terms = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.record_terms)[word * 32 + col].t[half * 4]);
-    if (ROWS)
+    const uint32_t mine = min(col, records_of(a, word) - 1);
+    next_xs = (a.scales + word * 32)[mine];
+    next_tb = (tbias + word * 32)[mine];
+    next_ab = (abias + word * 32)[mine];
 #pragma unroll
-      for (int i = 0; i < MASKS; ++i) next_allow[i] = allow_row[i][word];
+    for (int i = 0; i < MASKS; ++i) next_allow[i] = ROWS ? allow_row[i][word] : i ? 0 : shared_allow[shared ? word : 0];
   };
   uint32_t listed = 0;
   auto hand_on = [&] {
@@ -1110,7 +1129,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
     uint32_t place[kList / 64];
 #pragma unroll
     for (uint32_t i = 0; i < kList / 64; ++i)
-      if (i * 64 + lane < listed) place[i] = atomicAdd(&own.found[own.list[i * 64 + lane] >> 48], 1u);
+      if (i * 64 + lane < listed) place[i] = atomicAdd(&own.found[own.query[i * 64 + lane]], 1u);
     wave_sync();
     for (uint32_t i = lane; i < kQueries; i += 64) {
       if (own.found[i]) own.base[i] = atomicAdd(&a.count[(query0 + i) * kCountStride], own.found[i]);
@@ -1120,10 +1139,9 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
 #pragma unroll
     for (uint32_t i = 0; i < kList / 64; ++i)
       if (i * 64 + lane < listed) {
-        const uint64_t entry = own.list[i * 64 + lane];
-        const uint32_t mine = static_cast<uint32_t>(entry >> 48);
+        const uint32_t mine = own.query[i * 64 + lane];
         const uint64_t to = static_cast<uint64_t>(own.base[mine]) + place[i];
-        if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = entry & 0xFFFFFFFFFFFFull;
+        if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = own.key[i * 64 + lane];
       }
     wave_sync();
     listed = 0;
@@ -1136,6 +1154,9 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
     for (int c = 0; c < C; ++c) x[c] = next[c];
     const v4s terms = next_terms;
     const uint64_t word = b * a.stride;
+    const uint32_t there = records_of(a, word);
+    const uint32_t live = (there == 32 ? ~0u : (1u << there) - 1) & (shared ? next_allow[0] : ~0u);
+    const int xs = __float_as_int(next_xs), tb = __float_as_int(next_tb), ab = __float_as_int(next_ab);
     if (ROWS) {
       wave_sync();
 #pragma unroll
@@ -1147,27 +1168,40 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
     v16i ahead = tile_sums<C>(x, q[0], start);  // the matrix unit works on the next tile while this one is looked at
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      const v16f margin = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(terms, qterms[i], __builtin_bit_cast(v16f, ahead), 0, 0, 0);
+      const v16i sum = ahead;
+      const v16f margin = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(terms, qterms[i], __builtin_bit_cast(v16f, sum), 0, 0, 0);
       if (i + 1 < QT) ahead = tile_sums<C>(x, q[i + 1 < QT ? i + 1 : 0], start);
       int most = -0x7FFFFFFF - 1;  // as integers, floats' bits keep their order but for the negative ones among themselves
 #pragma unroll
       for (int v = 0; v < 16; ++v) most = max(most, __float_as_int(margin[v]));
-      if (__any(most >= limit[i])) {
+      if (__any(most >= limit[i])) {  // all lanes: they hold the records' scales for one another
         uint32_t maybe = 0;
 #pragma unroll
         for (uint32_t v = 0; v < 16; ++v) maybe |= (__float_as_int(margin[v]) >= limit[i] ? 1u : 0u) << v;
-        if (ROWS) {
-          const uint32_t w = own.allow[i * 32 + col] >> (half * 4);
-          maybe &= (w & 15u) | (w >> 4 & 0xF0u) | (w >> 8 & 0xF00u) | (w >> 12 & 0xF000u);
+        const uint32_t on = (ROWS ? live & own.allow[i * 32 + col] : live) >> (half * 4);
+        maybe &= (on & 15u) | (on >> 4 & 0xF0u) | (on >> 8 & 0xF00u) | (on >> 12 & 0xF000u);
+        while (__any(maybe != 0)) {
+          const uint32_t v = maybe ? __builtin_ctz(maybe) : 0, r = (v >> 2) * 8 + half * 4 + (v & 3);
+          int bits = sum[0];
+#pragma unroll
+          for (uint32_t e = 1; e < 16; ++e) bits = v == e ? sum[e] : bits;
+          const float score = exact_score(__int_as_float(bits) - kSumZero, qs[i],
+                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, xs)), a,
+                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, tb)),
+                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, ab)));
+          const uint64_t key = maybe ? offered_key(score, word * 32 + r) : 0;
+          maybe &= maybe - 1;
+          const uint64_t who = __ballot(key != 0);
+          if (key) {
+            const uint32_t to = listed + __popcll(who & ((1ull << lane) - 1));
+            own.key[to] = key;
+            own.query[to] = i * 32 + col;
+          }
+          listed += __popcll(who);
+          if (listed > kFull) hand_on();
         }
-        const uint64_t who = __ballot(maybe != 0);
-        if (maybe)
-          own.list[listed + __popcll(who & ((1ull << lane) - 1))] =
-              (word * 32 + half * 4) | static_cast<uint64_t>(maybe) << 32 | static_cast<uint64_t>(i * 32 + col) << 48;
-        listed += __popcll(who);
       }
     }
-    if (listed > kFull) hand_on();
   }
   if (listed) hand_on();
 }
@@ -1187,56 +1221,30 @@ __device__ inline int dot_codes(const int8_t* x, const v4i* q, uint32_t pitch) {
   return sum;
 }
 
-__global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
-  constexpr uint32_t kEntries = 256;
-  __shared__ Held h;
-  __shared__ v4i query[kMaxFusedPitch / 16];
-  __shared__ uint32_t records[kEntries * 16], n_records;
-  const PassArgs& p = a.pass;
-  const uint32_t row = blockIdx.x;
+__device__ inline uint64_t key_at(const PassArgs& p, uint32_t row, const v4i* query, float qs, uint64_t r) {
+  if (r >= p.n || (p.allow && !(p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u))) return 0;
+  return offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
+}
+__device__ inline void load_query(v4i* query, const PassArgs& p, uint32_t row) {
   if (threadIdx.x < p.pitch / 16)
     query[threadIdx.x] = reinterpret_cast<const v4i*>(p.qcodes + static_cast<uint64_t>(row) * p.pitch)[threadIdx.x];
+}
+
+__global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
+  __shared__ Held h;
+  __shared__ v4i query[kMaxFusedPitch / 16];
+  const PassArgs& p = a.pass;
+  const uint32_t row = blockIdx.x;
   begin(h);
   const float qs = p.qscales[row];
-  auto key_at = [&](uint64_t r) -> uint64_t {  // a query without a threshold lists what is behind the end or masked, too
-    if (r >= p.n || (p.allow && !(p.allow[row * p.allow_ld + (r >> 5)] >> (r & 31) & 1u))) return 0;
-    return offered_key(exact_score(static_cast<float>(dot_codes(p.codes + r * p.pitch, query, p.pitch)), qs, p, r), r);
-  };
-  const uint64_t listed = a.fixed ? a.fixed : p.count[row * kCountStride], held = listed < p.cap ? listed : p.cap;
-  const uint64_t* list = p.keys + row * p.cap;
-  if (a.fixed) {
-    offer_list(h, a.k, list, held);
-  } else {
-    for (uint64_t c = 0; c < held; c += kEntries) {
-      if (threadIdx.x == 0) n_records = 0;
-      __syncthreads();
-      if (c + threadIdx.x < held) {
-        const uint64_t entry = list[c + threadIdx.x];
-        const uint32_t first = static_cast<uint32_t>(entry);
-        uint32_t bits = static_cast<uint32_t>(entry >> 32);
-        uint32_t to = atomicAdd(&n_records, __popc(bits));
-        while (bits) {
-          const uint32_t v = __builtin_ctz(bits);
-          bits &= bits - 1;
-          records[to++] = first + (v >> 2) * 8 + (v & 3);
-        }
-      }
-      __syncthreads();
-      const uint32_t m = n_records;
-      for (uint32_t i = 0; i < m; i += 512) {
-        uint64_t key[2];
-#pragma unroll
-        for (uint32_t e = 0; e < 2; ++e) key[e] = i + e * 256 + threadIdx.x < m ? key_at(records[i + e * 256 + threadIdx.x]) : 0;
-        offer(h, a.k, key, c == 0 && i == 0);
-      }
-    }
-  }
+  const uint64_t listed = a.sample ? p.blocks * 32 : p.count[row * kCountStride];
+  offer_list(h, a.k, p.keys + row * p.cap, listed < p.cap ? listed : p.cap);
   if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
   finish(h, a.k);  // every thread has read the row's count: there is a barrier in between
   if (!a.last) {
     if (threadIdx.x == 0) {
       // a finer pass need not meet the coarser one's records again: where it finds fewer than k, that one's bound stays
-      if (h.count == a.k || a.fixed) {
+      if (h.count == a.k || a.sample) {
         const uint64_t key = h.count == a.k ? h.key[a.k - 1] : 0;
         const float thr = key ? fminf(key_value(key), 3.4028e38f) : -__builtin_huge_valf();  // an infinite one as the largest
         const float low = thr - 0x1p-20f * fabsf(thr);
@@ -1248,14 +1256,14 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
     return;
   }
   if (listed > p.cap) {
-    // Entries were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
+    // Keys were lost: all records again, against the floor that the kept ones gave.  The kept ones are met again, so
     // they go; the history's records, which no mask lets through, are offered again.
+    load_query(query, p, row);
     const uint64_t floor = h.count == a.k ? h.key[a.k - 1] - 1 : 0;  // the k-th best itself is an answer
     __syncthreads();
     begin(h, floor);
     for (uint64_t r0 = 0; r0 < p.n; r0 += 256) {
-      const uint64_t r = r0 + threadIdx.x;
-      const uint64_t key[1] = {key_at(r)};
+      const uint64_t key[1] = {key_at(p, row, query, qs, r0 + threadIdx.x)};
       offer(h, a.k, key, false);
     }
     if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
