@@ -231,8 +231,6 @@ hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const sh
       sel.extra_ld = seen.extra_ld;
     }
   }
-  if (p.passes > 1 && q == 0)  // the records' terms are the same for all blocks of rows
-    if (hipError_t e = F::launch_terms(pass, s); e != hipSuccess) return e;
   const uint64_t* extra = sel.extra;
   for (uint32_t i = 0; i < p.passes; ++i) {
     const bool last = i + 1 == p.passes;
@@ -242,6 +240,7 @@ hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const sh
     sel.pass = pass;
     sel.k = k;
     sel.sample = i == 0;
+    sel.terms = i == 0 && !last && q == 0;  // the same for all blocks of rows
     sel.extra = last ? extra : nullptr;
     sel.last = last;
     sel.values = values;

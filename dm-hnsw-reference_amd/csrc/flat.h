@@ -59,7 +59,7 @@ struct PassArgs {
   uint64_t* keys;
   uint64_t cap;
   // the others: the keys of what reaches the threshold, or lies a little below it, at keys[q * cap + 0 .. count - 1]
-  const void* record_terms;  // of all records, whole blocks
+  void* record_terms;        // of all records, whole blocks
   void* query_terms;
   int32_t* limit;            // per query
   uint32_t* count;           // query q's at q * kCountStride (may pass cap; the list then holds cap keys)
@@ -73,6 +73,7 @@ struct SelectArgs {
   const uint64_t* extra;  // nullable: extra_count[q] more keys at extra + q * extra_ld
   const uint32_t* extra_count;
   uint64_t extra_ld;
+  bool terms;             // write pass.record_terms beside it, as a shared allow, scales and biases have them
   bool last;              // write the answers; else thr, limit and query_terms, and clear count
   float* values;
   int32_t* ids;
@@ -137,7 +138,6 @@ uint32_t topk_slices(uint32_t nq, uint64_t n);
 
 hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s);
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s);
-hipError_t launch_terms(const PassArgs& a, hipStream_t s);  // record_terms, as allow (shared), scales and biases have them
 hipError_t launch_sample(const PassArgs& a, hipStream_t s);
 hipError_t launch_pass(const PassArgs& a, hipStream_t s);
 hipError_t launch_select(const SelectArgs& a, hipStream_t s);

@@ -618,7 +618,7 @@ __device__ inline int32_t key_id(uint64_t key) {
 // 4,096 random keys about k (1 + k / 512) pass it.
 constexpr uint32_t kKeys = 1024;
 
-struct Held {
+struct __attribute__((aligned(16))) Held {
   uint64_t key[kKeys];
   uint32_t top[256];
   uint32_t count;
@@ -708,9 +708,14 @@ __device__ inline void finish(Held& h, uint32_t k) {
   const uint32_t held = h.count;
   if (held <= 256) {  // each key's place is the number of larger ones
     const uint64_t mine = threadIdx.x < held ? h.key[threadIdx.x] : 0;
+    if (threadIdx.x == 0 && held < kKeys) h.key[held] = 0;  // keys are read in twos
+    __syncthreads();
     uint32_t place = 0;
 #pragma unroll 4
-    for (uint32_t i = 0; i < held; ++i) place += h.key[i] > mine;
+    for (uint32_t i = 0; i < held; i += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&h.key[i]);
+      place += (two.x > mine) + (two.y > mine);
+    }
     __syncthreads();
     if (threadIdx.x < held) h.key[place] = mine;
   } else {
@@ -960,12 +965,13 @@ __device__ inline int query_limit(float q, float low, bool there) {
   return !there || q != q ? 0x7FFFFFFF : query_plain(q, low) ? kMagic : -0x7FFFFFFF - 1;
 }
 
-__global__ __launch_bounds__(256) void terms_kernel(PassArgs a, Terms* out) {
-  const uint64_t r = blockIdx.x * 256ull + threadIdx.x;
+__device__ inline void write_record_terms(const PassArgs& a, uint64_t block) {  // of 256 records
+  const uint64_t r = block * 256 + threadIdx.x;
   if (r >= (a.n + 31) / 32 * 32) return;
   const uint64_t at = min(r, a.n - 1);
   const bool on = r < a.n && (!a.allow || a.allow_ld || (a.allow[r >> 5] >> (r & 31) & 1u));
-  out[r] = record_terms(a.scales[at], (a.tbias ? a.tbias[at] : 0.0f) + (a.abias ? a.abias[at] : 0.0f), on);
+  static_cast<Terms*>(a.record_terms)[r] =
+      record_terms(a.scales[at], (a.tbias ? a.tbias[at] : 0.0f) + (a.abias ? a.abias[at] : 0.0f), on);
 }
 
 // Both passes: a wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32
@@ -1235,6 +1241,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
   __shared__ v4i query[kMaxFusedPitch / 16];
   const PassArgs& p = a.pass;
   const uint32_t row = blockIdx.x;
+  if (row >= p.nq) return write_record_terms(p, row - p.nq);
   begin(h);
   const float qs = p.qscales[row];
   const uint64_t listed = a.sample ? p.blocks * 32 : p.count[row * kCountStride];
@@ -1274,10 +1281,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
 
 // The row's mask without its history: one workgroup per (row, kMaskWords words).
 constexpr uint32_t kMaskWords = 4096;
-__global__ __launch_bounds__(256) void seen_mask_kernel(SeenArgs a) {
-  __shared__ uint32_t mask[kMaskWords];
-  const uint32_t row = blockIdx.y;
-  const uint64_t w0 = static_cast<uint64_t>(blockIdx.x) * kMaskWords;
+__device__ inline void seen_mask(const SeenArgs& a, uint32_t row, uint64_t w0, uint32_t* mask) {
   const uint32_t width = static_cast<uint32_t>(a.mask_ld - w0 < kMaskWords ? a.mask_ld - w0 : kMaskWords);
   for (uint32_t i = threadIdx.x; i < width; i += 256)
     mask[i] = a.pass.allow ? a.pass.allow[row * a.pass.allow_ld + w0 + i] : 0xFFFFFFFFu;
@@ -1292,12 +1296,8 @@ __global__ __launch_bounds__(256) void seen_mask_kernel(SeenArgs a) {
 }
 
 // The history's records, each once: the ids sorted in LDS, a run's length its count.
-__global__ __launch_bounds__(256) void seen_keys_kernel(SeenArgs a) {
-  __shared__ uint32_t ids[kMaxSeen];
-  __shared__ v4i query[kMaxFusedPitch / 16];
-  __shared__ uint32_t count;
+__device__ inline void seen_keys(const SeenArgs& a, uint32_t row, uint32_t* ids, v4i* query, uint32_t& count) {
   const PassArgs& p = a.pass;
-  const uint32_t row = blockIdx.x;
   uint32_t n = 2;
   while (n < a.seen_n) n <<= 1;
   for (uint32_t i = threadIdx.x; i < n; i += 256) {
@@ -1343,6 +1343,16 @@ __global__ __launch_bounds__(256) void seen_keys_kernel(SeenArgs a) {
   }
   __syncthreads();
   if (threadIdx.x == 0) a.extra_count[row] = count;
+}
+
+// A row's keys (the first workgroup) and the tiles of its mask.
+__global__ __launch_bounds__(256) void seen_kernel(SeenArgs a) {
+  static_assert(kMaskWords == kMaxSeen, "one array serves both");
+  __shared__ uint32_t words[kMaxSeen];
+  __shared__ v4i query[kMaxFusedPitch / 16];
+  __shared__ uint32_t count;
+  if (blockIdx.x == 0) seen_keys(a, blockIdx.y, words, query, count);
+  else seen_mask(a, blockIdx.y, (blockIdx.x - 1ull) * kMaskWords, words);
 }
 
 }  // namespace
@@ -1420,13 +1430,6 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_terms(const PassArgs& a, hipStream_t s) {
-  const uint64_t records = (a.n + 31) / 32 * 32;
-  hipLaunchKernelGGL(terms_kernel, dim3(static_cast<uint32_t>((records + 255) / 256)), dim3(256), 0, s, a,
-                     static_cast<Terms*>(const_cast<void*>(a.record_terms)));
-  return hipGetLastError();
-}
-
 namespace {
 constexpr uint32_t kPassGroups = 512;  // two workgroups a CU
 
@@ -1470,14 +1473,14 @@ hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(select_kernel, dim3(a.pass.nq), dim3(256), 0, s, a);
+  const uint64_t terms = a.terms ? (a.pass.n + 255) / 256 : 0;
+  hipLaunchKernelGGL(select_kernel, dim3(static_cast<uint32_t>(a.pass.nq + terms)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
 hipError_t launch_seen(const SeenArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>((a.mask_ld + kMaskWords - 1) / kMaskWords), a.pass.nq);
-  hipLaunchKernelGGL(seen_mask_kernel, grid, dim3(256), 0, s, a);
-  hipLaunchKernelGGL(seen_keys_kernel, dim3(a.pass.nq), dim3(256), 0, s, a);
+  const dim3 grid(static_cast<uint32_t>(1 + (a.mask_ld + kMaskWords - 1) / kMaskWords), a.pass.nq);
+  hipLaunchKernelGGL(seen_kernel, grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
