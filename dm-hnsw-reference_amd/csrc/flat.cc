@@ -268,7 +268,8 @@ int shine_flat_quantize(int gpu_id, const void* d_rows, int elem, uint64_t n, ui
   return hip("flat quantize", quantize(d_rows, elem, n, dim, ld, d_codes, d_scales, d_half_norms, static_cast<hipStream_t>(stream)));
 }
 
-uint64_t shine_flat_scores_workspace(uint32_t nq, uint32_t dim) {
+uint64_t shine_flat_scores_workspace(uint32_t nq, uint64_t n, uint32_t dim) {
+  if (F::scores_from_rows(nq, F::code_pitch(dim), n)) return 0;
   const uint64_t rows = std::min(nq, kRowBlock);
   return aligned(rows * F::code_pitch(dim)) + aligned(4 * rows);
 }
@@ -279,31 +280,40 @@ int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_q
   if (const char* w = check_rows(d_queries, elem, nq, table->dim, ld)) return fail(w);
   if (nq == 0 || table->n == 0) return SHINE_OK;
   if (const char* w = check_rows(d_out, out_elem, nq, table->n, out_ld)) return fail(w);
-  if (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < shine_flat_scores_workspace(nq, table->dim))
+  const uint64_t need = shine_flat_scores_workspace(nq, table->n, table->dim);
+  if (need && (!d_workspace || !on(d_workspace, kAlign) || workspace_bytes < need))
     return fail("workspace is missing, not 256-byte aligned or smaller than shine_flat_scores_workspace");
   OnDevice dev(gpu_id);
   if (dev.e != hipSuccess) return hip("flat scores: device", dev.e);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t pitch = F::code_pitch(table->dim);
   const uint64_t rows = std::min(nq, kRowBlock);
+  F::ScoresArgs a{};
+  a.codes = table->codes;
+  a.scales = table->scales;
+  a.bias = table->bias;
+  a.pitch = pitch;
+  a.n = table->n;
+  a.ld = out_ld;
+  if (need == 0) {
+    a.nq = nq;
+    a.out = d_out;
+    a.queries = d_queries;
+    a.queries_ld = ld;
+    a.dim = table->dim;
+    return hip("flat scores", F::launch_scores_of_rows(elem, out_elem, a, s));
+  }
   int8_t* codes = static_cast<int8_t*>(d_workspace);
   float* scales = reinterpret_cast<float*>(codes + aligned(rows * pitch));
+  a.qcodes = codes;
+  a.qscales = scales;
   for (uint32_t q = 0; q < nq; q += kRowBlock) {
     const uint32_t m = std::min(kRowBlock, nq - q);
     if (hipError_t e = quantize(static_cast<const char*>(d_queries) + q * ld * elem_size(elem), elem, m, table->dim, ld,
                                 codes, scales, nullptr, s); e != hipSuccess)
       return hip("flat scores", e);
-    F::ScoresArgs a{};
-    a.qcodes = codes;
-    a.qscales = scales;
-    a.codes = table->codes;
-    a.scales = table->scales;
-    a.bias = table->bias;
     a.nq = m;
-    a.pitch = pitch;
-    a.n = table->n;
     a.out = static_cast<char*>(d_out) + q * out_ld * elem_size(out_elem);
-    a.ld = out_ld;
     if (hipError_t e = F::launch_scores(out_elem, a, s); e != hipSuccess) return hip("flat scores", e);
   }
   return SHINE_OK;

@@ -36,7 +36,13 @@ struct ScoresArgs {
   uint64_t n;    // records of this launch
   void* out;
   uint64_t ld;   // in elements
+  // scores_of_rows: instead of qcodes and qscales
+  const void* queries;
+  uint64_t queries_ld;
+  uint32_t dim;
 };
+// Few queries with a small table: quantised in the launch that scores them.
+inline bool scores_from_rows(uint32_t nq, uint32_t pitch, uint64_t n) { return nq <= 16 && pitch <= 256 && n <= 1u << 18; }
 
 constexpr uint32_t kCountStride = 32;  // queries' counts lie in memory lines of their own: all XCDs add to them
 constexpr uint32_t kTermBytes = 16;    // of a record or a query in the threshold test
@@ -142,6 +148,7 @@ hipError_t launch_sample(const PassArgs& a, hipStream_t s);
 hipError_t launch_pass(const PassArgs& a, hipStream_t s);
 hipError_t launch_select(const SelectArgs& a, hipStream_t s);
 hipError_t launch_seen(const SeenArgs& a, hipStream_t s);
+hipError_t launch_scores_of_rows(int elem, int out_elem, const ScoresArgs& a, hipStream_t s);
 hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s);
 hipError_t launch_topk(int elem, bool keys_only, const TopkArgs& a, hipStream_t s);
 hipError_t launch_merge(int elem, const MergeArgs& a, hipStream_t s);

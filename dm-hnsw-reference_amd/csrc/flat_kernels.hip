@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "flat.h"
 
@@ -37,18 +38,29 @@ __device__ inline __bf16 from_f32<__bf16>(float x) { return static_cast<__bf16>(
 // near scale / 2 (x and code * scale are multiples of a common unit there, their difference a 24-bit multiple of it).
 // For scales below 1e-30, where 1 / scale may be infinite, the quotient is taken in 64 bits: it is off by 2^-53, and a
 // quotient of 24-bit numbers that is no half is at least 2^-33 from every half.
-__device__ inline int code_of(float x, float scale, float inv) {
-  float m;
-  if (scale >= 1e-30f) {
-    m = rintf(x * inv);
-    const float e = fmaf(-m, scale, x), e2 = 2.0f * fabsf(e);
-    const float step = e > 0.0f ? 1.0f : -1.0f;
-    if (e2 > scale || (e2 == scale && (static_cast<int>(m) & 1))) m += step;
-  } else {
-    m = static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(scale)));
+struct Scale {
+  float scale, inv;
+  bool some;  // the row has codes other than 0
+  __device__ explicit Scale(uint32_t top) {  // the largest magnitude's bits
+    const bool finite = top < 0x7F800000u;
+    scale = finite ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7FC00000u);
+    some = finite && scale > 0.0f;
+    inv = 1.0f / scale;
   }
-  return static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f));
-}
+  __device__ int code(float x) const {
+    if (!some) return 0;
+    float m;
+    if (scale >= 1e-30f) {
+      m = rintf(x * inv);
+      const float e = fmaf(-m, scale, x), e2 = 2.0f * fabsf(e);
+      const float step = e > 0.0f ? 1.0f : -1.0f;
+      if (e2 > scale || (e2 == scale && (static_cast<int>(m) & 1))) m += step;
+    } else {
+      m = static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(scale)));
+    }
+    return static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f));
+  }
+};
 
 // V = 16 bytes of components that a lane takes in a step; components behind dim are 0
 template <class T, int V>
@@ -64,66 +76,73 @@ __device__ inline void load_components(float (&x)[V], const T* src, uint32_t c, 
 }
 
 // G lanes per row and S steps of 16 bytes a lane, held in registers between the maximum and the codes (S = 0: rows too wide
-// for that are read twice).
-template <class T, int G, int S>
+// for that are read twice).  A group takes R rows, all of them asked for before the first is looked at: with one row each,
+// too few bytes are on their way (1M x 128 f32: 200 us with one row, FIXME with four).
+template <class T, int G, int S, int R>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a, uint32_t pitch) {
   constexpr int V = 16 / sizeof(T), H = S ? S : 1;
   const uint32_t lane = threadIdx.x % G;
-  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (256 / G) + threadIdx.x / G;
-  if (row >= a.n) return;
-  const T* src = static_cast<const T*>(a.rows) + row * a.ld;
-  float x[H][V];
-  uint32_t top = 0;
-  auto raise = [&top](const float(&v)[V]) {
+  const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * (256 / G * R) + threadIdx.x / G;
+  float x[R][H][V];
+  if (S)
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  };
-  if (S) {
+    for (int k = 0; k < R; ++k) {
+      const T* src = static_cast<const T*>(a.rows) + min(row0 + k * (256 / G), a.n - 1) * a.ld;
 #pragma unroll
-    for (int j = 0; j < H; ++j) load_components<T, V>(x[j], src, (j * G + lane) * V, a.dim);
-#pragma unroll
-    for (int j = 0; j < H; ++j) raise(x[j]);
-  } else {
-    for (uint32_t c = lane * V; c < a.dim; c += G * V) {
-      load_components<T, V>(x[0], src, c, a.dim);
-      raise(x[0]);
+      for (int j = 0; j < H; ++j) load_components<T, V>(x[k][j], src, (j * G + lane) * V, a.dim);
     }
-  }
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, G)));
-  const bool finite = top < 0x7F800000u;
-  const float scale = finite ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7FC00000u);
-  const bool some = finite && scale > 0.0f;
-  const float inv = 1.0f / scale;
-  int squares = 0;
-  auto write = [&](const float(&v)[V], uint32_t c) {
-    uint32_t packed[V / 4] = {};
+  for (int k = 0; k < R; ++k) {
+    const uint64_t row = row0 + k * (256 / G);
+    if (row >= a.n) return;
+    const T* src = static_cast<const T*>(a.rows) + row * a.ld;
+    uint32_t top = 0;
+    auto raise = [&top](const float(&v)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int code = some ? code_of(v[i], scale, inv) : 0;
-      squares += code * code;
-      packed[i / 4] |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * (i % 4));
+      for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    };
+    if (S) {
+#pragma unroll
+      for (int j = 0; j < H; ++j) raise(x[k][j]);
+    } else {
+      for (uint32_t c = lane * V; c < a.dim; c += G * V) {
+        load_components<T, V>(x[0][0], src, c, a.dim);
+        raise(x[0][0]);
+      }
     }
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.codes + row * pitch + c);
-    if (V == 4) *dst = packed[0];
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[V / 4 - 1]);
-  };
-  if (S) {
 #pragma unroll
-    for (int j = 0; j < H; ++j)
-      if ((j * G + lane) * V < pitch) write(x[j], (j * G + lane) * V);
-  } else {
-    for (uint32_t c = lane * V; c < pitch; c += G * V) {
-      load_components<T, V>(x[0], src, c, a.dim);
-      write(x[0], c);
+    for (int o = G / 2; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, G)));
+    const Scale s(top);
+    int squares = 0;
+    auto write = [&](const float(&v)[V], uint32_t c) {
+      uint32_t packed[V / 4] = {};
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int code = s.code(v[i]);
+        squares += code * code;
+        packed[i / 4] |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * (i % 4));
+      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(a.codes + row * pitch + c);
+      if (V == 4) *dst = packed[0];
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[V / 4 - 1]);
+    };
+    if (S) {
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+        if ((j * G + lane) * V < pitch) write(x[k][j], (j * G + lane) * V);
+    } else {
+      for (uint32_t c = lane * V; c < pitch; c += G * V) {
+        load_components<T, V>(x[0][0], src, c, a.dim);
+        write(x[0][0], c);
+      }
     }
-  }
-  if (a.half_norms)
+    if (a.half_norms)
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
-  if (lane == 0) {
-    a.scales[row] = scale;
-    if (a.half_norms) a.half_norms[row] = -0.5f * ((static_cast<float>(squares) * scale) * scale);
+      for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
+    if (lane == 0) {
+      a.scales[row] = s.scale;
+      if (a.half_norms) a.half_norms[row] = -0.5f * ((static_cast<float>(squares) * s.scale) * s.scale);
+    }
   }
 }
 
@@ -245,7 +264,21 @@ struct Order {
 // the writes: memory accesses end in order, so what waits for a load must know how many writes are behind it.  Lanes
 // whose query is behind the last one hold the last one and write its scores once more; the block that the records end in
 // comes last, on its own.
-template <class T, int KC, int QT>
+//
+// E (not void): the queries' element type; each wave quantises its 16 queries itself, which saves a launch where few blocks
+// follow (1 x 10,000 x 128: FIXME).
+template <class E>
+__device__ inline void quantize_fragment(v4i& codes, const Scale& s, const float (&x)[16]) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t packed = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) packed |= (static_cast<uint32_t>(s.code(x[w * 4 + j])) & 0xFFu) << (8 * j);
+    codes[w] = static_cast<int>(packed);
+  }
+}
+
+template <class T, int KC, int QT, class E>
 __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per_range) {
   __shared__ float beside[4][2][32];  // each wave's records' scales and biases
   const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
@@ -255,15 +288,40 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
                  b1 = b0 + per_range < blocks ? b0 + per_range : blocks;
   if (b0 + wave >= b1) return;
   v4i q[QT][KC];
-  load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   float qs[QT];
   T* to[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t r = min(query0 + i * 16 + col, a.nq - 1);
-    qs[i] = a.qscales[r];
     to[i] = static_cast<T*>(a.out) + r * a.ld;
+    if constexpr (std::is_void_v<E>) {
+      qs[i] = a.qscales[r];
+    } else {
+      constexpr int V = 16 / sizeof(E);
+      const E* src = static_cast<const E*>(a.queries) + r * a.queries_ld;
+      float x[KC][16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int h = 0; h < 16; h += V) {
+          float part[V];
+          load_components<E, V>(part, src, c * 64 + group * 16 + h, a.dim);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            x[c][h + j] = part[j];
+            top = max(top, __float_as_uint(part[j]) & 0x7FFFFFFFu);
+          }
+        }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+      const Scale s(top);
+      qs[i] = s.scale;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) quantize_fragment<E>(q[i][c], s, x[c]);
+    }
   }
+  if constexpr (std::is_void_v<E>) load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
   const v4i start = magic_start();
   const float* biases = a.bias ? a.bias : a.scales;
   Block<KC> next;
@@ -1365,20 +1423,22 @@ __global__ __launch_bounds__(256) void seen_kernel(SeenArgs a) {
     default: return hipErrorInvalidValue;         \
   }
 
+template <class T, int G, int S, int R>
+void quantize_with(const QuantizeArgs& a, uint32_t pitch, hipStream_t s) {
+  constexpr uint32_t rows = 256 / G * R;
+  hipLaunchKernelGGL((quantize_kernel<T, G, S, R>), dim3(static_cast<uint32_t>((a.n + rows - 1) / rows)), dim3(256), 0, s, a, pitch);
+}
 template <class T>
 void quantize_by_width(const QuantizeArgs& a, hipStream_t s) {
   const uint32_t pitch = code_pitch(a.dim), steps = pitch * sizeof(T) / 16;  // 16-byte steps of a row
-#define SHINE_GROUP(GG, SS)                                                                                    \
-  hipLaunchKernelGGL((quantize_kernel<T, GG, SS>), dim3(static_cast<uint32_t>((a.n + 256 / GG - 1) / (256 / GG))), \
-                     dim3(256), 0, s, a, pitch)
-  if (steps <= 8) SHINE_GROUP(8, 1);
-  else if (steps <= 16) SHINE_GROUP(16, 1);
-  else if (steps <= 32) SHINE_GROUP(32, 1);
-  else if (steps <= 64) SHINE_GROUP(64, 1);
-  else if (steps <= 128) SHINE_GROUP(64, 2);
-  else if (steps <= 256) SHINE_GROUP(64, 4);
-  else SHINE_GROUP(64, 0);
-#undef SHINE_GROUP
+  const bool many = a.n * steps >= 1u << 20;  // enough to fill the GPU with groups of four rows
+  if (steps <= 8) many ? quantize_with<T, 8, 1, 4>(a, pitch, s) : quantize_with<T, 8, 1, 1>(a, pitch, s);
+  else if (steps <= 16) many ? quantize_with<T, 16, 1, 4>(a, pitch, s) : quantize_with<T, 16, 1, 1>(a, pitch, s);
+  else if (steps <= 32) many ? quantize_with<T, 32, 1, 4>(a, pitch, s) : quantize_with<T, 32, 1, 1>(a, pitch, s);
+  else if (steps <= 64) many ? quantize_with<T, 64, 1, 4>(a, pitch, s) : quantize_with<T, 64, 1, 1>(a, pitch, s);
+  else if (steps <= 128) quantize_with<T, 64, 2, 1>(a, pitch, s);
+  else if (steps <= 256) quantize_with<T, 64, 4, 1>(a, pitch, s);
+  else quantize_with<T, 64, 0, 1>(a, pitch, s);
 }
 
 hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s) {
@@ -1401,6 +1461,33 @@ Ranges ranges_of(uint64_t blocks, uint32_t query_blocks, uint32_t want) {
 }
 }  // namespace
 
+template <class T, class E>
+void scores_of_rows(const ScoresArgs& a, hipStream_t s) {
+  const Ranges r = ranges_of((a.n + 31) / 32, 1, 1024);
+  switch (a.pitch / 64) {
+    case 1: hipLaunchKernelGGL((scores_stream_kernel<T, 1, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
+    case 2: hipLaunchKernelGGL((scores_stream_kernel<T, 2, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
+    case 3: hipLaunchKernelGGL((scores_stream_kernel<T, 3, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
+    default: hipLaunchKernelGGL((scores_stream_kernel<T, 4, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
+  }
+}
+
+template <class T>
+hipError_t scores_of(int elem, const ScoresArgs& a, hipStream_t s) {
+  switch (elem) {
+    case kF32: scores_of_rows<T, float>(a, s); break;
+    case kF16: scores_of_rows<T, __half>(a, s); break;
+    case kBF16: scores_of_rows<T, __bf16>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_scores_of_rows(int elem, int out_elem, const ScoresArgs& a, hipStream_t s) {
+  SHINE_BY_ELEM(out_elem, return scores_of<T>(elem, a, s));
+  return hipErrorInvalidValue;
+}
+
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   // Up to 32 queries: streams of any number of workgroups, the more the better where the table's bytes count (1 x 4M x 128:
   // 107 us with 4096, 113 with 512).  More: rows of 128 codes stream in 512 workgroups (1024 x 100,000 x 96: 46 us with bf16
@@ -1411,7 +1498,7 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   {                                                                                                       \
     const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                 \
     const Ranges r = ranges_of((a.n + 31) / 32, qb, WANT);                                                \
-    hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);   \
+    hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ, void>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);   \
   }
     SHINE_BY_ELEM(out_elem, switch (a.pitch / 64) {
       case 1: if (a.nq <= 16) SHINE_STREAM(1, 1, 4096) else if (a.nq <= 32) SHINE_STREAM(1, 2, 2048) else SHINE_STREAM(1, 8, 512) break;

@@ -227,7 +227,7 @@ PROTOTYPES = {
     "shine_gpu_build_free": (I32, [P]),
     "shine_flat_pitch": (U32, [U32]),
     "shine_flat_quantize": (I32, [I32, P, I32, U64, U32, U64, P, P, P, P]),
-    "shine_flat_scores_workspace": (U64, [U32, U32]),
+    "shine_flat_scores_workspace": (U64, [U32, U64, U32]),
     "shine_flat_scores": (I32, [I32, C.POINTER(FlatTable), P, I32, U32, U64, P, I32, U64, P, U64, P]),
     "shine_flat_adjust": (I32, [I32, P, I32, U32, U64, U64, C.POINTER(FlatAdjustment), P, U64, P]),
     "shine_flat_topk_workspace": (U64, [U32, U64, U32]),

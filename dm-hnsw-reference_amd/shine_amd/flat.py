@@ -24,15 +24,18 @@ from . import _lib as L
 MAX_K = 256
 MAX_DIM = 16384
 
-_torch = None
+_torch = _current = None
 _elems = {}
 
 
 def _t():
-    global _torch
+    global _torch, _current
     if _torch is None:
         import torch
         _torch = torch
+        # the stream's handle alone where torch gives it: a Stream object costs 2 us a call
+        _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: torch.cuda.current_stream(index).cuda_stream)
         _elems.update({torch.float32: L.ELEM_F32, torch.float16: L.ELEM_F16, torch.bfloat16: L.ELEM_BF16})
     return _torch
 
@@ -92,7 +95,7 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
 
 
 def _stream(device) -> int:
-    return _t().cuda.current_stream(device).cuda_stream
+    return _current(device.index)
 
 
 def _workspace(size: int, device):
@@ -172,7 +175,7 @@ def scores(table: FlatTable, queries, dtype=None, out=None):
         raise ValueError(f"out must be ({nq}, {table.n}) of the asked dtype")
     optr, oelem, old = _rows(out, "out", table.device)
     lib = L.lib()
-    size = lib.shine_flat_scores_workspace(nq, table.dim)
+    size = lib.shine_flat_scores_workspace(nq, table.n, table.dim)
     ws = _workspace(size, table.device)
     L.check(lib.shine_flat_scores(table.device.index, C.byref(table._c), ptr, elem, nq, ld, optr, oelem, old,
                                   ws.data_ptr() if size else None, size, _stream(table.device)))

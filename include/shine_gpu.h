@@ -481,7 +481,7 @@ int shine_flat_quantize(int gpu_id, const void* d_rows, int elem, uint64_t n, ui
 
 /* out[i][j] = (float(sum of code products) * query scale i) * table scale j (+ table bias j), each step rounded to f32 (the
  * sum is exact), the result rounded to out_elem.  The queries are quantised as shine_flat_quantize does. */
-uint64_t shine_flat_scores_workspace(uint32_t nq, uint32_t dim);
+uint64_t shine_flat_scores_workspace(uint32_t nq, uint64_t n, uint32_t dim); /* a workspace of size 0 may be NULL */
 int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
                       void* d_out, int out_elem, uint64_t out_ld, void* d_workspace, uint64_t workspace_bytes, void* stream);
 

@@ -36,7 +36,8 @@ def test_pitch_and_workspaces():
     lib = L.lib()
     for dim, pitch in ((1, 64), (64, 64), (65, 128), (96, 128), (200, 256), (16384, 16384)):
         assert lib.shine_flat_pitch(dim) == pitch == flat.code_pitch(dim)
-    assert lib.shine_flat_scores_workspace(7, 96) >= 7 * 128 + 7 * 4
+    assert lib.shine_flat_scores_workspace(17, 1000, 96) >= 17 * 128 + 17 * 4
+    assert lib.shine_flat_scores_workspace(7, 1 << 20, 96) >= 7 * 128 + 7 * 4
     assert lib.shine_flat_search_workspace(7, 1000, 96, 10, None) >= 7 * 128 + 7 * 4
 
 
@@ -68,9 +69,9 @@ def test_scores_refusals():
     refused(f(0, table(), P, 0, 4, 31, P, 0, 100, P, big, None), "stride")
     refused(f(0, table(), P, 0, 4, 32, P, 2, 100, P, big, None), "element type")
     refused(f(0, table(), P, 0, 4, 32, P, 0, 99, P, big, None), "stride")
-    refused(f(0, table(), P, 0, 4, 32, P, 0, 100, None, big, None), "workspace")
-    refused(f(0, table(), P, 0, 4, 32, P, 0, 100, P + 128, big, None), "workspace")
-    refused(f(0, table(), P, 0, 4, 32, P, 0, 100, P, 100, None), "workspace")
+    refused(f(0, table(), P, 0, 17, 32, P, 0, 100, None, big, None), "workspace")
+    refused(f(0, table(), P, 0, 17, 32, P, 0, 100, P + 128, big, None), "workspace")
+    refused(f(0, table(), P, 0, 17, 32, P, 0, 100, P, 100, None), "workspace")
     assert f(0, table(), None, 0, 0, 32, None, 0, 100, None, 0, None) == L.OK
     assert f(0, table(n=0, codes=None, scales=None), P, 0, 4, 32, None, 0, 0, None, 0, None) == L.OK
 
