@@ -39,13 +39,14 @@ __device__ inline __bf16 from_f32<__bf16>(float x) { return static_cast<__bf16>(
 // For scales below 1e-30, where 1 / scale may be infinite, the quotient is taken in 64 bits: it is off by 2^-53, and a
 // quotient of 24-bit numbers that is no half is at least 2^-33 from every half.
 struct Scale {
-  float scale, inv;
+  float scale, inv, near;
   bool some;  // the row has codes other than 0
   __device__ explicit Scale(uint32_t top) {  // the largest magnitude's bits
     const bool finite = top < 0x7F800000u;
     scale = finite ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7FC00000u);
     some = finite && scale > 0.0f;
     inv = 1.0f / scale;
+    near = scale * 0.4999995f;
   }
   __device__ int code(float x) const {
     if (!some) return 0;
@@ -59,6 +60,25 @@ struct Scale {
       m = static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(scale)));
     }
     return static_cast<int>(fminf(fmaxf(m, -127.0f), 127.0f));
+  }
+  // Four codes in a word.  A remainder below `near` needs no correction and its integer no clamp (|x| <= the largest), so the
+  // four are corrected together or, nearly always, not at all: seven operations a component instead of about fifty.
+  __device__ uint32_t codes(const float* x) const {
+    uint32_t packed = 0;
+    float worst = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = rintf(x[i] * inv);
+      worst = fmaxf(worst, fabsf(fmaf(-m, scale, x[i])));
+      packed = __builtin_amdgcn_cvt_pk_u8_f32(m + 128.0f, i, packed);
+    }
+    packed ^= 0x80808080u;
+    if (!some || !(worst < near) || scale < 1e-30f) {
+      packed = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) packed |= (static_cast<uint32_t>(code(x[i])) & 0xFFu) << (8 * i);
+    }
+    return packed;
   }
 };
 
@@ -76,72 +96,85 @@ __device__ inline void load_components(float (&x)[V], const T* src, uint32_t c, 
 }
 
 // G lanes per row and S steps of 16 bytes a lane, held in registers between the maximum and the codes (S = 0: rows too wide
-// for that are read twice).  A group takes R rows, all of them asked for before the first is looked at: with one row each,
-// too few bytes are on their way (1M x 128 f32: 200 us with one row, FIXME with four).
+// for that are read twice).  A group takes R rows a turn and asks for the next turn's before it looks at this one's.  Bound by
+// HBM: 1M x 128 f32 takes 133 us, 4.8 TB/s, where a copy reaches 5.1; one row a turn takes 181 to 216, four rows 184, and
+// of 1,024 .. 8,192 workgroups and one for every turn 8,192 are best or near it for each width and type.
 template <class T, int G, int S, int R>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a, uint32_t pitch) {
   constexpr int V = 16 / sizeof(T), H = S ? S : 1;
+  constexpr uint32_t kRows = 256 / G * R;  // of a workgroup's turn
   const uint32_t lane = threadIdx.x % G;
-  const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * (256 / G * R) + threadIdx.x / G;
-  float x[R][H][V];
-  if (S)
+  float next[R][H][V];
+  auto fetch = [&](uint64_t row0) {
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       const T* src = static_cast<const T*>(a.rows) + min(row0 + k * (256 / G), a.n - 1) * a.ld;
 #pragma unroll
-      for (int j = 0; j < H; ++j) load_components<T, V>(x[k][j], src, (j * G + lane) * V, a.dim);
+      for (int j = 0; j < H; ++j) load_components<T, V>(next[k][j], src, (j * G + lane) * V, a.dim);
     }
+  };
+  uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kRows + threadIdx.x / G;
+  if (S) fetch(row0);
+  for (; row0 < a.n; row0 += static_cast<uint64_t>(gridDim.x) * kRows) {
+    float x[R][H][V];
 #pragma unroll
-  for (int k = 0; k < R; ++k) {
-    const uint64_t row = row0 + k * (256 / G);
-    if (row >= a.n) return;
-    const T* src = static_cast<const T*>(a.rows) + row * a.ld;
-    uint32_t top = 0;
-    auto raise = [&top](const float(&v)[V]) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    };
-    if (S) {
-#pragma unroll
-      for (int j = 0; j < H; ++j) raise(x[k][j]);
-    } else {
-      for (uint32_t c = lane * V; c < a.dim; c += G * V) {
-        load_components<T, V>(x[0][0], src, c, a.dim);
-        raise(x[0][0]);
-      }
-    }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, G)));
-    const Scale s(top);
-    int squares = 0;
-    auto write = [&](const float(&v)[V], uint32_t c) {
-      uint32_t packed[V / 4] = {};
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int code = s.code(v[i]);
-        squares += code * code;
-        packed[i / 4] |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * (i % 4));
-      }
-      uint32_t* dst = reinterpret_cast<uint32_t*>(a.codes + row * pitch + c);
-      if (V == 4) *dst = packed[0];
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[V / 4 - 1]);
-    };
-    if (S) {
+    for (int k = 0; k < R; ++k)
 #pragma unroll
       for (int j = 0; j < H; ++j)
-        if ((j * G + lane) * V < pitch) write(x[k][j], (j * G + lane) * V);
-    } else {
-      for (uint32_t c = lane * V; c < pitch; c += G * V) {
-        load_components<T, V>(x[0][0], src, c, a.dim);
-        write(x[0][0], c);
-      }
-    }
-    if (a.half_norms)
 #pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
-    if (lane == 0) {
-      a.scales[row] = s.scale;
-      if (a.half_norms) a.half_norms[row] = -0.5f * ((static_cast<float>(squares) * s.scale) * s.scale);
+        for (int i = 0; i < V; ++i) x[k][j][i] = next[k][j][i];
+    if (S) fetch(row0 + static_cast<uint64_t>(gridDim.x) * kRows);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const uint64_t row = row0 + k * (256 / G);
+      if (row >= a.n) break;
+      const T* src = static_cast<const T*>(a.rows) + row * a.ld;
+      uint32_t top = 0;
+      auto raise = [&top](const float(&v)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+      };
+      if (S) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) raise(x[k][j]);
+      } else {
+        for (uint32_t c = lane * V; c < a.dim; c += G * V) {
+          load_components<T, V>(x[0][0], src, c, a.dim);
+          raise(x[0][0]);
+        }
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, G)));
+      const Scale s(top);
+      int squares = 0;
+      auto write = [&](const float(&v)[V], uint32_t c) {
+        uint32_t packed[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          packed[i] = s.codes(v + i * 4);
+          squares = __builtin_amdgcn_sdot4(static_cast<int>(packed[i]), static_cast<int>(packed[i]), squares, false);
+        }
+        uint32_t* dst = reinterpret_cast<uint32_t*>(a.codes + row * pitch + c);
+        if (V == 4) *dst = packed[0];
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[V / 4 - 1]);
+      };
+      if (S) {
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+          if ((j * G + lane) * V < pitch) write(x[k][j], (j * G + lane) * V);
+      } else {
+        for (uint32_t c = lane * V; c < pitch; c += G * V) {
+          load_components<T, V>(x[0][0], src, c, a.dim);
+          write(x[0][0], c);
+        }
+      }
+      if (a.half_norms)
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) squares += __shfl_xor(squares, o, G);
+      if (lane == 0) {
+        a.scales[row] = s.scale;
+        if (a.half_norms) a.half_norms[row] = -0.5f * ((static_cast<float>(squares) * s.scale) * s.scale);
+      }
     }
   }
 }
@@ -266,16 +299,11 @@ struct Order {
 // comes last, on its own.
 //
 // E (not void): the queries' element type; each wave quantises its 16 queries itself, which saves a launch where few blocks
-// follow (1 x 10,000 x 128: FIXME).
+// follow (1 x 10,000 x 128: 8.7 us a call against 15.0).
 template <class E>
 __device__ inline void quantize_fragment(v4i& codes, const Scale& s, const float (&x)[16]) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint32_t packed = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) packed |= (static_cast<uint32_t>(s.code(x[w * 4 + j])) & 0xFFu) << (8 * j);
-    codes[w] = static_cast<int>(packed);
-  }
+  for (int w = 0; w < 4; ++w) codes[w] = static_cast<int>(s.codes(x + w * 4));
 }
 
 template <class T, int KC, int QT, class E>
@@ -973,7 +1001,7 @@ __device__ inline uint64_t offered_key(float v, uint64_t record) {
 // a product of four numbers of the record with four of the query, added to a sum that is already there: kMagic + sum is a
 // float (kMagic's), so one 32x32x8 bf16 instruction takes it as its start and leaves the margin in units of the integer
 // sum.  Per score that leaves half a maximum to the vector unit, where scaling takes two
-// fused multiply-adds (1024 x 1M x 128: FIXME us a pass against 244).  A number goes in as two bf16 (2^-17 of it is
+// fused multiply-adds (the last pass of 1024 x 1M x 128 fell from 244 to 211 us with it).  A number goes in as two bf16 (2^-17 of it is
 // lost), a product as three; the margin is raised by kSlack counts and 2^-13 of its terms, more than this, the roundings of
 // the additions and those of the definition come to.  What passes is scored again as the definition rounds.
 //
@@ -1426,16 +1454,16 @@ __global__ __launch_bounds__(256) void seen_kernel(SeenArgs a) {
 template <class T, int G, int S, int R>
 void quantize_with(const QuantizeArgs& a, uint32_t pitch, hipStream_t s) {
   constexpr uint32_t rows = 256 / G * R;
-  hipLaunchKernelGGL((quantize_kernel<T, G, S, R>), dim3(static_cast<uint32_t>((a.n + rows - 1) / rows)), dim3(256), 0, s, a, pitch);
+  const uint64_t groups = std::min<uint64_t>((a.n + rows - 1) / rows, 8192);
+  hipLaunchKernelGGL((quantize_kernel<T, G, S, R>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0, s, a, pitch);
 }
 template <class T>
 void quantize_by_width(const QuantizeArgs& a, hipStream_t s) {
   const uint32_t pitch = code_pitch(a.dim), steps = pitch * sizeof(T) / 16;  // 16-byte steps of a row
-  const bool many = a.n * steps >= 1u << 20;  // enough to fill the GPU with groups of four rows
-  if (steps <= 8) many ? quantize_with<T, 8, 1, 4>(a, pitch, s) : quantize_with<T, 8, 1, 1>(a, pitch, s);
-  else if (steps <= 16) many ? quantize_with<T, 16, 1, 4>(a, pitch, s) : quantize_with<T, 16, 1, 1>(a, pitch, s);
-  else if (steps <= 32) many ? quantize_with<T, 32, 1, 4>(a, pitch, s) : quantize_with<T, 32, 1, 1>(a, pitch, s);
-  else if (steps <= 64) many ? quantize_with<T, 64, 1, 4>(a, pitch, s) : quantize_with<T, 64, 1, 1>(a, pitch, s);
+  if (steps <= 8) quantize_with<T, 8, 1, 2>(a, pitch, s);
+  else if (steps <= 16) quantize_with<T, 16, 1, 2>(a, pitch, s);
+  else if (steps <= 32) quantize_with<T, 32, 1, 2>(a, pitch, s);
+  else if (steps <= 64) quantize_with<T, 64, 1, 2>(a, pitch, s);
   else if (steps <= 128) quantize_with<T, 64, 2, 1>(a, pitch, s);
   else if (steps <= 256) quantize_with<T, 64, 4, 1>(a, pitch, s);
   else quantize_with<T, 64, 0, 1>(a, pitch, s);
