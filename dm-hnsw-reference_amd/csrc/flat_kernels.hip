@@ -307,12 +307,10 @@ __device__ inline void quantize_fragment(v4i& codes, const Scale& s, const float
 }
 
 template <class T, int KC, int QT, class E>
-__global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per_range) {
+__global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint64_t per_range) {
   __shared__ float beside[4][2][32];  // each wave's records' scales and biases
   const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
-  const Place at = place_of(query_blocks);
-  const uint32_t query0 = at.query_block * QT * 16;
-  const uint64_t blocks = (a.n + 31) / 32, whole = a.n / 32, b0 = at.range * per_range,
+  const uint64_t blocks = (a.n + 31) / 32, whole = a.n / 32, b0 = blockIdx.x * per_range,
                  b1 = b0 + per_range < blocks ? b0 + per_range : blocks;
   if (b0 + wave >= b1) return;
   v4i q[QT][KC];
@@ -320,7 +318,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
   T* to[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const uint32_t r = min(query0 + i * 16 + col, a.nq - 1);
+    const uint32_t r = min(i * 16 + col, a.nq - 1);
     to[i] = static_cast<T*>(a.out) + r * a.ld;
     if constexpr (std::is_void_v<E>) {
       qs[i] = a.qscales[r];
@@ -349,7 +347,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
       for (int c = 0; c < KC; ++c) quantize_fragment<E>(q[i][c], s, x[c]);
     }
   }
-  if constexpr (std::is_void_v<E>) load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
+  if constexpr (std::is_void_v<E>) load_queries<KC, QT>(q, a.qcodes, 0, a.nq);
   const v4i start = magic_start();
   const float* biases = a.bias ? a.bias : a.scales;
   Block<KC> next;
@@ -410,6 +408,136 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint32
       Order<T>::store(to[i] + b * 32, group, v, static_cast<uint32_t>(a.n - b * 32));
     }
   }
+}
+
+// More than 32 queries write more than they read: 128-byte lines of the rows, each whole and by one instruction, whatever the
+// rows' starts.  Lines written in parts cost the memory a read and a write each where a part is evicted before the other comes
+// (rows of 100,003 f32 in the streams above: 8.05M write requests, 0.85M of them partial, for 6.4M lines' halves).  A wave keeps
+// QT * 16 queries and goes through neighbouring records, a line's number of them a turn.  Queries are the products' rows, so
+// that a lane has its record's scale and bias in registers and sums of four queries.  A row's scores go into a ring of two lines
+// in LDS, at the offsets that they have in memory's lines; what completes a line is written, the rest is there for the next
+// turn.  Rings of 16 queries are turned against one another so that the 64 lanes of a write, and of a read, meet different banks.
+//
+// A run's first line begins in the records before: long runs of f32 score them again (one turn more of 8 or more), short ones and
+// 16-bit scores, whose turns are twice as long, write the line's part.  1024 x 100,003 x 96, kernel and quantising: f32 162 -> 106 us (the part: 119),
+// bf16 78 -> 55 (scored again: 58); rows of 100,000: 114 -> 105 and 47 -> 50.  128 queries a wave: 130 and 75; 32, with four
+// waves a SIMD: 125 and 90.  What bounds it is the writing, 4.1 TB/s of 6.7 that a fill reaches.
+template <class T, int KC, int QT>
+__global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per) {
+  constexpr uint32_t kLine = 128 / sizeof(T), kPiece = 16 / sizeof(T);  // scores of a line and of 16 bytes
+  constexpr int NT = kLine / 16, U = QT * 2;
+  const bool again = sizeof(T) == 4 && per >= 8;
+  __shared__ __attribute__((aligned(16))) uint8_t rings[4][QT * 16][256];
+  const uint32_t lane = threadIdx.x & 63, wave = wave_number(), col = lane & 15, group = lane >> 4;
+  const Place at = place_of(query_blocks);
+  const uint32_t query0 = at.query_block * QT * 16;
+  const uint64_t lines = (a.n + kLine - 1) / kLine, first = (at.range * 4ull + wave) * per, end = min(first + per, lines);
+  if (first >= end) return;
+  uint8_t* ring = &rings[wave][0][0];
+  T* out = static_cast<T*>(a.out);
+  auto row_of = [&](uint32_t r) { return out + min(query0 + r, a.nq - 1) * a.ld; };
+  auto turned = [](uint32_t r) { return (r & 1) * 128 + (r >> 2 & 3) * 64; };
+  v4i q[QT][KC];
+  load_queries<KC, QT>(q, a.qcodes, query0, a.nq);
+  float qs[QT][4];
+  uint32_t place[QT];  // a byte each for four rows: where in their rings column 0 of an even block's first tile goes
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    place[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t r = i * 16 + group * 4 + j;
+      qs[i][j] = a.qscales[min(query0 + r, a.nq - 1)];
+      const uint32_t shift = reinterpret_cast<uint64_t>(row_of(r)) & 127;
+      place[i] |= ((turned(r) + shift + col * sizeof(T)) & 255) << (8 * j);
+    }
+  }
+  uint64_t line[U];  // where the line goes that holds the first score of a row
+#pragma unroll
+  for (int u = 0; u < U; ++u) line[u] = (reinterpret_cast<uint64_t>(row_of(u * 8 + (lane >> 3))) & ~127ull) + (lane & 7) * 16;
+  const v4i start = magic_start();
+  const float* biases = a.bias ? a.bias : a.scales;
+  const bool biased = a.bias;
+  v4i next[NT][KC], x[NT][KC];
+  float next_xs[NT], next_bias[NT], xs[NT], bias[NT];
+  auto fetch = [&](uint64_t b) {
+    const int8_t* p = a.codes + b * (kLine * KC * 64);
+    const uint32_t last = static_cast<uint32_t>(min(a.n - b * kLine, static_cast<uint64_t>(kLine))) - 1;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t r = min(t * 16 + col, last);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) next[t][c] = *reinterpret_cast<const v4i*>(p + r * (KC * 64) + group * 16 + c * 64);
+      next_xs[t] = (a.scales + b * kLine)[r];
+      next_bias[t] = (biases + b * kLine)[r];
+    }
+  };
+  auto stage = [&] {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        x[t][c] = next[t][c];
+        asm volatile("" : "+v"(x[t][c]));
+      }
+      xs[t] = next_xs[t];
+      bias[t] = biased ? next_bias[t] : -0.0f;
+      asm volatile("" : "+v"(xs[t]), "+v"(bias[t]));
+    }
+  };
+  auto ring_piece = [&](uint32_t r, uint32_t parity) { return ring + r * 256 + ((turned(r) + parity + (lane & 7) * 16) & 255); };
+  // the scores [from, to) of line b: pieces of 16 bytes, or one by one where a piece is not all of these
+  auto edge = [&](uint64_t b, uint32_t parity, uint64_t from, uint64_t to) {
+#pragma unroll 2
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t r = u * 8 + (lane >> 3);
+      T* row = row_of(r);
+      const int64_t at = static_cast<int64_t>(b * kLine) + (lane & 7) * kPiece - (reinterpret_cast<uint64_t>(row) & 127) / sizeof(T);
+      const Vec<T, kPiece> v = *reinterpret_cast<const Vec<T, kPiece>*>(ring_piece(r, parity));
+      const int64_t low = from, high = to;
+      if (at >= low && at + kPiece <= high) {
+        *reinterpret_cast<Vec<T, kPiece>*>(row + at) = v;
+      } else if (at + kPiece > low && at < high) {
+#pragma unroll
+        for (uint32_t e = 0; e < kPiece; ++e)
+          if (at + e >= low && at + e < high) row[at + e] = v.v[e];
+      }
+    }
+  };
+  const uint64_t b0 = again && first ? first - 1 : first, from = again ? 0 : first * kLine;
+  fetch(b0);
+  stage();
+  uint32_t parity = 0;
+  for (uint64_t b = b0; b < end; ++b, parity ^= 128) {
+    fetch(b + 1 < end ? b + 1 : b);
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        v4i acc = start;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i][c], x[t][c], acc, 0, 0, 0);
+        const uint32_t to = ((place[i] & 0x7F7F7F7Fu) + t * 16 * sizeof(T) * 0x01010101u) ^ (place[i] & 0x80808080u) ^ parity * 0x01010101u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<T*>(ring + (i * 16 + group * 4 + j) * 256 + (to >> (8 * j) & 255)) =
+              from_f32<T>(((__int_as_float(acc[j]) - kMagicF) * qs[i][j]) * xs[t] + bias[t]);
+      }
+    wave_sync();
+    if (b < first) {
+      stage();
+    } else if (b == (again ? 0 : first) || b + 1 == lines) {
+      edge(b, parity, from, a.n);
+      stage();  // in each branch: behind them all it would wait for all writes
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        *reinterpret_cast<v4i*>(line[u] + b * 128) = *reinterpret_cast<const v4i*>(ring_piece(u * 8 + (lane >> 3), parity));
+      stage();
+    }
+    wave_sync();
+  }
+  if (!again || end == lines) edge(end, parity, from, min(end * kLine, a.n));
 }
 
 // Wider rows: tiles of 256 records x 128 queries, four waves of 128 x 64 each, 64 codes of every row a step.  A step's codes go
@@ -1493,10 +1621,10 @@ template <class T, class E>
 void scores_of_rows(const ScoresArgs& a, hipStream_t s) {
   const Ranges r = ranges_of((a.n + 31) / 32, 1, 1024);
   switch (a.pitch / 64) {
-    case 1: hipLaunchKernelGGL((scores_stream_kernel<T, 1, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
-    case 2: hipLaunchKernelGGL((scores_stream_kernel<T, 2, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
-    case 3: hipLaunchKernelGGL((scores_stream_kernel<T, 3, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
-    default: hipLaunchKernelGGL((scores_stream_kernel<T, 4, 1, E>), dim3(r.grid), dim3(256), 0, s, a, 1, r.per); break;
+    case 1: hipLaunchKernelGGL((scores_stream_kernel<T, 1, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
+    case 2: hipLaunchKernelGGL((scores_stream_kernel<T, 2, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
+    case 3: hipLaunchKernelGGL((scores_stream_kernel<T, 3, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
+    default: hipLaunchKernelGGL((scores_stream_kernel<T, 4, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
   }
 }
 
@@ -1516,25 +1644,45 @@ hipError_t launch_scores_of_rows(int elem, int out_elem, const ScoresArgs& a, hi
   return hipErrorInvalidValue;
 }
 
+template <class T, int KC>
+void scores_in_lines_of(const ScoresArgs& a, hipStream_t s) {
+  constexpr int QT = 4;
+  constexpr uint32_t kLine = 128 / sizeof(T);
+  const uint32_t qb = (a.nq + QT * 16 - 1) / (QT * 16);
+  const Ranges r = ranges_of(((a.n + kLine - 1) / kLine), qb, 512);  // of per_wave * 4 lines
+  hipLaunchKernelGGL((scores_lines_kernel<T, KC, QT>), dim3(r.grid), dim3(256), 0, s, a, qb, (r.per + 3) / 4);
+}
+template <class T>
+void scores_in_lines(const ScoresArgs& a, hipStream_t s) {
+  if (a.pitch <= 64) return scores_in_lines_of<T, 1>(a, s);
+  if (a.pitch <= 128) return scores_in_lines_of<T, 2>(a, s);
+  if constexpr (sizeof(T) == 4) {
+    if (a.pitch <= 192) return scores_in_lines_of<T, 3>(a, s);
+    scores_in_lines_of<T, 4>(a, s);
+  }
+}
+
 hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   // Up to 32 queries: streams of any number of workgroups, the more the better where the table's bytes count (1 x 4M x 128:
-  // 107 us with 4096, 113 with 512).  More: rows of 128 codes stream in 512 workgroups (1024 x 100,000 x 96: 46 us with bf16
-  // scores, 117 with f32; in tiles 56 and 109), wider ones go in tiles (1024 x 100,000 x 200: 66 and 123 us; streamed, with
-  // 64 queries a wave, 66 and 158).
-  if (a.pitch <= (a.nq <= 32 ? kStreamPitch : 128)) {
+  // 107 us with 4096, 113 with 512).  More: lines for rows of 128 codes, and with f32 scores of 256 (1024 x 100,003 x 200: 128 us,
+  // in tiles 170); 16-bit scores of wider rows than 128 go in tiles (1024 x 100,000 x 200: 68 us, in lines 119).
+  if (a.nq <= 32 && a.pitch <= kStreamPitch) {
 #define SHINE_STREAM(KK, QQ, WANT)                                                                        \
   {                                                                                                       \
-    const uint32_t qb = (a.nq + QQ * 16 - 1) / (QQ * 16);                                                 \
-    const Ranges r = ranges_of((a.n + 31) / 32, qb, WANT);                                                \
-    hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ, void>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);   \
+    const Ranges r = ranges_of((a.n + 31) / 32, 1, WANT);                                                 \
+    hipLaunchKernelGGL((scores_stream_kernel<T, KK, QQ, void>), dim3(r.grid), dim3(256), 0, s, a, r.per);   \
   }
     SHINE_BY_ELEM(out_elem, switch (a.pitch / 64) {
-      case 1: if (a.nq <= 16) SHINE_STREAM(1, 1, 4096) else if (a.nq <= 32) SHINE_STREAM(1, 2, 2048) else SHINE_STREAM(1, 8, 512) break;
-      case 2: if (a.nq <= 16) SHINE_STREAM(2, 1, 4096) else if (a.nq <= 32) SHINE_STREAM(2, 2, 2048) else SHINE_STREAM(2, 8, 512) break;
+      case 1: if (a.nq <= 16) SHINE_STREAM(1, 1, 4096) else SHINE_STREAM(1, 2, 2048) break;
+      case 2: if (a.nq <= 16) SHINE_STREAM(2, 1, 4096) else SHINE_STREAM(2, 2, 2048) break;
       case 3: if (a.nq <= 16) SHINE_STREAM(3, 1, 4096) else SHINE_STREAM(3, 2, 2048) break;
       default: if (a.nq <= 16) SHINE_STREAM(4, 1, 4096) else SHINE_STREAM(4, 2, 2048) break;
     });
 #undef SHINE_STREAM
+    return hipGetLastError();
+  }
+  if (a.nq > 32 && a.pitch <= (out_elem == kF32 ? kStreamPitch : 128)) {
+    SHINE_BY_ELEM(out_elem, scores_in_lines<T>(a, s));
     return hipGetLastError();
   }
   const uint32_t few = static_cast<uint32_t>((a.n + 127) / 128), qb = (a.nq + kTileQueries - 1) / kTileQueries,

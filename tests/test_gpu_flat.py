@@ -642,3 +642,24 @@ def test_python_refusals():
         flat.adjust(x, seen=torch.zeros((20, 1), dtype=torch.int32, device="cuda"), repetition=torch.ones(19, device="cuda"))
     with pytest.raises(Exception, match="stride"):
         flat.topk(x[:1].expand(5, 32), 3)
+
+
+# More than 32 queries: lines of 128 bytes, whole ones and the rows' ends; runs of one line and of many.
+LINES = [(33, 1, 64), (33, 31, 64), (64, 32, 128), (65, 33, 96), (33, 63, 128), (40, 64, 64), (100, 129, 100), (70, 1000, 128),
+         (64, 4099, 30), (33, 700, 150), (50, 999, 256), (2000, 17003, 16), (1990, 17001, 200)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n,dim", LINES)
+def test_scores_in_rows_that_start_anywhere(dtype, nq, n, dim):
+    x, q = rows(n, dim, n + dim), rows(nq, dim, nq)
+    want = scores32(x, q, "l2").to(dtype)  # each step rounds as the definition does: equal bits
+    t = F().FlatTable(x.cuda(), metric="l2")
+    for before, ld in ((0, n), (1, n + 1), (2, n + 5), (7, n + 16)):
+        room = torch.full((before + nq * ld + 3,), 7.0, dtype=dtype, device="cuda")
+        out = room[before:before + nq * ld].view(nq, ld)[:, :n]
+        F().scores(t, q.cuda(), out=out)
+        got = room.cpu()
+        assert torch.equal(got[before:before + nq * ld].view(nq, ld)[:, :n], want), (before, ld)
+        assert bool((got[:before] == 7).all()) and bool((got[before + nq * ld:] == 7).all())
+        assert bool((got[before:before + nq * ld].view(nq, ld)[:, n:] == 7).all()), "written behind a row"
