@@ -419,9 +419,10 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint64
 // turn.  Rings of 16 queries are turned against one another so that the 64 lanes of a write, and of a read, meet different banks.
 //
 // A run's first line begins in the records before: long runs of f32 score them again (one turn more of 8 or more), short ones and
-// 16-bit scores, whose turns are twice as long, write the line's part.  1024 x 100,003 x 96, kernel and quantising: f32 162 -> 106 us (the part: 119),
-// bf16 78 -> 55 (scored again: 58); rows of 100,000: 114 -> 105 and 47 -> 50.  128 queries a wave: 130 and 75; 32, with four
-// waves a SIMD: 125 and 90.  What bounds it is the writing, 4.1 TB/s of 6.7 that a fill reaches.
+// 16-bit scores, whose turns are twice as long, write the line's part.  1024 x 100,003 x 96, kernel and quantising: f32 166 ->
+// 106 us (with the part 119), bf16 into four buffers by turns 97 -> 77 (into one, which the caches half hold, 77 -> 60); rows of
+// 100,000: 114 -> 105, 74 -> 69 (47 -> 55).  128 queries a wave: 130; 32, with four waves a SIMD: 125.  What bounds it is the
+// writing: 4.1 TB/s, of 6.7 that a fill reaches.
 template <class T, int KC, int QT>
 __global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per) {
   constexpr uint32_t kLine = 128 / sizeof(T), kPiece = 16 / sizeof(T);  // scores of a line and of 16 bytes
@@ -717,12 +718,14 @@ __global__ __launch_bounds__(256) void scores_few_kernel(ScoresArgs a) {
 // for each column that is met (integer additions: any order gives the same counts).  Then every column is read, changed
 // and written once, 16 bytes a lane.  Tiles start at multiples of 32 records, so a lane's columns share a word of allowed
 // bits and one of met ones.
-// A batch of loads is asked for before anything of it is written (memory accesses end in order), the first one before the
-// history is counted.
+// Two steps' loads are asked for before anything of them is written (memory accesses end in order), the first two before the
+// history is counted.  256 x 151,937 bf16 with histories of 2,048 and masks: 45 us, 3.6 TB/s, and 42 without the histories; four
+// steps' loads take the registers of every third wave (56 us), tiles of 4,096 columns read the histories twice (47; but 141
+// against 102 with histories of 16,384), of 16,384 leave fewer waves (65).
 template <class T, int TILE>
 __global__ __launch_bounds__(256) void adjust_kernel(AdjustArgs a) {
   constexpr int V = 16 / sizeof(T);
-  constexpr uint32_t kSteps = TILE / (256 * V), kTogether = kSteps < 4 ? kSteps : 4;
+  constexpr uint32_t kSteps = TILE / (256 * V), kTogether = kSteps < 2 ? kSteps : 2;
   __shared__ uint32_t count[TILE / 2], met[TILE / 32];
   const uint32_t row = blockIdx.y;
   const uint64_t c0 = static_cast<uint64_t>(blockIdx.x) * TILE;
