@@ -830,14 +830,15 @@ __device__ inline int32_t key_id(uint64_t key) {
 }
 
 // A workgroup of 256 threads holds up to kKeys keys and a floor below which nothing can be an answer.  The floor comes from
-// maxima: of 256 keys, one of each thread's share, the k-th largest is no larger than the k-th largest of all, so counting for
-// each of the 256 how many are larger (256 comparisons a thread, about 1 us) raises the floor without sorting anything: of
-// 4,096 random keys about k (1 + k / 512) pass it.
+// counting: the orders of some keys in 256 bins between their least and largest, then the bin that holds the k-th largest in
+// 256 finer ones, until few keys are in it: about 1,000 cycles a level, whatever the numbers are, where comparing each of 256
+// maxima with each took 4,000 to 6,500.
 constexpr uint32_t kKeys = 1024;
 
 struct __attribute__((aligned(16))) Held {
   uint64_t key[kKeys];
-  uint32_t top[256];
+  uint32_t bin[256];
+  uint32_t least[4], largest[4];  // of each wave
   uint32_t count;
   uint64_t floor;  // keys up to it are no answers, but for those held
 };
@@ -850,23 +851,100 @@ __device__ inline void begin(Held& h, uint64_t floor = 0) {
   __syncthreads();
 }
 
-// `order`: the high word of the largest key of the thread's share.  The low 8 bits give way to the thread's number, so
-// that all 256 differ.  Ends with a barrier.
-__device__ inline void raise_floor(Held& h, uint32_t order, uint32_t k) {
-  const uint32_t mine = (order & ~255u) | threadIdx.x;
-  h.top[threadIdx.x] = mine;
-  __syncthreads();
-  uint32_t larger = 0;
-#pragma unroll 8
-  for (uint32_t i = 0; i < 64; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(h.top)[i];
-    larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+// x of a lane before, for scans over a wave: rows of 16 lanes first, then their last lanes; 0 where there is none
+template <int CTRL, int ROWS>
+__device__ inline uint32_t before(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xF, false));
+}
+__device__ inline uint32_t scan_sum(uint32_t x) {  // of the lanes up to this one
+  x += before<0x111, 0xF>(x);
+  x += before<0x112, 0xF>(x);
+  x += before<0x114, 0xF>(x);
+  x += before<0x118, 0xF>(x);
+  x += before<0x142, 0xA>(x);
+  x += before<0x143, 0xC>(x);
+  return x;
+}
+__device__ inline uint32_t of_lane(uint32_t x, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+__device__ inline uint32_t wave_max(uint32_t x) {
+  x = max(x, before<0x111, 0xF>(x));
+  x = max(x, before<0x112, 0xF>(x));
+  x = max(x, before<0x114, 0xF>(x));
+  x = max(x, before<0x118, 0xF>(x));
+  x = max(x, before<0x142, 0xA>(x));
+  x = max(x, before<0x143, 0xC>(x));
+  return of_lane(x, 63);
+}
+
+// `order`: high words of keys that are all different ones (0: none).  Leaves up to `slack` more than k of them above the
+// floor, but for keys of one order.  Ends with a barrier.
+template <int M>
+__device__ inline void raise_floor(Held& h, const uint32_t (&order)[M], uint32_t k, uint32_t slack) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t largest = 0, inverse = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    largest = max(largest, order[i]);
+    inverse = max(inverse, order[i] ? ~order[i] : 0u);
   }
-  if (larger == k - 1) {
-    const uint64_t floor = static_cast<uint64_t>(mine & ~255u) << 32;
-    if (floor > h.floor) h.floor = floor;
+  largest = wave_max(largest);
+  inverse = wave_max(inverse);
+  if (lane == 0) {
+    h.largest[threadIdx.x >> 6] = largest;
+    h.least[threadIdx.x >> 6] = ~inverse;
   }
+  h.bin[threadIdx.x] = 0;
   __syncthreads();
+  uint32_t top = max(max(h.largest[0], h.largest[1]), max(h.largest[2], h.largest[3])),
+           base = min(min(h.least[0], h.least[1]), min(h.least[2], h.least[3])), need = k, floor = 0;
+  while (base <= top) {  // the same for all threads
+    const uint32_t range = top - base, shift = range < 256 ? 0 : 24 - __builtin_clz(range);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (order[i] >= base && order[i] <= top) atomicAdd(&h.bin[(order[i] - base) >> shift], 1u);
+    __syncthreads();
+    const uint4 c = reinterpret_cast<const uint4*>(h.bin)[63 - lane];  // lane 0: the highest four
+    const uint32_t sum = c.x + c.y + c.z + c.w, reached = scan_sum(sum);
+    const uint64_t there = __ballot(reached >= need);
+    if (!there) break;  // fewer than k
+    const int l = __builtin_ctzll(there);
+    uint32_t above = of_lane(reached - sum, l), bin = (63 - l) * 4 + 3, in = of_lane(c.w, l);
+    if (above + in < need) above += in, --bin, in = of_lane(c.z, l);
+    if (above + in < need) above += in, --bin, in = of_lane(c.y, l);
+    if (above + in < need) above += in, --bin, in = of_lane(c.x, l);
+    floor = base + (bin << shift);
+    need -= above;
+    if (shift == 0 || in <= need + slack) break;
+    base = floor;
+    top = floor + (1u << shift) - 1;
+    __syncthreads();
+    h.bin[threadIdx.x] = 0;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && static_cast<uint64_t>(floor) << 32 > h.floor) h.floor = static_cast<uint64_t>(floor) << 32;
+  __syncthreads();
+}
+__device__ inline uint32_t slack_of(uint32_t k) { return 4 + k / 8; }
+
+// Places the keys whose bits are set, a wave's with one addition to the count; returns the bits of those without room.
+template <int N, class Key>
+__device__ inline uint32_t place(Held& h, uint32_t pending, Key key) {
+  const uint32_t n = __popc(pending), upto = scan_sum(n), all = of_lane(upto, 63);
+  if (all == 0) return 0;
+  uint32_t at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(&h.count, all);
+  at = of_lane(at, 0) + upto - n;
+  uint32_t left = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (pending >> i & 1u) {
+      if (at < kKeys) h.key[at] = key(i);
+      else left |= 1u << i;
+      ++at;
+    }
+  return left;
 }
 
 // descending, over the first n (a power of two) keys
@@ -886,26 +964,27 @@ __device__ inline void sort_keys(uint64_t* key, uint32_t n) {
     }
 }
 
-// Makes room: raises the floor from what is held and drops what does not pass.  Where that leaves more than half (k near
-// 256, many equal values, all the best in one thread's share), sorts and keeps the best k.  All threads call it behind a
-// barrier; it ends with one.
-__device__ inline void make_room(Held& h, uint32_t k) {
+// Makes room: raises the floor from what is held and drops what does not pass.  Where that leaves more than half (many equal
+// values), sorts and keeps the best k.  All threads call it behind a barrier; it ends with one.
+__device__ inline void make_room(Held& h, uint32_t k, uint32_t slack) {
+  constexpr int M = kKeys / 256;
   const uint32_t held = h.count < kKeys ? h.count : kKeys;
-  uint64_t key[kKeys / 256];
-  uint64_t best = 0;
+  uint64_t key[M];
+  uint32_t order[M];
 #pragma unroll
-  for (uint32_t i = 0; i < kKeys / 256; ++i) {
+  for (uint32_t i = 0; i < M; ++i) {
     const uint32_t at = i * 256 + threadIdx.x;
     key[i] = at < held ? h.key[at] : 0;
-    best = key[i] > best ? key[i] : best;
+    order[i] = static_cast<uint32_t>(key[i] >> 32);
   }
-  raise_floor(h, static_cast<uint32_t>(best >> 32), k);
+  raise_floor(h, order, k, slack);
   if (threadIdx.x == 0) h.count = 0;
   __syncthreads();
   const uint64_t floor = h.floor;
+  uint32_t kept = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kKeys / 256; ++i)
-    if (key[i] > floor || (key[i] && key[i] == floor)) h.key[atomicAdd(&h.count, 1u)] = key[i];
+  for (uint32_t i = 0; i < M; ++i) kept |= (key[i] && key[i] >= floor ? 1u : 0u) << i;
+  place<M>(h, kept, [&](int i) { return key[i]; });
   __syncthreads();
   const uint32_t left = h.count;
   if (left <= kKeys / 2) return;
@@ -921,7 +1000,7 @@ __device__ inline void make_room(Held& h, uint32_t k) {
 
 // The answers: the best k of what is held, in order.  Ends with a barrier.
 __device__ inline void finish(Held& h, uint32_t k) {
-  if (h.count > 256) make_room(h, k);
+  if (h.count > 256) make_room(h, k, min(256 - k, slack_of(k)));
   const uint32_t held = h.count;
   if (held <= 256) {  // each key's place is the number of larger ones
     const uint64_t mine = threadIdx.x < held ? h.key[threadIdx.x] : 0;
@@ -950,32 +1029,22 @@ __device__ inline void finish(Held& h, uint32_t k) {
 template <int N>
 __device__ inline void offer(Held& h, uint32_t k, const uint64_t (&key)[N], bool first) {
   if (first) {
-    uint64_t best = 0;
+    uint32_t order[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = key[i] > best ? key[i] : best;
-    raise_floor(h, static_cast<uint32_t>(best >> 32), k);
+    for (int i = 0; i < N; ++i) order[i] = static_cast<uint32_t>(key[i] >> 32);
+    raise_floor(h, order, k, slack_of(k));
   }
-  uint32_t pending = 0;
   uint64_t floor = h.floor;
+  uint32_t pending = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) pending |= (key[i] > floor ? 1u : 0u) << i;
   for (;;) {
-    if (pending) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (pending >> i & 1u) {
-          bool settled = key[i] <= floor;
-          if (!settled) {
-            const uint32_t at = atomicAdd(&h.count, 1u);
-            settled = at < kKeys;
-            if (settled) h.key[at] = key[i];
-          }
-          if (settled) pending &= ~(1u << i);
-        }
-    }
+    pending = place<N>(h, pending, [&](int i) { return key[i]; });
     if (!__syncthreads_or(pending != 0)) return;
-    make_room(h, k);
+    make_room(h, k, slack_of(k));
     floor = h.floor;
+#pragma unroll
+    for (int i = 0; i < N; ++i) pending &= ~((key[i] > floor ? 0u : 1u) << i);
   }
 }
 
@@ -1030,36 +1099,27 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
       top[i] = fmaxf(fmaxf(v[i * 4], v[i * 4 + 1]), fmaxf(v[i * 4 + 2], v[i * 4 + 3]));
     best = fmaxf(best, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
     if (--until == 0) {
-      raise_floor(h, best >= kLowest ? static_cast<uint32_t>(key_of(best, 0) >> 32) : 0, a.k);
+      const uint32_t order[1] = {best >= kLowest ? static_cast<uint32_t>(key_of(best, 0) >> 32) : 0};
+      raise_floor(h, order, a.k, slack_of(a.k));
       until = turns * 3;
       turns *= 4;
     }
     uint64_t floor = h.floor;
-    float low = floor ? key_value(floor) : kLowest;
+    const float low = floor ? key_value(floor) : kLowest;
+    auto key = [&](int i) {
+      return key_of(v[i], static_cast<uint32_t>(a.first + c + (i / V) * V * 256 + threadIdx.x * V + i % V));
+    };
     uint32_t pending = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) pending |= (v[i] >= low ? 1u : 0u) << i;
     for (;;) {  // as offer() does
-      if (pending) {
+      if (static_cast<uint32_t>(floor) && pending)  // a floor of its id too
 #pragma unroll
-        for (int g = 0; g < N; g += 4)
-          if (pending >> g & 15u) {
-#pragma unroll
-            for (int i = g; i < g + 4; ++i)
-              if (pending >> i & 1u) {
-                const uint64_t key = key_of(v[i], static_cast<uint32_t>(a.first + c + (i / V) * V * 256 + threadIdx.x * V + i % V));
-                bool settled = key <= floor;
-                if (!settled) {
-                  const uint32_t at = atomicAdd(&h.count, 1u);
-                  settled = at < kKeys;
-                  if (settled) h.key[at] = key;
-                }
-                if (settled) pending &= ~(1u << i);
-              }
-          }
-      }
+        for (int i = 0; i < N; ++i)
+          if (pending >> i & 1u && key(i) <= floor) pending &= ~(1u << i);
+      pending = place<N>(h, pending, key);
       if (!__syncthreads_or(pending != 0)) break;
-      make_room(h, a.k);
+      make_room(h, a.k, slack_of(a.k));
       floor = h.floor;
     }
   }
@@ -1090,7 +1150,7 @@ __device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* src, uint
 #pragma unroll
     for (int i = 0; i < N; ++i) key[i] = next[i];
     if (c + 256 * N < count) fetch(c + 256 * N);
-    offer(h, k, key, c == 0);
+    offer(h, k, key, c == 0 && count > k + 64);  // fewer are put in order as fast
   }
 }
 
