@@ -1349,6 +1349,13 @@ __global__ __launch_bounds__(256, 2) void sample_kernel(PassArgs a, uint32_t que
   }
 }
 
+// Where a record's 16-byte piece lies in a tile of 32 records in LDS, so that the 8 lanes that one LDS cycle serves meet
+// different banks both where they hold neighbouring pieces and where they hold one piece of neighbouring records.
+template <int C>
+__device__ inline uint32_t tile_piece(uint32_t record, uint32_t piece) {
+  return record * (C * 2) + (piece ^ (C % 4 ? record >> 1 & 3 : record & 7));
+}
+
 // The other passes: the keys of what reaches the threshold.  A wave lists them in LDS and hands its list on when it runs full,
 // with one addition to each query's count: additions to one address from all over the GPU are served one after another.
 // What a score needs beside its sum is in registers, a record's in lane r % 32: a load from memory would wait for the next
@@ -1357,10 +1364,13 @@ template <int KC, int QT, bool ROWS>
 __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
   constexpr uint32_t kQueries = QT * 32, kList = 512, kFull = kList - 64;  // a turn of the listing adds at most 64 keys
   constexpr int C = KC * 2;
-  struct Own {  // each wave's
-    uint64_t key[kList];
+  constexpr bool kTurned = KC > 2;  // the codes come by way of LDS
+  struct __attribute__((aligned(16))) Own {  // each wave's
+    v4i tile[kTurned ? C * 64 : 1];
+    uint2 found[kList];  // record and sum, then the key
     uint32_t query[kList];
-    uint32_t found[kQueries], base[kQueries];
+    uint32_t count[kQueries], base[kQueries];
+    float scale[kQueries];
     uint32_t allow[ROWS ? kQueries : 1];
   };
   __shared__ Own owns[4];
@@ -1374,35 +1384,34 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
   load_tile_queries<C, QT>(q, a, query0);
   v4s qterms[QT];
   int limit[QT];
-  float qs[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const uint32_t query = query0 + i * 32 + col, r = min(query, a.nq - 1);
     qterms[i] = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.query_terms)[r].t[half * 4]);
     limit[i] = query < a.nq ? a.limit[r] : 0x7FFFFFFF;
-    qs[i] = a.qscales[r];
+    if (half == 0) own.scale[i * 32 + col] = a.qscales[r];
   }
-  for (uint32_t i = lane; i < kQueries; i += 64) own.found[i] = 0;
+  for (uint32_t i = lane; i < kQueries; i += 64) own.count[i] = 0;
   constexpr int MASKS = (kQueries + 63) / 64;  // queries whose mask words a lane fetches
   const uint32_t* allow_row[MASKS];
 #pragma unroll
   for (int i = 0; i < MASKS; ++i) allow_row[i] = a.allow + (ROWS ? min(query0 + i * 64 + lane, a.nq - 1) * a.allow_ld : 0);
-  const float* tbias = a.tbias ? a.tbias : a.scales;
-  const float* abias = a.abias ? a.abias : a.scales;
   const uint32_t* shared_allow = a.allow ? a.allow : reinterpret_cast<const uint32_t*>(a.scales);
   const bool shared = !ROWS && a.allow;
   v4i next[C];
   v4s next_terms;
-  float next_xs, next_tb, next_ab;
   uint32_t next_allow[MASKS];
   auto fetch = [&](uint64_t b) {
     const uint64_t word = min(b, last) * a.stride;
-    load_tile_block<C>(next, a, word);
+    if (kTurned) {
+      const uint32_t end = records_of(a, word) * (C * 32) - 16;  // behind the last record: anything
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c)
+        next[c] = *reinterpret_cast<const v4i*>(a.codes + word * (32 * C * 32) + min(c * 1024 + lane * 16, end));
+    } else {
+      load_tile_block<C>(next, a, word);
+    }
     next_terms = *reinterpret_cast<const v4s*>(&static_cast<const Terms*>(a.record_terms)[word * 32 + col].t[half * 4]);
-    const uint32_t mine = min(col, records_of(a, word) - 1);
-    next_xs = (a.scales + word * 32)[mine];
-    next_tb = (tbias + word * 32)[mine];
-    next_ab = (abias + word * 32)[mine];
 #pragma unroll
     for (int i = 0; i < MASKS; ++i) next_allow[i] = ROWS ? allow_row[i][word] : i ? 0 : shared_allow[shared ? word : 0];
   };
@@ -1411,35 +1420,58 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
     wave_sync();
     uint32_t place[kList / 64];
 #pragma unroll
-    for (uint32_t i = 0; i < kList / 64; ++i)
-      if (i * 64 + lane < listed) place[i] = atomicAdd(&own.found[own.query[i * 64 + lane]], 1u);
+    for (uint32_t i = 0; i < kList / 64; ++i) {
+      place[i] = ~0u;
+      if (i * 64 + lane < listed) {
+        const uint2 e = own.found[i * 64 + lane];
+        const uint32_t mine = own.query[i * 64 + lane];
+        const uint64_t key = offered_key(exact_score(__uint_as_float(e.y) - kSumZero, own.scale[mine], a, e.x), e.x);
+        own.found[i * 64 + lane] = make_uint2(static_cast<uint32_t>(key), static_cast<uint32_t>(key >> 32));
+        if (key) place[i] = atomicAdd(&own.count[mine], 1u);
+      }
+    }
     wave_sync();
     for (uint32_t i = lane; i < kQueries; i += 64) {
-      if (own.found[i]) own.base[i] = atomicAdd(&a.count[(query0 + i) * kCountStride], own.found[i]);
-      own.found[i] = 0;
+      if (own.count[i]) own.base[i] = atomicAdd(&a.count[(query0 + i) * kCountStride], own.count[i]);
+      own.count[i] = 0;
     }
     wave_sync();
 #pragma unroll
     for (uint32_t i = 0; i < kList / 64; ++i)
-      if (i * 64 + lane < listed) {
+      if (place[i] != ~0u) {
         const uint32_t mine = own.query[i * 64 + lane];
         const uint64_t to = static_cast<uint64_t>(own.base[mine]) + place[i];
-        if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = own.key[i * 64 + lane];
+        const uint2 key = own.found[i * 64 + lane];
+        if (to < a.cap) a.keys[(query0 + mine) * a.cap + to] = static_cast<uint64_t>(key.y) << 32 | key.x;
       }
     wave_sync();
     listed = 0;
   };
   const v16i start = sums_start();
+  uint32_t to[C], from[C];
+#pragma unroll
+  for (uint32_t c = 0; c < C; ++c) {
+    to[c] = tile_piece<C>((c * 64 + lane) / (C * 2), (c * 64 + lane) % (C * 2));
+    from[c] = tile_piece<C>(col, c * 2 + half);
+  }
   fetch(b0 + wave);
   for (uint64_t b = b0 + wave; b < b1; b += 4) {
     v4i x[C];
+    if (kTurned) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) x[c] = next[c];
+      for (int c = 0; c < C; ++c) own.tile[to[c]] = next[c];
+      wave_sync();
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = own.tile[from[c]];
+      wave_sync();
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = next[c];
+    }
     const v4s terms = next_terms;
     const uint64_t word = b * a.stride;
     const uint32_t there = records_of(a, word);
     const uint32_t live = (there == 32 ? ~0u : (1u << there) - 1) & (shared ? next_allow[0] : ~0u);
-    const int xs = __float_as_int(next_xs), tb = __float_as_int(next_tb), ab = __float_as_int(next_ab);
     if (ROWS) {
       wave_sync();
 #pragma unroll
@@ -1457,7 +1489,7 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
       int most = -0x7FFFFFFF - 1;  // as integers, floats' bits keep their order but for the negative ones among themselves
 #pragma unroll
       for (int v = 0; v < 16; ++v) most = max(most, __float_as_int(margin[v]));
-      if (__any(most >= limit[i])) {  // all lanes: they hold the records' scales for one another
+      if (__any(most >= limit[i])) {
         uint32_t maybe = 0;
 #pragma unroll
         for (uint32_t v = 0; v < 16; ++v) maybe |= (__float_as_int(margin[v]) >= limit[i] ? 1u : 0u) << v;
@@ -1468,18 +1500,13 @@ __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query
           int bits = sum[0];
 #pragma unroll
           for (uint32_t e = 1; e < 16; ++e) bits = v == e ? sum[e] : bits;
-          const float score = exact_score(__int_as_float(bits) - kSumZero, qs[i],
-                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, xs)), a,
-                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, tb)),
-                                          __int_as_float(__builtin_amdgcn_ds_bpermute(r * 4, ab)));
-          const uint64_t key = maybe ? offered_key(score, word * 32 + r) : 0;
-          maybe &= maybe - 1;
-          const uint64_t who = __ballot(key != 0);
-          if (key) {
+          const uint64_t who = __ballot(maybe != 0);
+          if (maybe) {
             const uint32_t to = listed + __popcll(who & ((1ull << lane) - 1));
-            own.key[to] = key;
+            own.found[to] = make_uint2(static_cast<uint32_t>(word * 32 + r), static_cast<uint32_t>(bits));
             own.query[to] = i * 32 + col;
           }
+          maybe &= maybe - 1;
           listed += __popcll(who);
           if (listed > kFull) hand_on();
         }
