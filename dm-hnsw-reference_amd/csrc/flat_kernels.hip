@@ -1133,10 +1133,11 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a, bool to_keys) {
   }
 }
 
-// All threads call it behind a barrier.
-__device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* src, uint64_t count) {
+// All threads call it behind a barrier.  `key`: of an entry (0: none) and its place in the list.
+template <class Entry, class Key>
+__device__ inline void offer_list(Held& h, uint32_t k, const Entry* src, uint64_t count, Key key_of_entry) {
   constexpr int N = 8;
-  uint64_t next[N];
+  Entry next[N];
   auto fetch = [&](uint64_t c) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -1148,10 +1149,13 @@ __device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* src, uint
   for (uint64_t c = 0; c < count; c += 256 * N) {
     uint64_t key[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) key[i] = next[i];
+    for (int i = 0; i < N; ++i) key[i] = next[i] ? key_of_entry(next[i], c + i * 256 + threadIdx.x) : 0;
     if (c + 256 * N < count) fetch(c + 256 * N);
     offer(h, k, key, c == 0 && count > k + 64);  // fewer are put in order as fast
   }
+}
+__device__ inline void offer_list(Held& h, uint32_t k, const uint64_t* keys, uint64_t count) {
+  offer_list(h, k, keys, count, [](uint64_t key, uint64_t) { return key; });
 }
 
 template <class T>
@@ -1168,7 +1172,7 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
 // ---------------------------------------------------------------------------------------------- search
 // The best k of all records without the score matrix.  A pass scores every stride-th block of 32 records and lists, for
 // each query, the keys from its threshold on; the k-th best key of a coarser pass (a lower bound of the k-th best of all
-// records) is the next pass's threshold, the coarsest pass stores all its keys, and the last pass is over all records.
+// records) is the next pass's threshold, the coarsest pass stores all its scores, and the last pass is over all records.
 // A list whose room ends loses nothing but time: its row is scanned again, alone, where the answers are selected.
 
 // The score as shine_flat_scores and then shine_flat_adjust round it; tb and ab count where the biases are given.
@@ -1293,7 +1297,8 @@ __device__ inline v16i tile_sums(const v4i (&x)[C], const v4i (&q)[C], const v16
   return sum;
 }
 
-// The coarsest pass: a few thousand records of every query, all of whose keys are stored.
+// The coarsest pass: a few thousand records of every query; the orders of all their scores are stored, the high words of keys
+// whose low ones their places tell.
 template <int KC, int QT>
 __global__ __launch_bounds__(256, 2) void sample_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
   constexpr int C = KC * 2;
@@ -1329,19 +1334,19 @@ __global__ __launch_bounds__(256, 2) void sample_kernel(PassArgs a, uint32_t que
       const uint32_t query = query0 + i * 32 + col;
       const v16i sum = tile_sums<C>(x, q[i], start);
       if (query < a.nq) {
-        ulonglong2* to = reinterpret_cast<ulonglong2*>(a.keys + query * a.cap + b * 32 + half * 4);
+        uint32_t* to = reinterpret_cast<uint32_t*>(a.keys + query * a.cap) + b * 32 + half * 4;
         const uint32_t on = there & allow[i];
 #pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-          uint64_t key[2];
+        for (int v = 0; v < 16; v += 4) {
+          uint32_t order[4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t r = (v >> 2) * 8 + half * 4 + (v & 3) + e;
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t r = v * 2 + half * 4 + e;
             const float score = exact_score(__int_as_float(sum[v + e]) - kSumZero, qs[i], beside[wave][0][r], a,
                                             beside[wave][1][r], beside[wave][2][r]);
-            key[e] = on >> r & 1u ? offered_key(score, word * 32 + r) : 0;
+            order[e] = on >> r & 1u ? static_cast<uint32_t>(offered_key(score, 0) >> 32) : 0;
           }
-          to[(v >> 2) * 4 + (v & 3) / 2] = make_ulonglong2(key[0], key[1]);
+          *reinterpret_cast<uint4*>(to + v * 2) = make_uint4(order[0], order[1], order[2], order[3]);
         }
       }
     }
@@ -1356,10 +1361,18 @@ __device__ inline uint32_t tile_piece(uint32_t record, uint32_t piece) {
   return record * (C * 2) + (piece ^ (C % 4 ? record >> 1 & 3 : record & 7));
 }
 
-// The other passes: the keys of what reaches the threshold.  A wave lists them in LDS and hands its list on when it runs full,
-// with one addition to each query's count: additions to one address from all over the GPU are served one after another.
-// What a score needs beside its sum is in registers, a record's in lane r % 32: a load from memory would wait for the next
-// block's codes, which are on their way.
+// The other passes: the keys of what reaches the threshold.  A wave lists records and sums in LDS and hands its list on when it
+// runs full: only then they are scored (a load of a scale among the tiles would wait for the next block's codes, which are on
+// their way) and each query's count is added to once, for additions to one address from all over the GPU are served one after
+// another.
+//
+// Rows of more than 128 codes come by way of LDS: loads of 32 bytes of 32 rows, as the products want them, keep the cache busy
+// for about 70 cycles each, four times as long as loads of 1,024 neighbouring bytes (256 x 800k x 200: 109 us a pass, by way of
+// LDS 70; without any loads 45).  128 codes: 1024 x 1M x 128, 174 us so and 180 by way of LDS.
+//
+// 1024 x 1M x 128, last pass: 171 us, 1.6 POP/s of integer products of the 2.1 that a large library product reaches; nothing
+// listed 154, and without loads and lists 117.  256 x 200k x 200 with masks, k = 100: 43 us, of which listing 2,900 records a
+// query takes 20.
 template <int KC, int QT, bool ROWS>
 __global__ __launch_bounds__(256, 2) void pass_kernel(PassArgs a, uint32_t query_blocks, uint64_t per_range) {
   constexpr uint32_t kQueries = QT * 32, kList = 512, kFull = kList - 64;  // a turn of the listing adds at most 64 keys
@@ -1549,7 +1562,12 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
   begin(h);
   const float qs = p.qscales[row];
   const uint64_t listed = a.sample ? p.blocks * 32 : p.count[row * kCountStride];
-  offer_list(h, a.k, p.keys + row * p.cap, listed < p.cap ? listed : p.cap);
+  if (a.sample)
+    offer_list(h, a.k, reinterpret_cast<const uint32_t*>(p.keys + row * p.cap), listed, [&](uint32_t order, uint64_t at) {
+      return static_cast<uint64_t>(order) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>((at >> 5) * p.stride * 32 + (at & 31)));
+    });
+  else
+    offer_list(h, a.k, p.keys + row * p.cap, listed < p.cap ? listed : p.cap);
   if (a.extra) offer_list(h, a.k, a.extra + row * a.extra_ld, a.extra_count[row]);
   finish(h, a.k);  // every thread has read the row's count: there is a barrier in between
   if (!a.last) {
