@@ -1207,7 +1207,7 @@ __device__ inline uint64_t offered_key(float v, uint64_t record) {
 //   w hi          y hi      w = 1 / x, y = -l / q
 //   w hi          y lo
 //   w lo          y hi
-//   2^-13 |u|     v hi
+//   2^-13 s / x   v hi     s: the sum of the biases' magnitudes, by which their additions round even where they cancel
 //   2^-13 w       |y hi|
 // The margin still has kMagic in it: the score fails where it is below kMagic, for floats of which some are positive and for
 // their bits as integers alike.
@@ -1226,13 +1226,13 @@ struct __attribute__((aligned(16))) Terms {
 // A record for which the margin says nothing always passes (scales and biases whose quotients may overflow), one that is no
 // answer never does: its terms are u = +-1e20 alone.  The reciprocals are within 2^-22.
 constexpr float kNear = 1e9f, kSure = 1e20f;
-__device__ inline Terms record_terms(float x, float b, bool on) {
+__device__ inline Terms record_terms(float x, float b, float size, bool on) {
   x = x == 0.0f ? 1.0f : x;  // its codes and so its sums are 0, whatever they are scaled by
-  const bool plain = on && x > 1.0f / kNear && x < kNear && fabsf(b) < kNear;
+  const bool plain = on && x > 1.0f / kNear && x < kNear && size < kNear;
   const bool none = !on || x != x || !(b > -__builtin_huge_valf());
   const float w = plain ? __builtin_amdgcn_rcpf(x) : 0.0f, u = plain ? b * w : none ? -kSure : kSure;
   const Two a(u), c(w);
-  return {{a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(plain ? 0x1p-13f * fabsf(u) : 0.0f), static_cast<__bf16>(0x1p-13f * w)}};
+  return {{a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(plain ? 0x1p-13f * (size * w) : 0.0f), static_cast<__bf16>(0x1p-13f * w)}};
 }
 // Queries for which the margin says nothing (no threshold yet, scales or thresholds whose quotients may overflow) have no
 // terms, and a limit that every margin reaches; those that are not there or have no scale one that none does.
@@ -1251,8 +1251,8 @@ __device__ inline void write_record_terms(const PassArgs& a, uint64_t block) {  
   if (r >= (a.n + 31) / 32 * 32) return;
   const uint64_t at = min(r, a.n - 1);
   const bool on = r < a.n && (!a.allow || a.allow_ld || (a.allow[r >> 5] >> (r & 31) & 1u));
-  static_cast<Terms*>(a.record_terms)[r] =
-      record_terms(a.scales[at], (a.tbias ? a.tbias[at] : 0.0f) + (a.abias ? a.abias[at] : 0.0f), on);
+  const float tb = a.tbias ? a.tbias[at] : 0.0f, ab = a.abias ? a.abias[at] : 0.0f;
+  static_cast<Terms*>(a.record_terms)[r] = record_terms(a.scales[at], tb + ab, fabsf(tb) + fabsf(ab), on);
 }
 
 // Both passes: a wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32

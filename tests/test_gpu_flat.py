@@ -663,3 +663,135 @@ def test_scores_in_rows_that_start_anywhere(dtype, nq, n, dim):
         assert torch.equal(got[before:before + nq * ld].view(nq, ld)[:, :n], want), (before, ld)
         assert bool((got[:before] == 7).all()) and bool((got[before + nq * ld:] == 7).all())
         assert bool((got[before:before + nq * ld].view(nq, ld)[:, n:] == 7).all()), "written behind a row"
+
+
+# Searches of several passes, bit for bit as step by step: every width of rows, masks of each kind, parts of a block.
+@pytest.mark.parametrize("dim", [40, 128, 150, 256])
+@pytest.mark.parametrize("nq,n,k,h,bias,allow", [
+    (20, 9001, 1, 0, None, "rows"), (40, 20017, 100, 30, "shared", "rows"), (130, 70003, 10, 300, None, "shared"),
+    (300, 33000, 256, 5, "shared", "rows"), (65, 300001, 17, 0, None, None), (33, 8200, 3, 4096, None, None),
+    (17, 12345, 40, 4097, None, "shared")])
+def test_search_of_several_passes_with_adjustments(dim, nq, n, k, h, bias, allow):
+    flat = F()
+    table = flat.FlatTable(rows(n, dim, n + 1).cuda(), metric="l2")
+    q = rows(nq, dim, nq + 2).cuda()
+    a = cuda(adjustments(nq, n, 4, h, bias, allow))
+    values, ids = flat.search(table, q, k, **a)
+    s = flat.scores(table, q)
+    v, i = flat.topk(flat.adjust(s, **a) if a else s, k)
+    assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+@pytest.mark.parametrize("dim", [64, 200])
+def test_search_of_several_passes_with_little_left(dim):
+    flat = F()
+    n, k = 40011, 8
+    table = flat.FlatTable(rows(n, dim, 1).cuda())
+    left = [[], [40010], [0, 31, 32, 20000, 40000, 40009, 40010], list(range(17, n, 1500)), list(range(39000, n))]
+    allow = torch.zeros((20, (n + 31) // 32), dtype=torch.int64)
+    for i in range(20):
+        for j in left[i % 5]:
+            allow[i, j // 32] |= 1 << (j % 32)
+    allow = torch.where(allow >= 2 ** 31, allow - 2 ** 32, allow).int().cuda()
+    q = rows(20, dim, 2).cuda()
+    values, ids = flat.search(table, q, k, allow=allow)
+    v, i = flat.topk(flat.adjust(flat.scores(table, q), allow=allow), k)
+    assert torch.equal(ids, i) and torch.equal(values, v)
+    assert all(set(ids[r].tolist()) <= set(left[r % 5]) | {-1} for r in range(20))
+    assert all(int((ids[r] >= 0).sum()) == min(k, len(left[r % 5])) for r in range(20))
+
+
+def test_more_rows_than_a_launch_takes():
+    flat = F()
+    nq, n = 33001, 37
+    x, q = rows(n, 48, 1).cuda(), rows(nq, 48, 2).cuda()
+    table = flat.FlatTable(x, metric="l2")
+    s = flat.scores(table, q)
+    bias = rows(1, n, 3).cuda()
+    seen = torch.randint(-1, n, (nq, 3), dtype=torch.int32, generator=torch.Generator().manual_seed(4)).cuda()
+    rep = torch.linspace(1, 2, nq).cuda()
+    t = flat.adjust(s, bias=bias, seen=seen, repetition=rep)
+    v, i = flat.topk(t, 4)
+    found = flat.search(table, q, 4, bias=bias, seen=seen, repetition=rep)
+    assert torch.equal(found[0], v) and torch.equal(found[1], i)
+    for part in (slice(0, 70), slice(32700, 32800), slice(32960, nq)):
+        sp = flat.scores(table, q[part])
+        assert torch.equal(sp, s[part])
+        tp = flat.adjust(sp, bias=bias, seen=seen[part], repetition=rep[part].contiguous())
+        assert torch.equal(tp, t[part])
+        assert torch.equal(flat.topk(tp, 4)[1], i[part])
+    want = topk_plain(scores32(x.cpu(), q[-50:].cpu(), "l2"), 4)
+    assert torch.equal(flat.topk(s[-50:], 4)[1].cpu(), want[1])
+
+
+def test_offsets_beyond_32_bits():
+    """2.4e9 scores of 16 bits, codes of 3.8e9 bytes: the ends of the table and of the matrix against a table of the ends"""
+    flat = F()
+    if torch.cuda.get_device_properties(0).total_memory < 64 << 30:
+        pytest.skip("needs 64 GB")
+    n, nq, end = 60_000_001, 40, 1000
+    x = torch.randn((n, 16), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    q = rows(nq, 16, 2).cuda()
+    table, tail = flat.FlatTable(x, metric="l2"), flat.FlatTable(x[-end:], metric="l2")
+    del x
+    s = flat.scores(table, q, dtype=torch.float16)
+    want = flat.scores(tail, q, dtype=torch.float16)
+    assert torch.equal(s[:, -end:], want)
+    s.clamp_(max=0)
+    s[-1, -1], s[-1, 0], s[0, n // 2] = 5, 4, 3
+    values, ids = flat.topk(s, 2)
+    assert values[-1].tolist() == [5, 4] and ids[-1].tolist() == [n - 1, 0] and ids[0, 0] == n // 2
+    bits = torch.full(((n + 31) // 32,), -1, dtype=torch.int32, device="cuda")
+    bits[-1] = 0  # the last record is alone in its word
+    flat.adjust(s, allow=bits, out=s)
+    assert s[:, -1].eq(NEG).all() and flat.topk(s, 1)[1][-1] == 0
+    del s
+    f = flat.scores(table, q[-17:])  # (17, n) of 32 bits: 4.1e9 bytes
+    found = flat.search(table, q[-17:], 5)
+    want = flat.topk(f, 5)
+    assert torch.equal(found[0], want[0]) and torch.equal(found[1], want[1])
+
+
+@pytest.mark.parametrize("dim", [64, 200])
+def test_search_with_biases_that_cancel_the_norms(dim):
+    """((sum * q) * x - norm) + norm: what the additions round off decides between records"""
+    flat = F()
+    n = 30011
+    table = flat.FlatTable(rows(n, dim, 1, scale=300.0).cuda(), metric="l2")
+    q = rows(40, dim, 2, scale=1e-3).cuda()
+    for bias in (-table.bias, -table.bias + 64.0, -table.bias * 1.0001):
+        values, ids = flat.search(table, q, 20, bias=bias)
+        v, i = flat.topk(flat.adjust(flat.scores(table, q), bias=bias), 20)
+        assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+@pytest.mark.parametrize("dim", [64, 200])
+def test_search_with_biases_that_are_no_numbers(dim):
+    flat = F()
+    n = 30011
+    table = flat.FlatTable(rows(n, dim, 1).cuda(), metric="l2")
+    q = rows(40, dim, 2).cuda()
+    bias = rows(1, n, 3)[0]
+    bias[::7], bias[1::5000], bias[2::11], bias[3::9000] = NEG, math.inf, math.nan, 3e38
+    bias[4::13] = -3.4028234663852886e38
+    for b in (bias, torch.where(bias.isinf() & (bias > 0), torch.tensor(0.0), bias)):
+        values, ids = flat.search(table, q, 30, bias=b.cuda())
+        v, i = flat.topk(flat.adjust(flat.scores(table, q), bias=b.cuda()), 30)
+        assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+@pytest.mark.parametrize("dim", [64, 200])
+def test_search_of_equal_products_whose_biases_cancel(dim):
+    """the product is the same for all records: the roundings of the additions alone tell them apart"""
+    flat = F()
+    n, half = 30011, dim // 2
+    g = torch.Generator().manual_seed(1)
+    x = torch.ones(n, dim)
+    x[:, half:] = torch.randint(-127, 128, (n, dim - half), generator=g).float()
+    x[:, -1] = 127  # scale 50: codes are these numbers
+    table = flat.FlatTable((50 * x).cuda(), metric="l2")
+    q = torch.zeros(40, dim)
+    q[:, :half] = 127 * torch.linspace(0.001, 0.01, 40)[:, None]
+    values, ids = flat.search(table, q.cuda(), 20, bias=-table.bias)
+    v, i = flat.topk(flat.adjust(flat.scores(table, q.cuda()), bias=-table.bias), 20)
+    assert torch.equal(ids, i) and torch.equal(values, v)
