@@ -118,12 +118,17 @@ struct SearchPlan {
   uint64_t codes, scales, scores, keys, terms, query_terms, limit, count, mask, extra, extra_count, total;  // offsets into the workspace
 };
 
-// Fused passes cost less than the score matrix once it is larger than the table: from 17 queries on.  A bias for each row
-// is as large as the matrix itself, and wide rows' queries do not fit the registers: these are searched stepwise.
+// Fused passes cost less than the score matrix once it is larger than about 24M scores: with 128 codes and k = 10,
+// 1024 x 20,000 take 51 us a call (stepwise 48), 256 x 131,072 take 47 (63), 2048 x 20,000 take 69 (79), 1024 x 65,536 take 62
+// (133); with few queries the table is read more often than the matrix would be (16 x 1M: 58 and 58, 8 x 1M: 57 and 48).  A
+// bias for each row is as large as the matrix itself, and wide rows' queries do not fit the registers: these are searched
+// stepwise.
+constexpr uint64_t kFusedScores = 24u << 20;
 SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const shine_flat_adjustment* a) {
   SearchPlan p{};
   const uint32_t pitch = F::code_pitch(dim), seen_n = a ? a->seen_n : 0;
-  p.fused = nq > 16 && n > 0 && pitch <= F::kMaxFusedPitch && seen_n <= F::kMaxSeen && !(a && a->bias && a->bias_ld);
+  p.fused = nq > 16 && nq * n > kFusedScores && pitch <= F::kMaxFusedPitch && seen_n <= F::kMaxSeen &&
+            !(a && a->bias && a->bias_ld);
   p.rows = std::min(std::max(nq, 1u), 2048u);
   uint64_t at = 0;
   auto take = [&at](uint64_t bytes) {
@@ -132,7 +137,9 @@ SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const 
     return here;
   };
   if (p.fused) {
-    const uint64_t blocks = (n + 31) / 32, coarse = k > 64 ? 256 : 128;  // blocks of the coarsest pass
+    // Blocks of the coarsest pass: 256 where a short list of 128 would take a pass more (256 x 200k x 200, k = 10: 56 us, with
+    // 128 66) and for long answers (1024 x 2M x 64, k = 100: 505 us, 547), else 128 (1024 x 1M x 128, k = 10: 219 us, 226).
+    const uint64_t blocks = (n + 31) / 32, coarse = k > 64 || (blocks > 128 * 32 && blocks <= 256 * 32) ? 256 : 128;
     uint64_t ratio = 1;
     if (blocks <= 256) {
       p.passes = 1;
@@ -269,7 +276,7 @@ int shine_flat_quantize(int gpu_id, const void* d_rows, int elem, uint64_t n, ui
 }
 
 uint64_t shine_flat_scores_workspace(uint32_t nq, uint64_t n, uint32_t dim) {
-  if (F::scores_from_rows(nq, F::code_pitch(dim), n)) return 0;
+  if (F::scores_from_rows(nq, F::code_pitch(dim))) return 0;
   const uint64_t rows = std::min(nq, kRowBlock);
   return aligned(rows * F::code_pitch(dim)) + aligned(4 * rows);
 }
@@ -409,10 +416,12 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
   char* ws = static_cast<char*>(d_workspace);
   for (uint32_t q = 0; q < nq; q += p.rows) {
     const uint32_t m = std::min(p.rows, nq - q);
-    if (hipError_t e = quantize(static_cast<const char*>(d_queries) + q * ld * elem_size(elem), elem, m, table->dim, ld,
-                                reinterpret_cast<int8_t*>(ws + p.codes), reinterpret_cast<float*>(ws + p.scales), nullptr, s);
-        e != hipSuccess)
-      return hip("flat search", e);
+    const char* rows = static_cast<const char*>(d_queries) + q * ld * elem_size(elem);
+    const bool from_rows = !p.fused && F::scores_from_rows(m, pitch);
+    if (!from_rows)
+      if (hipError_t e = quantize(rows, elem, m, table->dim, ld, reinterpret_cast<int8_t*>(ws + p.codes),
+                                  reinterpret_cast<float*>(ws + p.scales), nullptr, s); e != hipSuccess)
+        return hip("flat search", e);
     if (p.fused) {
       if (hipError_t e = search_fused(p, *table, adjustment, q, m, k, ws, d_values + static_cast<uint64_t>(q) * k,
                                       d_ids + static_cast<uint64_t>(q) * k, s); e != hipSuccess)
@@ -432,7 +441,12 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
       a.n = cols;
       a.out = ws + p.scores;
       a.ld = p.cols;
-      if (hipError_t e = F::launch_scores(F::kF32, a, s); e != hipSuccess) return hip("flat search", e);
+      a.queries = rows;
+      a.queries_ld = ld;
+      a.dim = table->dim;
+      if (hipError_t e = from_rows ? F::launch_scores_of_rows(elem, F::kF32, a, s) : F::launch_scores(F::kF32, a, s);
+          e != hipSuccess)
+        return hip("flat search", e);
       if (!neutral(adjustment)) {
         F::AdjustArgs b = adjust_args(*adjustment, q);
         b.scores = b.out = a.out;

@@ -656,26 +656,22 @@ __global__ __launch_bounds__(256, 2) void scores_wide_kernel(ScoresArgs a, uint3
 }
 
 // Wide rows, few queries: every wave 32 records, the queries' codes from the caches.
-template <class T, int QT>
+template <class T>
 __global__ __launch_bounds__(256) void scores_few_kernel(ScoresArgs a) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
   const uint64_t record0 = (static_cast<uint64_t>(blockIdx.x) * 4 + wave_number()) * 32;
   if (record0 >= a.n) return;
   const uint32_t last = static_cast<uint32_t>(min(a.n - record0, 32ul)) - 1;
   const int8_t* xbase = a.codes + record0 * a.pitch;
-  uint32_t xat[2], qat[QT];
+  uint32_t xat[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) xat[t] = min(Order<T>::kPaired ? (col >> 2) * 8 + t * 4 + (col & 3) : t * 16 + col, last) * a.pitch + group * 16;
-#pragma unroll
-  for (int i = 0; i < QT; ++i) qat[i] = min(i * 16 + col, a.nq - 1) * a.pitch + group * 16;
-  v4i acc[QT][2] = {};
+  const uint32_t qat = min(col, a.nq - 1) * a.pitch + group * 16;
+  v4i acc[2] = {};
   auto step = [&](const v4i(&x)[2], uint32_t c) {
+    const v4i q = *reinterpret_cast<const v4i*>(a.qcodes + qat + c);
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-      const v4i q = *reinterpret_cast<const v4i*>(a.qcodes + qat[i] + c);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t], q, acc[i][t], 0, 0, 0);
-    }
+    for (int t = 0; t < 2; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t], q, acc[t], 0, 0, 0);
   };
   uint32_t c = 0;
   for (; c + 256 <= a.pitch; c += 256) {  // four steps' records are asked for together
@@ -700,17 +696,14 @@ __global__ __launch_bounds__(256) void scores_few_kernel(ScoresArgs a) {
     xs[j] = a.scales[r];
     b[j] = a.bias ? a.bias[r] : -0.0f;
   }
+  const uint32_t q = min(col, a.nq - 1);  // behind the last query: the last one once more
+  const float qs = a.qscales[q];
+  float v[8];
 #pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    const uint32_t q = min(i * 16 + col, a.nq - 1);  // behind the last query: the last one once more
-    const float qs = a.qscales[q];
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (static_cast<float>(acc[i][j >> 2][j & 3]) * qs) * xs[j] + b[j];
-    T* row = static_cast<T*>(a.out) + q * a.ld + record0;
-    if (last == 31) Order<T>::store(row, group, v);
-    else Order<T>::store(row, group, v, last + 1);
-  }
+  for (int j = 0; j < 8; ++j) v[j] = (static_cast<float>(acc[j >> 2][j & 3]) * qs) * xs[j] + b[j];
+  T* row = static_cast<T*>(a.out) + q * a.ld + record0;
+  if (last == 31) Order<T>::store(row, group, v);
+  else Order<T>::store(row, group, v, last + 1);
 }
 
 // ---------------------------------------------------------------------------------------------- adjust
@@ -1795,8 +1788,9 @@ hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
   }
   const uint32_t few = static_cast<uint32_t>((a.n + 127) / 128), qb = (a.nq + kTileQueries - 1) / kTileQueries,
                  rb = static_cast<uint32_t>((a.n + kTileRecords - 1) / kTileRecords);
-  SHINE_BY_ELEM(out_elem, if (a.nq <= 16) hipLaunchKernelGGL((scores_few_kernel<T, 1>), dim3(few), dim3(256), 0, s, a);
-                else if (a.nq <= 32) hipLaunchKernelGGL((scores_few_kernel<T, 2>), dim3(few), dim3(256), 0, s, a);
+  // Up to 16 queries: 8 x 100,000 x 768: 21.7 us, in tiles 24.0; 16 x 400,000 x 768: 77.6 and 83.0 (32 in two such tiles a wave:
+  // 30.4 us for 100,000, in tiles 25.3).
+  SHINE_BY_ELEM(out_elem, if (a.nq <= 16) hipLaunchKernelGGL(scores_few_kernel<T>, dim3(few), dim3(256), 0, s, a);
                 else hipLaunchKernelGGL(scores_wide_kernel<T>, dim3((rb + 7) / 8 * 8 * qb), dim3(256), 0, s, a, qb, rb));
   return hipGetLastError();
 }
@@ -1832,7 +1826,7 @@ hipError_t launch_sample(const PassArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
-  const bool few = a.nq <= 32;
+  const bool few = a.nq <= 32;  // 32 x 1M x 128: 59 us a call, 63 with room for 128
   switch (a.pitch / 64) {
     case 1: few ? pass_with<1, 1>(a, s) : pass_with<1, 4>(a, s); break;
     case 2: few ? pass_with<2, 1>(a, s) : pass_with<2, 4>(a, s); break;
@@ -1856,7 +1850,8 @@ hipError_t launch_seen(const SeenArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s) {
-  // wide tiles read the history less often, narrow ones spread a small call over more of the GPU
+  // Narrow tiles spread a small call over more of the GPU, wide ones read long histories less often (256 x 151,937 f32: 89 us
+  // with histories of 8,192, in narrow tiles 128; of 2,048: 61 and 58; 64 x 50,000 with 8,192: 19 and 16).
   const bool wide = a.nq * ((a.n + 8191) / 8192) >= 512;
   const uint64_t tile = wide ? 8192 : 2048;
   const dim3 grid(static_cast<uint32_t>((a.n + tile - 1) / tile), a.nq);
@@ -1865,6 +1860,7 @@ hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Rows are cut where there are too few for the GPU (1 x 1M: 15 us, in one piece 279; 1024 x 20,000: 20.5 either way).
 uint32_t topk_slices(uint32_t nq, uint64_t n) {
   const uint64_t want = (1024 + nq - 1) / nq, most = (n + 4095) / 4096;
   const uint64_t s = want < most ? want : most;

@@ -37,7 +37,7 @@ def test_pitch_and_workspaces():
     for dim, pitch in ((1, 64), (64, 64), (65, 128), (96, 128), (200, 256), (16384, 16384)):
         assert lib.shine_flat_pitch(dim) == pitch == flat.code_pitch(dim)
     assert lib.shine_flat_scores_workspace(17, 1000, 96) >= 17 * 128 + 17 * 4
-    assert lib.shine_flat_scores_workspace(7, 1 << 20, 96) >= 7 * 128 + 7 * 4
+    assert lib.shine_flat_scores_workspace(7, 1 << 20, 300) >= 7 * 320 + 7 * 4
     assert lib.shine_flat_search_workspace(7, 1000, 96, 10, None) >= 7 * 128 + 7 * 4
 
 

@@ -795,3 +795,74 @@ def test_search_of_equal_products_whose_biases_cancel(dim):
     values, ids = flat.search(table, q.cuda(), 20, bias=-table.bias)
     v, i = flat.topk(flat.adjust(flat.scores(table, q.cuda()), bias=-table.bias), 20)
     assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+# Small score matrices are searched by way of the matrix.  The scenarios above once more, with their queries repeated until the
+# matrix is too large for that and the passes over the table search it.
+class Repeating:
+    MATRIX = 26 << 20
+
+    def __init__(self, flat):
+        self.flat = flat
+
+    def __getattr__(self, name):
+        return getattr(self.flat, name)
+
+    def search(self, table, q, k, **a):
+        nq = q.shape[0]
+        times = 1 + self.MATRIX // (nq * table.n)
+
+        def again(x):
+            return x.repeat(times, *[1] * (x.dim() - 1)) if x.shape[0] == nq else x
+
+        values, ids = self.flat.search(table, again(q), k, **{name: again(x) for name, x in a.items()})
+        values, ids = values.view(times, nq, k), ids.view(times, nq, k)
+        assert torch.equal(ids, ids[:1].expand_as(ids)) and torch.equal(values, values[:1].expand_as(values))
+        return values[0], ids[0]
+
+
+@pytest.mark.parametrize("scenario,arguments", [
+    (test_search_equal_records_come_in_id_order, ()), (test_search_of_sorted_records, ()), (test_search_with_scales_far_apart, ()),
+    (test_search_with_biases_that_cancel_the_norms, (64,)), (test_search_with_biases_that_cancel_the_norms, (200,)),
+    (test_search_with_biases_that_are_no_numbers, (64,)), (test_search_with_biases_that_are_no_numbers, (200,)),
+    (test_search_of_equal_products_whose_biases_cancel, (64,)), (test_search_of_equal_products_whose_biases_cancel, (200,)),
+    (test_search_of_several_passes_with_little_left, (64,)), (test_search_of_several_passes_with_little_left, (200,))] +
+    [(test_search_of_many_records, (n,)) for n in (8193, 131072, 400001)] +
+    [(test_search_when_a_sample_misses_the_best, (n, every, k)) for n, every in ((30000, 8), (30000, 4), (270000, 9))
+     for k in (1, 10, 256)] +
+    [(test_search_of_several_passes_with_adjustments, (dim,) + c) for dim in (40, 128, 150, 256) for c in (
+        (20, 9001, 1, 0, None, "rows"), (40, 20017, 100, 30, "shared", "rows"), (130, 70003, 10, 300, None, "shared"),
+        (300, 33000, 256, 5, "shared", "rows"), (65, 300001, 17, 0, None, None), (33, 8200, 3, 4096, None, None))] +
+    [(test_search, (64, 4099, 128, 10, metric)) for metric in ("ip", "l2")])
+def test_search_scenarios_in_passes(scenario, arguments, monkeypatch):
+    flat = Repeating(F())
+    monkeypatch.setitem(globals(), "F", lambda: flat)
+    scenario(*arguments)
+
+
+def test_passes_captured_and_replayed_beside_other_streams():
+    flat = F()
+    n, nq = 30000, 2500  # two blocks of rows
+    table = flat.FlatTable(rows(n, 200, 1).cuda(), metric="l2")
+    a = cuda(adjustments(nq, n, 5, 20, "shared", "rows"))
+    q = rows(nq, 200, 20).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        flat.search(table, q, 10, **a)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = flat.search(table, q, 10, **a)
+    other = rows(nq, 200, 30).cuda()
+    want_other = flat.topk(flat.scores(table, other), 5)
+    for turn in range(4):
+        q.copy_(rows(nq, 200, 100 + turn))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = flat.search(table, other, 5)
+        torch.cuda.synchronize()
+        want = flat.topk(flat.adjust(flat.scores(table, q), **a), 10)
+        assert torch.equal(out[1], want[1]) and torch.equal(out[0], want[0])
+        assert torch.equal(beside[1], want_other[1]) and torch.equal(beside[0], want_other[0])
