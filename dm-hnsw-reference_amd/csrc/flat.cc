@@ -69,6 +69,17 @@ const char* check_adjustment(const shine_flat_adjustment* a, uint32_t nq, uint64
   return nullptr;
 }
 
+// Rows of width n that share memory without being the same rows; rows of one stride may lie between one another's.
+bool tangled(const void* a, uint64_t a_ld, const void* b, uint64_t b_ld, uint64_t nq, uint64_t n, uint64_t size) {
+  if (nq < 2) a_ld = b_ld = n;
+  if (a == b && a_ld == b_ld) return false;
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (x + ((nq - 1) * a_ld + n) * size <= y || y + ((nq - 1) * b_ld + n) * size <= x) return false;
+  if (a_ld != b_ld) return true;
+  const uint64_t apart = (y > x ? y - x : x - y) % (a_ld * size);
+  return apart < n * size || a_ld * size - apart < n * size;
+}
+
 F::AdjustArgs adjust_args(const shine_flat_adjustment& a, uint32_t row) {
   F::AdjustArgs r{};
   r.bias = a.bias ? a.bias + row * a.bias_ld : nullptr;
@@ -334,6 +345,8 @@ int shine_flat_adjust(int gpu_id, const void* d_scores, int elem, uint32_t nq, u
   if (const char* w = check_adjustment(adjustment, nq, n)) return fail(w);
   if (nq == 0 || n == 0) return SHINE_OK;
   if (const char* w = check_rows(d_out, elem, nq, n, out_ld)) return fail(w);
+  if (tangled(d_scores, ld, d_out, out_ld, nq, n, elem_size(elem)))
+    return fail("out overlaps the scores without being the same rows");
   OnDevice dev(gpu_id);
   if (dev.e != hipSuccess) return hip("flat adjust: device", dev.e);
   for (uint32_t q = 0; q < nq; q += kRowBlock) {

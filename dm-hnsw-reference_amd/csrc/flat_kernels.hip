@@ -1597,7 +1597,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a) {
 }
 
 // A search's history is taken out of the passes: seen_mask forbids its records, seen_keys scores them, penalties and all, on
-// their own (256 users x 200,000 records with 128 ids each: 12 us, bound by the latency of sorting the ids).
+// their own (256 users x 200,000 records with 256 ids each: 12 us, bound by the latency of sorting the ids).
 //
 // The row's mask without its history: one workgroup per (row, kMaskWords words).
 constexpr uint32_t kMaskWords = 4096;

@@ -41,37 +41,46 @@ def _t():
 
 
 def _rows(x, name: str, device=None):
-    """(pointer, element type, row stride) of a 2-D tensor of rows, or ValueError."""
+    """(pointer, element type, row stride, rows, width) of a 2-D tensor of rows, or ValueError."""
     torch = _t()
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+    if not isinstance(x, torch.Tensor) or len(shape := x.shape) != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
     elem = _elems.get(x.dtype)
     if elem is None:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, not {x.dtype}")
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0 or not x.is_cuda:
         raise ValueError(f"{name} must be on a GPU")
-    if device is not None and x.device != device:
+    if device is not None and index != device.index:
         raise ValueError(f"{name} is on {x.device}, not on {device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: flat scoring has none")
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    return x.data_ptr(), elem, x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    n, width = shape
+    ld = width
+    if not x.is_contiguous():
+        ld, unit = x.stride()
+        if width > 1 and unit != 1:
+            raise ValueError(f"{name} must have unit stride along its last dimension")
+        if n < 2:
+            ld = width
+    return x.data_ptr(), elem, ld, n, width
 
 
 def _side(x, name: str, dtype, nq: int, width: int | None, device):
     """(pointer, row stride, width) of an adjustment given for each row (nq, width), or shared (1, width) or (width,)."""
-    torch = _t()
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != device:
+    if not isinstance(x, _torch.Tensor) or x.dtype != dtype or x.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor on {device}")
-    if x.dim() == 1:
-        x = x[None]
-    if x.dim() != 2 or x.shape[0] not in (1, nq) or (width is not None and x.shape[1] != width):
+    shape = x.shape
+    n, w = (1, *shape) if len(shape) == 1 else shape if len(shape) == 2 else (-1, 0)
+    if n != 1 and n != nq or n < 0 or (width is not None and w != width):
         raise ValueError(f"{name} must have {'one row or ' + str(nq)} rows" +
                          (f" of {width}" if width is not None else ""))
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0, x.shape[1]
+    ld = w
+    if not x.is_contiguous():
+        if w > 1 and x.stride(-1) != 1:
+            raise ValueError(f"{name} must have unit stride along its last dimension")
+        ld = x.stride(0)
+    return x.data_ptr(), ld if n > 1 else 0, w
 
 
 def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presence):
@@ -88,7 +97,7 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
             if seen is None:
                 raise ValueError(f"{name} needs seen")
             if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != device or \
-                    x.shape != (nq,) or (nq > 1 and x.stride(0) != 1):
+                    x.shape != (nq,) or not x.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous float32 tensor of {nq} numbers on {device}")
             setattr(a, name, x.data_ptr())
     return a
@@ -119,8 +128,7 @@ def code_pitch(dim: int) -> int:
 
 def _quantize(rows, norms: bool):
     torch = _t()
-    ptr, elem, ld = _rows(rows, "rows")
-    n, dim = rows.shape
+    ptr, elem, ld, n, dim = _rows(rows, "rows")
     if not 1 <= dim <= MAX_DIM:
         raise ValueError(f"dim must be in [1, {MAX_DIM}]")
     codes = torch.empty((n, code_pitch(dim)), dtype=torch.int8, device=rows.device)
@@ -157,23 +165,22 @@ class FlatTable:
 def _queries(table, queries):
     if not isinstance(table, FlatTable):
         raise ValueError("table must be a FlatTable")
-    ptr, elem, ld = _rows(queries, "queries", table.device)
-    if queries.shape[1] != table.dim:
-        raise ValueError(f"queries have dim {queries.shape[1]}, the table {table.dim}")
-    return ptr, elem, ld
+    ptr, elem, ld, nq, dim = _rows(queries, "queries", table.device)
+    if dim != table.dim:
+        raise ValueError(f"queries have dim {dim}, the table {table.dim}")
+    return ptr, elem, ld, nq
 
 
 def scores(table: FlatTable, queries, dtype=None, out=None):
     """The scores (nq, n) of every record, (float(sum of code products) * query scale) * record scale [+ bias], in `dtype`
     (default float32) or into `out`."""
     torch = _t()
-    ptr, elem, ld = _queries(table, queries)
-    nq = queries.shape[0]
+    ptr, elem, ld, nq = _queries(table, queries)
     if out is None:
         out = torch.empty((nq, table.n), dtype=dtype or torch.float32, device=table.device)
     elif (dtype is not None and out.dtype != dtype) or out.shape != (nq, table.n):
         raise ValueError(f"out must be ({nq}, {table.n}) of the asked dtype")
-    optr, oelem, old = _rows(out, "out", table.device)
+    optr, oelem, old = _rows(out, "out", table.device)[:3]
     lib = L.lib()
     size = lib.shine_flat_scores_workspace(nq, table.n, table.dim)
     ws = _workspace(size, table.device)
@@ -195,14 +202,13 @@ def adjust(scores, bias=None, allow=None, seen=None, repetition=None, frequency=
     `out` may be `scores` itself.
     """
     torch = _t()
-    ptr, elem, ld = _rows(scores, "scores")
-    nq, n = scores.shape
+    ptr, elem, ld, nq, n = _rows(scores, "scores")
     a = _adjustment(nq, n, scores.device, bias, allow, seen, repetition, frequency, presence)
     if out is None:
         out = torch.empty((nq, n), dtype=scores.dtype, device=scores.device)
     elif out.dtype != scores.dtype or out.shape != scores.shape:
         raise ValueError("out must have the scores' shape and dtype")
-    optr, _, old = _rows(out, "out", scores.device)
+    optr, _, old = _rows(out, "out", scores.device)[:3]
     L.check(L.lib().shine_flat_adjust(scores.device.index, ptr, elem, nq, n, ld, C.byref(a), optr, old,
                                       _stream(scores.device)))
     return out
@@ -212,8 +218,7 @@ def topk(scores, k: int):
     """The k largest scores of every row in descending order, ties to the lower id: values (nq, k) and ids int32 (nq, k).
     -infinity and NaN are never returned: places without an answer hold id -1 and -infinity."""
     torch = _t()
-    ptr, elem, ld = _rows(scores, "scores")
-    nq, n = scores.shape
+    ptr, elem, ld, nq, n = _rows(scores, "scores")
     if not 1 <= k <= MAX_K:
         raise ValueError(f"k must be in [1, {MAX_K}]")
     values = torch.empty((nq, k), dtype=scores.dtype, device=scores.device)
@@ -231,8 +236,8 @@ def search(table: FlatTable, queries, k: int, bias=None, allow=None, seen=None, 
     """topk(adjust(scores(table, queries), ...), k), bit for bit, without the score matrix: values float32 (nq, k) and ids
     int32 (nq, k)."""
     torch = _t()
-    ptr, elem, ld = _queries(table, queries)
-    nq, device = queries.shape[0], table.device
+    ptr, elem, ld, nq = _queries(table, queries)
+    device = table.device
     if not 1 <= k <= MAX_K:
         raise ValueError(f"k must be in [1, {MAX_K}]")
     a = None

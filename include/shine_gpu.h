@@ -485,7 +485,8 @@ uint64_t shine_flat_scores_workspace(uint32_t nq, uint64_t n, uint32_t dim); /* 
 int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,
                       void* d_out, int out_elem, uint64_t out_ld, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
-/* See shine_flat_adjustment.  d_out may be d_scores (with the same stride); otherwise the two do not overlap. */
+/* See shine_flat_adjustment.  d_out may be d_scores (with the same stride); rows that overlap otherwise are
+ * refused. */
 int shine_flat_adjust(int gpu_id, const void* d_scores, int elem, uint32_t nq, uint64_t n, uint64_t ld,
                       const shine_flat_adjustment* adjustment, void* d_out, uint64_t out_ld, void* stream);
 

@@ -140,3 +140,11 @@ def test_python_refuses_what_is_no_gpu_row_tensor():
         flat.FlatTable(torch.zeros(2, 2), metric="cosine")
     with pytest.raises(ValueError, match="FlatTable"):
         flat.search(torch.zeros(2, 2), torch.zeros(2, 2), 1)
+
+
+def test_adjust_refuses_rows_that_overlap():
+    f = L.lib().shine_flat_adjust
+    for out, ld, out_ld in ((P + 4, 100, 100), (P, 100, 101), (P + 396, 100, 100), (P - 396, 100, 100), (P + 99 * 4, 250, 250),
+                            (P + (250 + 151) * 4, 250, 250), (P + 1000, 100, 300)):
+        refused(f(0, P, 0, 4, 100, ld, adjustment(), out, out_ld, None), "overlaps")
+    refused(f(0, P, 0, 1, 100, 100, adjustment(), P + 4, 100, None), "overlaps")

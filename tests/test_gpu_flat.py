@@ -866,3 +866,18 @@ def test_passes_captured_and_replayed_beside_other_streams():
         want = flat.topk(flat.adjust(flat.scores(table, q), **a), 10)
         assert torch.equal(out[1], want[1]) and torch.equal(out[0], want[0])
         assert torch.equal(beside[1], want_other[1]) and torch.equal(beside[0], want_other[0])
+
+
+def test_adjust_from_and_to_rows_that_lie_between_each_other():
+    flat = F()
+    both = rows(9, 202, 1)
+    bias = rows(1, 100, 2)[0]
+    for a, b in ((0, 100), (102, 1), (0, 0), (50, 50)):
+        here = both.cuda()
+        out = flat.adjust(here[:, a:a + 100], bias=bias.cuda(), out=here[:, b:b + 100])
+        want = both.clone()
+        want[:, b:b + 100] = both[:, a:a + 100] + bias
+        assert torch.equal(here.cpu(), want) and out.data_ptr() == here[:, b:].data_ptr()
+    import shine_amd
+    with pytest.raises(shine_amd.ShineError, match="overlaps"):
+        flat.adjust(here[:, :100], bias=bias.cuda(), out=here[:, 60:160])
