@@ -418,12 +418,15 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint64
 // in LDS, at the offsets that they have in memory's lines; what completes a line is written, the rest is there for the next
 // turn.  Rings of 16 queries are turned against one another so that the 64 lanes of a write, and of a read, meet different banks.
 //
-// A run's first line begins in the records before: long runs of f32 score them again (one turn more of 8 or more), short ones and
-// 16-bit scores, whose turns are twice as long, write the line's part.  1024 x 100,003 x 96, kernel and quantising: f32 166 ->
-// 106 us (with the part 119), bf16 into four buffers by turns 97 -> 77 (into one, which the caches half hold, 77 -> 60); rows of
-// 100,000: 114 -> 105, 74 -> 69 (47 -> 55).  128 queries a wave: 130; 32, with four waves a SIMD: 125.  What bounds it is the
-// writing: 4.1 TB/s, of 6.7 that a fill reaches.
-template <class T, int KC, int QT>
+// A run's first line begins in the records before: long runs of f32 score them again (a turn more of 8 or more lines), short ones
+// and 16-bit scores, whose turns are twice as long, write the line's part.  Memory accesses end in order, so a turn's end, where
+// the next turn's codes are taken, waits for the writes of the turn before it: P lines a turn, two where the registers have room
+// for their codes, put that off (100 us a call against 106).
+//
+// 1024 x 100,003 x 96, kernel and quantising: f32 166 -> 100 us (with lines' parts written 119), bf16 into four buffers by turns
+// 97 -> 77 (into one, which the caches half hold, 77 -> 60); rows of 100,000: 114 -> 100, 74 -> 69 (47 -> 55).  128 queries a wave:
+// 130; 32, with four waves a SIMD: 125.  What bounds it is the writing: 4.4 TB/s, of 6.7 that a fill reaches.
+template <class T, int KC, int QT, int P>
 __global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per) {
   constexpr uint32_t kLine = 128 / sizeof(T), kPiece = 16 / sizeof(T);  // scores of a line and of 16 bytes
   constexpr int NT = kLine / 16, U = QT * 2;
@@ -459,32 +462,54 @@ __global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint
   const v4i start = magic_start();
   const float* biases = a.bias ? a.bias : a.scales;
   const bool biased = a.bias;
-  v4i next[NT][KC], x[NT][KC];
-  float next_xs[NT], next_bias[NT], xs[NT], bias[NT];
-  auto fetch = [&](uint64_t b) {
-    const int8_t* p = a.codes + b * (kLine * KC * 64);
-    const uint32_t last = static_cast<uint32_t>(min(a.n - b * kLine, static_cast<uint64_t>(kLine))) - 1;
+  v4i next[P][NT][KC], x[P][NT][KC];
+  float next_xs[P][NT], next_bias[P][NT], xs[P][NT], bias[P][NT];
+  auto fetch = [&](uint64_t b0) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint32_t r = min(t * 16 + col, last);
+    for (int p = 0; p < P; ++p) {
+      const uint64_t b = min(b0 + p, lines - 1);
+      const int8_t* from = a.codes + b * (kLine * KC * 64);
+      const uint32_t last = static_cast<uint32_t>(min(a.n - b * kLine, static_cast<uint64_t>(kLine))) - 1;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) next[t][c] = *reinterpret_cast<const v4i*>(p + r * (KC * 64) + group * 16 + c * 64);
-      next_xs[t] = (a.scales + b * kLine)[r];
-      next_bias[t] = (biases + b * kLine)[r];
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t r = min(t * 16 + col, last);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) next[p][t][c] = *reinterpret_cast<const v4i*>(from + r * (KC * 64) + group * 16 + c * 64);
+        next_xs[p][t] = (a.scales + b * kLine)[r];
+        next_bias[p][t] = (biases + b * kLine)[r];
+      }
     }
   };
   auto stage = [&] {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        x[t][c] = next[t][c];
-        asm volatile("" : "+v"(x[t][c]));
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          x[p][t][c] = next[p][t][c];
+          asm volatile("" : "+v"(x[p][t][c]));
+        }
+        xs[p][t] = next_xs[p][t];
+        bias[p][t] = biased ? next_bias[p][t] : -0.0f;
+        asm volatile("" : "+v"(xs[p][t]), "+v"(bias[p][t]));
       }
-      xs[t] = next_xs[t];
-      bias[t] = biased ? next_bias[t] : -0.0f;
-      asm volatile("" : "+v"(xs[t]), "+v"(bias[t]));
-    }
+  };
+  auto score = [&](int p, uint32_t parity) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        v4i acc = start;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i][c], x[p][t][c], acc, 0, 0, 0);
+        const uint32_t to = ((place[i] & 0x7F7F7F7Fu) + t * 16 * sizeof(T) * 0x01010101u) ^ (place[i] & 0x80808080u) ^ parity * 0x01010101u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<T*>(ring + (i * 16 + group * 4 + j) * 256 + (to >> (8 * j) & 255)) =
+              from_f32<T>(((__int_as_float(acc[j]) - kMagicF) * qs[i][j]) * xs[p][t] + bias[p][t]);
+      }
+    wave_sync();
   };
   auto ring_piece = [&](uint32_t r, uint32_t parity) { return ring + r * 256 + ((turned(r) + parity + (lane & 7) * 16) & 255); };
   // the scores [from, to) of line b: pieces of 16 bytes, or one by one where a piece is not all of these
@@ -505,40 +530,35 @@ __global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint
       }
     }
   };
-  const uint64_t b0 = again && first ? first - 1 : first, from = again ? 0 : first * kLine;
+  const uint64_t b0 = again && first ? first - P : first, from = again ? 0 : first * kLine,
+                 whole = again ? max(first, 1ul) : first + 1;  // the first line that is all of this run's
+  auto parity_of = [&](uint64_t b, int p) { return P == 2 ? p * 128u : static_cast<uint32_t>(b - b0 & 1) * 128u; };
   fetch(b0);
   stage();
-  uint32_t parity = 0;
-  for (uint64_t b = b0; b < end; ++b, parity ^= 128) {
-    fetch(b + 1 < end ? b + 1 : b);
+  for (uint64_t b = b0; b < end; b += P) {
+    fetch(b + P);
+    if (b >= whole && b + P < lines) {
 #pragma unroll
-    for (int i = 0; i < QT; ++i)
+      for (int p = 0; p < P; ++p) {
+        score(p, parity_of(b, p));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        v4i acc = start;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i][c], x[t][c], acc, 0, 0, 0);
-        const uint32_t to = ((place[i] & 0x7F7F7F7Fu) + t * 16 * sizeof(T) * 0x01010101u) ^ (place[i] & 0x80808080u) ^ parity * 0x01010101u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<T*>(ring + (i * 16 + group * 4 + j) * 256 + (to >> (8 * j) & 255)) =
-              from_f32<T>(((__int_as_float(acc[j]) - kMagicF) * qs[i][j]) * xs[t] + bias[t]);
+        for (int u = 0; u < U; ++u)
+          *reinterpret_cast<v4i*>(line[u] + (b + p) * 128) = *reinterpret_cast<const v4i*>(ring_piece(u * 8 + (lane >> 3), parity_of(b, p)));
+        wave_sync();
       }
-    wave_sync();
-    if (b < first) {
-      stage();
-    } else if (b == (again ? 0 : first) || b + 1 == lines) {
-      edge(b, parity, from, a.n);
-      stage();  // in each branch: behind them all it would wait for all writes
+      stage();  // in each branch: behind them both it would wait for all writes
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        *reinterpret_cast<v4i*>(line[u] + b * 128) = *reinterpret_cast<const v4i*>(ring_piece(u * 8 + (lane >> 3), parity));
+      for (int p = 0; p < P; ++p)
+        if (b + p + 1 >= first && b + p < end) {
+          score(p, parity_of(b, p));
+          if (b + p >= first) edge(b + p, parity_of(b, p), from, a.n);
+          wave_sync();
+        }
       stage();
     }
-    wave_sync();
   }
-  if (!again || end == lines) edge(end, parity, from, min(end * kLine, a.n));
+  if (!again || end == lines) edge(end, static_cast<uint32_t>(end - b0 & 1) * 128, from, min(end * kLine, a.n));
 }
 
 // Wider rows: tiles of 256 records x 128 queries, four waves of 128 x 64 each, 64 codes of every row a step.  A step's codes go
@@ -1755,8 +1775,10 @@ void scores_in_lines_of(const ScoresArgs& a, hipStream_t s) {
   constexpr int QT = 4;
   constexpr uint32_t kLine = 128 / sizeof(T);
   const uint32_t qb = (a.nq + QT * 16 - 1) / (QT * 16);
-  const Ranges r = ranges_of(((a.n + kLine - 1) / kLine), qb, 512);  // of per_wave * 4 lines
-  hipLaunchKernelGGL((scores_lines_kernel<T, KC, QT>), dim3(r.grid), dim3(256), 0, s, a, qb, (r.per + 3) / 4);
+  const Ranges r = ranges_of((a.n + kLine - 1) / kLine, qb, 512);
+  constexpr int P = sizeof(T) == 4 && KC <= 2 ? 2 : 1;
+  const uint64_t per = (r.per + 4 * P - 1) / (4 * P) * P;
+  hipLaunchKernelGGL((scores_lines_kernel<T, KC, QT, P>), dim3(r.grid), dim3(256), 0, s, a, qb, per);
 }
 template <class T>
 void scores_in_lines(const ScoresArgs& a, hipStream_t s) {
