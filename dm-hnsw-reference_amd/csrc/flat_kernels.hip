@@ -1001,6 +1001,7 @@ __device__ inline void make_room(Held& h, uint32_t k, uint32_t slack) {
   place<M>(h, kept, [&](int i) { return key[i]; });
   __syncthreads();
   const uint32_t left = h.count;
+  __syncthreads();  // behind it the count may grow again
   if (left <= kKeys / 2) return;
   for (uint32_t i = left + threadIdx.x; i < kKeys; i += 256) h.key[i] = 0;
   __syncthreads();

@@ -881,3 +881,16 @@ def test_adjust_from_and_to_rows_that_lie_between_each_other():
     import shine_amd
     with pytest.raises(shine_amd.ShineError, match="overlaps"):
         flat.adjust(here[:, :100], bias=bias.cuda(), out=here[:, 60:160])
+
+
+def test_topk_of_rising_rows_many_times():
+    """room is made in every turn of every workgroup: the answers do not depend on how its waves take turns"""
+    n = 60000
+    x = torch.arange(n, dtype=torch.float32).repeat(512, 1)
+    x[1::2] = x[1::2].view(256, -1, 4)[:, :, [2, 0, 3, 1]].reshape(256, n)  # nearly rising
+    x = x.cuda()
+    for k in (100, 256):
+        want = torch.arange(n - 1, n - 1 - k, -1, dtype=torch.float32, device="cuda").expand(512, k)
+        for _ in range(40):
+            values, ids = F().topk(x, k)
+            assert torch.equal(values, want) and torch.equal(x.gather(1, ids.long()), want)
