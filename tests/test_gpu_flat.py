@@ -894,3 +894,23 @@ def test_topk_of_rising_rows_many_times():
         for _ in range(40):
             values, ids = F().topk(x, k)
             assert torch.equal(values, want) and torch.equal(x.gather(1, ids.long()), want)
+
+
+@pytest.mark.parametrize("nq", [33, 120])
+@pytest.mark.parametrize("k", [10, 256])
+def test_search_gives_the_same_answers_every_time(nq, k):
+    """by way of the matrix and in passes, whose lists run full: in whatever order waves and workgroups come"""
+    n = 270000
+    x = rows(n, 32, 5) * 0.1
+    x[:, 0] = torch.where((torch.arange(n) // 32) % 9 == 0, -1.0, 1.0)
+    q = rows(nq, 32, 6) * 0.1
+    q[:, 0] = 1
+    a = cuda(adjustments(nq, n, 3, 40, "shared", "rows"))
+    flat = F()
+    table = flat.FlatTable(x.cuda())
+    want = flat.topk(flat.adjust(flat.scores(table, q.cuda()), **a), k)
+    s = flat.scores(table, q.cuda())
+    for _ in range(40):
+        assert torch.equal(flat.scores(table, q.cuda()), s)
+        values, ids = flat.search(table, q.cuda(), k, **a)
+        assert torch.equal(ids, want[1]) and torch.equal(values, want[0])
