@@ -32,11 +32,11 @@ def _t():
     global _torch, _current
     if _torch is None:
         import torch
-        _torch = torch
         # the stream's handle alone where torch gives it: a Stream object costs 2 us a call
         _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
             (lambda index: torch.cuda.current_stream(index).cuda_stream)
         _elems.update({torch.float32: L.ELEM_F32, torch.float16: L.ELEM_F16, torch.bfloat16: L.ELEM_BF16})
+        _torch = torch  # last: other threads take it as a sign that the rest is there
     return _torch
 
 

@@ -914,3 +914,30 @@ def test_search_gives_the_same_answers_every_time(nq, k):
         assert torch.equal(flat.scores(table, q.cuda()), s)
         values, ids = flat.search(table, q.cuda(), k, **a)
         assert torch.equal(ids, want[1]) and torch.equal(values, want[0])
+
+
+def test_calls_from_several_threads():
+    import threading
+    flat = F()
+    table = flat.FlatTable(rows(60000, 64, 1).cuda(), metric="l2")
+    qs = [rows(nq, 64, nq).cuda() for nq in (3, 40, 500, 900)]
+    want = [flat.search(table, q, 20) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                values, ids = flat.search(table, qs[i], 20)
+                v, j = flat.topk(flat.scores(table, qs[i]), 20)
+                if not (torch.equal(values, want[i][0]) and torch.equal(ids, want[i][1]) and torch.equal(v, want[i][0])
+                        and torch.equal(j, want[i][1])):
+                    wrong.append(i)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(qs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
