@@ -1242,8 +1242,9 @@ struct __attribute__((aligned(16))) Terms {
 // A record for which the margin says nothing always passes (scales and biases whose quotients may overflow), one that is no
 // answer never does: its terms are u = +-1e20 alone.  The reciprocals are within 2^-22.
 constexpr float kNear = 1e9f, kSure = 1e20f;
-__device__ inline Terms record_terms(float x, float b, float size, bool on) {
-  x = x == 0.0f ? 1.0f : x;  // its codes and so its sums are 0, whatever they are scaled by
+// A record of scale 0 is as one of scale 1 if its sums are 0 too: if it has no `codes`.
+__device__ inline Terms record_terms(float x, float b, float size, bool on, bool codes) {
+  x = x == 0.0f && !codes ? 1.0f : x;
   const bool plain = on && x > 1.0f / kNear && x < kNear && size < kNear;
   const bool none = !on || x != x || !(b > -__builtin_huge_valf());
   const float w = plain ? __builtin_amdgcn_rcpf(x) : 0.0f, u = plain ? b * w : none ? -kSure : kSure;
@@ -1262,13 +1263,24 @@ __device__ inline int query_limit(float q, float low, bool there) {
   return !there || q != q ? 0x7FFFFFFF : query_plain(q, low) ? kMagic : -0x7FFFFFFF - 1;
 }
 
+// Whether a row has codes other than 0: a scale may be set to 0 with its codes left as they are
+__device__ inline bool has_codes(const PassArgs& a, uint64_t record) {
+  uint32_t some = 0;
+  for (uint32_t c = 0; c < a.pitch; c += 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(a.codes + record * a.pitch + c);
+    some |= v.x | v.y | v.z | v.w;
+  }
+  return some != 0;
+}
+
 __device__ inline void write_record_terms(const PassArgs& a, uint64_t block) {  // of 256 records
   const uint64_t r = block * 256 + threadIdx.x;
   if (r >= (a.n + 31) / 32 * 32) return;
   const uint64_t at = min(r, a.n - 1);
   const bool on = r < a.n && (!a.allow || a.allow_ld || (a.allow[r >> 5] >> (r & 31) & 1u));
   const float tb = a.tbias ? a.tbias[at] : 0.0f, ab = a.abias ? a.abias[at] : 0.0f;
-  static_cast<Terms*>(a.record_terms)[r] = record_terms(a.scales[at], tb + ab, fabsf(tb) + fabsf(ab), on);
+  const float x = a.scales[at];
+  static_cast<Terms*>(a.record_terms)[r] = record_terms(x, tb + ab, fabsf(tb) + fabsf(ab), on, x == 0.0f && has_codes(a, at));
 }
 
 // Both passes: a wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32

@@ -941,3 +941,25 @@ def test_calls_from_several_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("nq", [40, 1400])  # by way of the matrix, and in passes
+@pytest.mark.parametrize("dim", [32, 200])
+def test_search_of_records_whose_scales_were_changed(dim, nq):
+    """scales of 0 and below 0 beside codes that stay: the scores are those of the changed scales"""
+    flat = F()
+    n = 20000
+    q = rows(nq, dim, 4).cuda()
+    bias = torch.full((n,), -100.0)
+    bias[::200] = 0  # the answers
+    for scale in (0.0, -0.0, -1e-3):
+        table = flat.FlatTable(rows(n, dim, 3).cuda())
+        table.scales[::200] = scale
+        values, ids = flat.search(table, q, 10, bias=bias.cuda())
+        v, i = flat.topk(flat.adjust(flat.scores(table, q), bias=bias.cuda()), 10)
+        assert (i % 200 == 0).all() and torch.equal(ids, i) and torch.equal(values, v)
+    x = rows(n, dim, 3)
+    x[::200] = 0  # no codes either
+    table = flat.FlatTable(x.cuda())
+    values, ids = flat.search(table, q, 10, bias=bias.cuda())
+    assert torch.equal(ids.cpu(), (torch.arange(10) * 200).int().expand(nq, 10)) and (values == 0).all()
