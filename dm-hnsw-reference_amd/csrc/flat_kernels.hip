@@ -1242,11 +1242,13 @@ struct __attribute__((aligned(16))) Terms {
 // A record for which the margin says nothing always passes (scales and biases whose quotients may overflow), one that is no
 // answer never does: its terms are u = +-1e20 alone.  The reciprocals are within 2^-22.
 constexpr float kNear = 1e9f, kSure = 1e20f;
-// A record of scale 0 is as one of scale 1 if its sums are 0 too: if it has no `codes`.
-__device__ inline Terms record_terms(float x, float b, float size, bool on, bool codes) {
+// A record of scale 0 is as one of scale 1 if its sums are 0 too: if it has no `codes`.  Each bias on its own may say that it is no
+// answer; two finite ones do not, even where their sum b overflows: a large product takes them one after the other.
+__device__ inline Terms record_terms(float x, float tb, float ab, bool on, bool codes) {
+  const float b = tb + ab, size = fabsf(tb) + fabsf(ab);
   x = x == 0.0f && !codes ? 1.0f : x;
   const bool plain = on && x > 1.0f / kNear && x < kNear && size < kNear;
-  const bool none = !on || x != x || !(b > -__builtin_huge_valf());
+  const bool none = !on || x != x || !(tb > -__builtin_huge_valf()) || !(ab > -__builtin_huge_valf());
   const float w = plain ? __builtin_amdgcn_rcpf(x) : 0.0f, u = plain ? b * w : none ? -kSure : kSure;
   const Two a(u), c(w);
   return {{a.hi, a.hi, a.lo, c.hi, c.hi, c.lo, static_cast<__bf16>(plain ? 0x1p-13f * (size * w) : 0.0f), static_cast<__bf16>(0x1p-13f * w)}};
@@ -1280,7 +1282,7 @@ __device__ inline void write_record_terms(const PassArgs& a, uint64_t block) {  
   const bool on = r < a.n && (!a.allow || a.allow_ld || (a.allow[r >> 5] >> (r & 31) & 1u));
   const float tb = a.tbias ? a.tbias[at] : 0.0f, ab = a.abias ? a.abias[at] : 0.0f;
   const float x = a.scales[at];
-  static_cast<Terms*>(a.record_terms)[r] = record_terms(x, tb + ab, fabsf(tb) + fabsf(ab), on, x == 0.0f && has_codes(a, at));
+  static_cast<Terms*>(a.record_terms)[r] = record_terms(x, tb, ab, on, x == 0.0f && has_codes(a, at));
 }
 
 // Both passes: a wave keeps QT * 32 queries and looks at every fourth block of the workgroup's, in tiles of 32 records x 32

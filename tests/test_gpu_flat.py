@@ -963,3 +963,29 @@ def test_search_of_records_whose_scales_were_changed(dim, nq):
     table = flat.FlatTable(x.cuda())
     values, ids = flat.search(table, q, 10, bias=bias.cuda())
     assert torch.equal(ids.cpu(), (torch.arange(10) * 200).int().expand(nq, 10)) and (values == 0).all()
+
+
+@pytest.mark.parametrize("nq", [40, 1400])
+def test_search_of_a_record_whose_biases_add_up_to_infinity(nq):
+    """The table's bias and the call's are added to the score one after the other: with u = 2^104 the product is (2^24 - 1) u, the
+    largest number, adding -(1.5 * 2^22 + 1.5) u ends halfway between two numbers and goes up to the even one, and what is left is
+    what the second bias takes off.  The score is 0, far above the others, though the biases' sum is -infinity."""
+    flat = F()
+    n, j, unit = 20000, 7777, 2.0 ** 104
+    first = (1.5 * 2 ** 22 + 1.5) * unit
+    second = (2.0 ** 24 - 0.5) * unit - first
+    table = flat.FlatTable(rows(n, 32, 1).cuda(), metric="l2")
+    table.codes[j] = 0
+    table.codes[j, 1] = 64
+    table.scales[j] = torch.finfo(torch.float32).max / 64
+    table.bias[j] = -first
+    bias = torch.full((n,), -1000.0)
+    bias[j] = -second
+    q = torch.ones(nq, 32)
+    q[:, 0] = 127  # scale 1, codes 127 and 1
+    s = flat.adjust(flat.scores(table, q.cuda()), bias=bias.cuda())
+    assert (s[:, j] == 0).all() and table.bias[j].item() == -first and bias[j].item() == -second
+    assert (table.bias[j] + bias.cuda()[j]).item() == NEG
+    values, ids = flat.search(table, q.cuda(), 10, bias=bias.cuda())
+    v, i = flat.topk(s, 10)
+    assert (i[:, 0] == j).all() and torch.equal(ids, i) and torch.equal(values, v)
