@@ -156,10 +156,16 @@ class FlatTable:
                               self.bias.data_ptr() if metric == "l2" else None, self.n, self.dim, 0)
 
     def distances(self, values, queries):
-        """Squared L2 distances of the scores `values` (nq, ...) of an "l2" table: |q|^2 - 2 value."""
+        """Squared L2 distances of the scores `values` (nq, ...) of an "l2" table: max(|q|^2 - 2 value, 0), between the rows
+        that the codes of the queries and of the records stand for.  Places without an answer are infinitely far."""
         if self.metric != "l2":
             raise ValueError("the table's scores are inner products")
-        return queries.float().square().sum(1).reshape(-1, *[1] * (values.dim() - 1)) - 2.0 * values.float()
+        queries = queries.to(self.device)
+        _queries(self, queries)
+        half = _quantize(queries, True)[2].to(values.device)  # -|q|^2 / 2, of the quantised query as in its scores
+        values = values.float()
+        far = (-2.0 * (half.reshape(-1, *[1] * (values.dim() - 1)) + values)).clamp_min(0.0)
+        return far.masked_fill(values == float("-inf"), float("inf"))
 
 
 def _queries(table, queries):

@@ -989,3 +989,47 @@ def test_search_of_a_record_whose_biases_add_up_to_infinity(nq):
     values, ids = flat.search(table, q.cuda(), 10, bias=bias.cuda())
     v, i = flat.topk(s, 10)
     assert (i[:, 0] == j).all() and torch.equal(ids, i) and torch.equal(values, v)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim,unit", [(4000, 96, True), (700, 200, False), (50, 7, False)])
+def test_distances_of_queries_as_they_are(n, dim, unit, dtype):
+    """|q^ - x^|^2 between the rows that the codes stand for, never below 0, for queries that were not quantised before.
+
+    With H = (|q^|^2 + |x^|^2) / 2 >= |<q^, x^>|: the product's three roundings and each half norm's three come to 6 u32 H, the
+    score's addition and the last one, of at most 2 H each, to 4 u32 H, and twice all of it is 20 u32 H."""
+    flat = F()
+    x = rows(n, dim, dim)
+    m = min(n, 60)
+    q = x[:m] + torch.linspace(-0.3, 0.7, m).clamp_min(0)[:, None] * rows(m, dim, 2)  # records themselves, and rows farther away
+    if unit:
+        x, q = torch.nn.functional.normalize(x), torch.nn.functional.normalize(q)
+    x, q = x.to(dtype), q.to(dtype)
+    table = flat.FlatTable(x.cuda(), metric="l2")
+    values, ids = flat.search(table, q.cuda(), 5)
+    d = table.distances(values, q.cuda())
+    assert d.dtype == torch.float32 and (d >= 0).all()
+    xc, xs = codes64(x)
+    qc, qs = codes64(q)
+    xd, qd = xc * xs[:, None], qc * qs[:, None]
+    found = xd[ids.cpu().long()]
+    want = (qd[:, None] - found).square().sum(2)
+    half = (qd.square().sum(1)[:, None] + found.square().sum(2)) / 2
+    assert ((d.cpu().double() - want).abs() <= 20.01 * U32 * half).all()
+    assert torch.equal(table.distances(values.cpu(), q), d.cpu())
+    whole = table.distances(flat.scores(table, q.cuda()), q.cuda())
+    assert torch.equal(whole.gather(1, ids.long()), d)
+
+
+def test_distances_of_places_without_an_answer():
+    flat = F()
+    table = flat.FlatTable(rows(3, 16, 1).cuda(), metric="l2")
+    q = rows(4, 16, 2)
+    q[1, 3], q[2, 5] = math.nan, math.inf
+    values, ids = flat.search(table, q.cuda(), 5)
+    d = table.distances(values, q.cuda())
+    assert torch.equal(d.isposinf(), ids < 0) and d[[0, 3], :3].isfinite().all()
+    with pytest.raises(ValueError, match="dim 15"):
+        table.distances(values, q[:, :15].cuda())
+    with pytest.raises(ValueError, match="inner products"):
+        flat.FlatTable(rows(3, 16, 1).cuda()).distances(values, q.cuda())
