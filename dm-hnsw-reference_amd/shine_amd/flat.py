@@ -13,7 +13,8 @@ or step by step, with the score matrix in hand:
     values, ids = topk(s, 10)
 
 Tensors are CUDA tensors of torch.float32, float16 or bfloat16 with unit stride along their last dimension; calls run on
-the current stream of the tensors' device and do not wait for it.  There are no gradients.
+the current stream of the tensors' device and do not wait for it.  There are no gradients: tensors that require one are
+refused unless under torch.no_grad().
 """
 from __future__ import annotations
 
@@ -40,6 +41,11 @@ def _t():
     return _torch
 
 
+def _no_gradient(x, name: str):
+    if x.requires_grad and _torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: flat scoring has none")
+
+
 def _rows(x, name: str, device=None):
     """(pointer, element type, row stride, rows, width) of a 2-D tensor of rows, or ValueError."""
     torch = _t()
@@ -53,8 +59,7 @@ def _rows(x, name: str, device=None):
         raise ValueError(f"{name} must be on a GPU")
     if device is not None and index != device.index:
         raise ValueError(f"{name} is on {x.device}, not on {device}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: flat scoring has none")
+    _no_gradient(x, name)
     n, width = shape
     ld = width
     if not x.is_contiguous():
@@ -70,6 +75,7 @@ def _side(x, name: str, dtype, nq: int, width: int | None, device):
     """(pointer, row stride, width) of an adjustment given for each row (nq, width), or shared (1, width) or (width,)."""
     if not isinstance(x, _torch.Tensor) or x.dtype != dtype or x.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor on {device}")
+    _no_gradient(x, name)
     shape = x.shape
     n, w = (1, *shape) if len(shape) == 1 else shape if len(shape) == 2 else (-1, 0)
     if n != 1 and n != nq or n < 0 or (width is not None and w != width):
@@ -99,6 +105,7 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
             if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != device or \
                     x.shape != (nq,) or not x.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous float32 tensor of {nq} numbers on {device}")
+            _no_gradient(x, name)
             setattr(a, name, x.data_ptr())
     return a
 

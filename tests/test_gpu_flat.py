@@ -1033,3 +1033,23 @@ def test_distances_of_places_without_an_answer():
         table.distances(values, q[:, :15].cuda())
     with pytest.raises(ValueError, match="inner products"):
         flat.FlatTable(rows(3, 16, 1).cuda()).distances(values, q.cuda())
+
+
+def test_adjustments_that_require_gradients_are_refused():
+    flat = F()
+    x = rows(20, 32, 1).cuda()
+    table = flat.FlatTable(x)
+    seen = torch.zeros((20, 1), dtype=torch.int32, device="cuda")
+    for name, like in (("bias", torch.zeros(20)), ("bias", torch.zeros(20, 20)), ("repetition", torch.ones(20)),
+                       ("frequency", torch.ones(20)), ("presence", torch.ones(20))):
+        a = {name: like.cuda().requires_grad_()}
+        if name != "bias":
+            a["seen"] = seen
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            flat.adjust(flat.scores(table, x), **a)
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            flat.search(table, x, 3, **a)
+        with torch.no_grad():
+            want = flat.adjust(flat.scores(table, x), **{k: v.detach() for k, v in a.items()})
+            assert torch.equal(flat.adjust(flat.scores(table, x), **a), want)
+            assert torch.equal(flat.search(table, x, 3, **a)[1], flat.topk(want, 3)[1])
