@@ -62,7 +62,7 @@ const char* check_adjustment(const shine_flat_adjustment* a, uint32_t nq, uint64
   if (a->allow && a->allow_ld && a->allow_ld < (n + 31) / 32 && nq > 1) return "allow row stride is shorter than a row";
   if (a->seen_n > F::kMaxHistory) return "seen_n must be at most 65535";
   if (a->seen_n && !a->seen) return "seen is NULL with seen_n > 0";
-  if (a->seen_n && a->seen_ld < a->seen_n && nq > 1) return "seen row stride is shorter than a row";
+  if (a->seen_n && a->seen_ld && a->seen_ld < a->seen_n && nq > 1) return "seen row stride is shorter than a row";
   if (!on(a->bias, 4) || !on(a->allow, 4) || !on(a->seen, 4) || !on(a->repetition, 4) || !on(a->frequency, 4) ||
       !on(a->presence, 4))
     return "an adjustment array is not 4-byte aligned";

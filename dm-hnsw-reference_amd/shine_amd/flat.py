@@ -205,9 +205,9 @@ def scores(table: FlatTable, queries, dtype=None, out=None):
 def adjust(scores, bias=None, allow=None, seen=None, repetition=None, frequency=None, presence=None, out=None):
     """Scores (nq, n) with penalties for shown records, biases and a filter, in this order, computed in float32:
 
-    * seen (nq, h) int32, record ids, repeats counted, -1 skipped: a record met c > 0 times has its score divided by
-      repetition[i] where positive and multiplied by it elsewhere, then frequency[i] * c + presence[i] taken off
-      (float32 (nq,) each);
+    * seen (h,), (1, h) or (nq, h) int32, record ids, repeats counted, -1 skipped: a record met c > 0 times has its score
+      divided by repetition[i] where positive and multiplied by it elsewhere, then frequency[i] * c + presence[i] taken
+      off (float32 (nq,) each);
     * bias float32 (n,), (1, n) or (nq, n), added;
     * allow int32, (n + 31) // 32 words for all rows or for each: bit j % 32 of word j // 32 set where record j may be
       returned; the others' scores become -infinity.

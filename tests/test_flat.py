@@ -148,3 +148,10 @@ def test_adjust_refuses_rows_that_overlap():
                             (P + (250 + 151) * 4, 250, 250), (P + 1000, 100, 300)):
         refused(f(0, P, 0, 4, 100, ld, adjustment(), out, out_ld, None), "overlaps")
     refused(f(0, P, 0, 1, 100, 100, adjustment(), P + 4, 100, None), "overlaps")
+
+
+def test_a_history_of_stride_0_is_shared_by_all_rows():
+    """accepted as a shared bias or mask is: what is refused next is the missing workspace, or the overlap"""
+    a = dict(seen=P, seen_n=3, seen_ld=0)
+    refused(L.lib().shine_flat_search(0, table(), P, 0, 4, 32, 10, adjustment(**a), P, P, None, 1 << 40, None), "workspace")
+    refused(L.lib().shine_flat_adjust(0, P, 0, 4, 100, 100, adjustment(**a), P + 4, 100, None), "overlaps")

@@ -1053,3 +1053,21 @@ def test_adjustments_that_require_gradients_are_refused():
             want = flat.adjust(flat.scores(table, x), **{k: v.detach() for k, v in a.items()})
             assert torch.equal(flat.adjust(flat.scores(table, x), **a), want)
             assert torch.equal(flat.search(table, x, 3, **a)[1], flat.topk(want, 3)[1])
+
+
+@pytest.mark.parametrize("nq,n", [(3, 700), (40, 9001), (2100, 20000)])
+def test_a_history_shared_by_all_rows(nq, n):
+    flat = F()
+    table = flat.FlatTable(rows(n, 64, 1).cuda(), metric="l2")
+    q = rows(nq, 64, 2).cuda()
+    s = flat.scores(table, q)
+    a = cuda(adjustments(nq, n, 3, 50))
+    seen = a.pop("seen")[0]
+    for one in (seen, seen[None], seen[:1], seen[:0]):
+        each = one.reshape(1, -1).repeat(nq, 1)
+        want = flat.adjust(s, seen=each, **a)
+        assert torch.equal(flat.adjust(s, seen=one, **a), want)
+        assert torch.equal(flat.adjust(s, seen=one.reshape(1, -1).expand(nq, -1), **a), want)
+        v, i = flat.topk(want, 20)
+        values, ids = flat.search(table, q, 20, seen=one, **a)
+        assert torch.equal(ids, i) and torch.equal(values, v)
