@@ -34,7 +34,9 @@ struct OnDevice {
 
 int fail(const char* what) { return set_error(SHINE_ERR_ARG, what); }
 int hip(const char* what, hipError_t e) {
-  return e == hipSuccess ? SHINE_OK : set_error(SHINE_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+  if (e == hipSuccess) return SHINE_OK;
+  (void)hipGetLastError();  // it is reported here, and not by whoever asks for the last error next
+  return set_error(SHINE_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 bool float_elem(int e) { return e == F::kF32 || e == F::kF16 || e == F::kBF16; }
 uint64_t elem_size(int e) { return e == F::kF32 ? 4 : 2; }

@@ -1712,35 +1712,45 @@ __global__ __launch_bounds__(256) void seen_kernel(SeenArgs a) {
 
 }  // namespace
 
-#define SHINE_BY_ELEM(elem, CALL)                 \
-  switch (elem) {                                 \
-    case kF32: { using T = float; CALL; break; }  \
-    case kF16: { using T = __half; CALL; break; } \
-    case kBF16: { using T = __bf16; CALL; break; } \
-    default: return hipErrorInvalidValue;         \
+// The launch's own error.  hipGetLastError would also give, and clear, what an earlier call of the program left behind.
+template <class T>
+struct As {
+  using type = T;
+};
+template <class... P>
+hipError_t launch(void (*kernel)(P...), dim3 grid, hipStream_t s, typename As<P>::type... p) {
+  void* args[] = {&p...};
+  return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(256), args, 0, s);
+}
+
+#define SHINE_BY_ELEM(elem, CALL)                  \
+  switch (elem) {                                  \
+    case kF32: { using T = float; return CALL; }   \
+    case kF16: { using T = __half; return CALL; }  \
+    case kBF16: { using T = __bf16; return CALL; } \
+    default: return hipErrorInvalidValue;          \
   }
 
 template <class T, int G, int S, int R>
-void quantize_with(const QuantizeArgs& a, uint32_t pitch, hipStream_t s) {
+hipError_t quantize_with(const QuantizeArgs& a, uint32_t pitch, hipStream_t s) {
   constexpr uint32_t rows = 256 / G * R;
   const uint64_t groups = std::min<uint64_t>((a.n + rows - 1) / rows, 8192);
-  hipLaunchKernelGGL((quantize_kernel<T, G, S, R>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0, s, a, pitch);
+  return launch(quantize_kernel<T, G, S, R>, dim3(static_cast<uint32_t>(groups)), s, a, pitch);
 }
 template <class T>
-void quantize_by_width(const QuantizeArgs& a, hipStream_t s) {
+hipError_t quantize_by_width(const QuantizeArgs& a, hipStream_t s) {
   const uint32_t pitch = code_pitch(a.dim), steps = pitch * sizeof(T) / 16;  // 16-byte steps of a row
-  if (steps <= 8) quantize_with<T, 8, 1, 2>(a, pitch, s);
-  else if (steps <= 16) quantize_with<T, 16, 1, 2>(a, pitch, s);
-  else if (steps <= 32) quantize_with<T, 32, 1, 2>(a, pitch, s);
-  else if (steps <= 64) quantize_with<T, 64, 1, 2>(a, pitch, s);
-  else if (steps <= 128) quantize_with<T, 64, 2, 1>(a, pitch, s);
-  else if (steps <= 256) quantize_with<T, 64, 4, 1>(a, pitch, s);
-  else quantize_with<T, 64, 0, 1>(a, pitch, s);
+  if (steps <= 8) return quantize_with<T, 8, 1, 2>(a, pitch, s);
+  if (steps <= 16) return quantize_with<T, 16, 1, 2>(a, pitch, s);
+  if (steps <= 32) return quantize_with<T, 32, 1, 2>(a, pitch, s);
+  if (steps <= 64) return quantize_with<T, 64, 1, 2>(a, pitch, s);
+  if (steps <= 128) return quantize_with<T, 64, 2, 1>(a, pitch, s);
+  if (steps <= 256) return quantize_with<T, 64, 4, 1>(a, pitch, s);
+  return quantize_with<T, 64, 0, 1>(a, pitch, s);
 }
 
 hipError_t launch_quantize(int elem, const QuantizeArgs& a, hipStream_t s) {
   SHINE_BY_ELEM(elem, quantize_by_width<T>(a, s));
-  return hipGetLastError();
 }
 
 namespace {
@@ -1759,131 +1769,122 @@ Ranges ranges_of(uint64_t blocks, uint32_t query_blocks, uint32_t want) {
 }  // namespace
 
 template <class T, class E>
-void scores_of_rows(const ScoresArgs& a, hipStream_t s) {
+hipError_t scores_of_rows(const ScoresArgs& a, hipStream_t s) {
   const Ranges r = ranges_of((a.n + 31) / 32, 1, 1024);
   switch (a.pitch / 64) {
-    case 1: hipLaunchKernelGGL((scores_stream_kernel<T, 1, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-    case 2: hipLaunchKernelGGL((scores_stream_kernel<T, 2, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-    case 3: hipLaunchKernelGGL((scores_stream_kernel<T, 3, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-    default: hipLaunchKernelGGL((scores_stream_kernel<T, 4, 1, E>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
+    case 1: return launch(scores_stream_kernel<T, 1, 1, E>, dim3(r.grid), s, a, r.per);
+    case 2: return launch(scores_stream_kernel<T, 2, 1, E>, dim3(r.grid), s, a, r.per);
+    case 3: return launch(scores_stream_kernel<T, 3, 1, E>, dim3(r.grid), s, a, r.per);
+    default: return launch(scores_stream_kernel<T, 4, 1, E>, dim3(r.grid), s, a, r.per);
   }
 }
 
 template <class T>
 hipError_t scores_of(int elem, const ScoresArgs& a, hipStream_t s) {
   switch (elem) {
-    case kF32: scores_of_rows<T, float>(a, s); break;
-    case kF16: scores_of_rows<T, __half>(a, s); break;
-    case kBF16: scores_of_rows<T, __bf16>(a, s); break;
+    case kF32: return scores_of_rows<T, float>(a, s);
+    case kF16: return scores_of_rows<T, __half>(a, s);
+    case kBF16: return scores_of_rows<T, __bf16>(a, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_scores_of_rows(int elem, int out_elem, const ScoresArgs& a, hipStream_t s) {
-  SHINE_BY_ELEM(out_elem, return scores_of<T>(elem, a, s));
-  return hipErrorInvalidValue;
+  SHINE_BY_ELEM(out_elem, scores_of<T>(elem, a, s));
 }
 
 template <class T, int KC>
-void scores_in_lines_of(const ScoresArgs& a, hipStream_t s) {
+hipError_t scores_in_lines_of(const ScoresArgs& a, hipStream_t s) {
   constexpr int QT = 4;
   constexpr uint32_t kLine = 128 / sizeof(T);
   const uint32_t qb = (a.nq + QT * 16 - 1) / (QT * 16);
   const Ranges r = ranges_of((a.n + kLine - 1) / kLine, qb, 512);
   constexpr int P = sizeof(T) == 4 && KC <= 2 ? 2 : 1;
   const uint64_t per = (r.per + 4 * P - 1) / (4 * P) * P;
-  hipLaunchKernelGGL((scores_lines_kernel<T, KC, QT, P>), dim3(r.grid), dim3(256), 0, s, a, qb, per);
-}
-template <class T>
-void scores_in_lines(const ScoresArgs& a, hipStream_t s) {
-  if (a.pitch <= 64) return scores_in_lines_of<T, 1>(a, s);
-  if (a.pitch <= 128) return scores_in_lines_of<T, 2>(a, s);
-  if constexpr (sizeof(T) == 4) {
-    if (a.pitch <= 192) return scores_in_lines_of<T, 3>(a, s);
-    scores_in_lines_of<T, 4>(a, s);
-  }
+  return launch(scores_lines_kernel<T, KC, QT, P>, dim3(r.grid), s, a, qb, per);
 }
 
-hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
+template <class T>
+hipError_t scores_of_codes(const ScoresArgs& a, hipStream_t s) {
   // Up to 32 queries: streams (32 x 1M x 128: 51 us, in lines 60).  More: lines for rows of 128 codes, and with f32 scores of
   // 256 (1024 x 100,003 x 200: 128 us, in tiles 170); 16-bit scores of wider rows than 128 go in tiles (1024 x 100,000 x 200:
   // 68 us, in lines 119).
   if (a.nq <= 32 && a.pitch <= kStreamPitch) {
     const Ranges r = ranges_of((a.n + 31) / 32, 1, 2048);
-    SHINE_BY_ELEM(out_elem, switch (a.pitch / 64) {
-      case 1: hipLaunchKernelGGL((scores_stream_kernel<T, 1, 2, void>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-      case 2: hipLaunchKernelGGL((scores_stream_kernel<T, 2, 2, void>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-      case 3: hipLaunchKernelGGL((scores_stream_kernel<T, 3, 2, void>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-      default: hipLaunchKernelGGL((scores_stream_kernel<T, 4, 2, void>), dim3(r.grid), dim3(256), 0, s, a, r.per); break;
-    });
-    return hipGetLastError();
+    switch (a.pitch / 64) {
+      case 1: return launch(scores_stream_kernel<T, 1, 2, void>, dim3(r.grid), s, a, r.per);
+      case 2: return launch(scores_stream_kernel<T, 2, 2, void>, dim3(r.grid), s, a, r.per);
+      case 3: return launch(scores_stream_kernel<T, 3, 2, void>, dim3(r.grid), s, a, r.per);
+      default: return launch(scores_stream_kernel<T, 4, 2, void>, dim3(r.grid), s, a, r.per);
+    }
   }
-  if (a.nq > 32 && a.pitch <= (out_elem == kF32 ? kStreamPitch : 128)) {
-    SHINE_BY_ELEM(out_elem, scores_in_lines<T>(a, s));
-    return hipGetLastError();
+  if (a.nq > 32) {
+    if (a.pitch <= 64) return scores_in_lines_of<T, 1>(a, s);
+    if (a.pitch <= 128) return scores_in_lines_of<T, 2>(a, s);
+    if constexpr (sizeof(T) == 4) {
+      if (a.pitch <= 192) return scores_in_lines_of<T, 3>(a, s);
+      if (a.pitch <= kStreamPitch) return scores_in_lines_of<T, 4>(a, s);
+    }
   }
-  const uint32_t few = static_cast<uint32_t>((a.n + 127) / 128), qb = (a.nq + kTileQueries - 1) / kTileQueries,
-                 rb = static_cast<uint32_t>((a.n + kTileRecords - 1) / kTileRecords);
   // Up to 16 queries: 8 x 100,000 x 768: 21.7 us, in tiles 24.0; 16 x 400,000 x 768: 77.6 and 83.0 (32 in two such tiles a wave:
   // 30.4 us for 100,000, in tiles 25.3).
-  SHINE_BY_ELEM(out_elem, if (a.nq <= 16) hipLaunchKernelGGL(scores_few_kernel<T>, dim3(few), dim3(256), 0, s, a);
-                else hipLaunchKernelGGL(scores_wide_kernel<T>, dim3((rb + 7) / 8 * 8 * qb), dim3(256), 0, s, a, qb, rb));
-  return hipGetLastError();
+  if (a.nq <= 16) return launch(scores_few_kernel<T>, dim3(static_cast<uint32_t>((a.n + 127) / 128)), s, a);
+  const uint32_t qb = (a.nq + kTileQueries - 1) / kTileQueries, rb = static_cast<uint32_t>((a.n + kTileRecords - 1) / kTileRecords);
+  return launch(scores_wide_kernel<T>, dim3((rb + 7) / 8 * 8 * qb), s, a, qb, rb);
+}
+
+hipError_t launch_scores(int out_elem, const ScoresArgs& a, hipStream_t s) {
+  SHINE_BY_ELEM(out_elem, scores_of_codes<T>(a, s));
 }
 
 namespace {
 constexpr uint32_t kPassGroups = 512;  // two workgroups a CU
 
 template <int KC, int QT>
-void sample_with(const PassArgs& a, hipStream_t s) {
+hipError_t sample_with(const PassArgs& a, hipStream_t s) {
   const uint32_t qb = (a.nq + QT * 32 - 1) / (QT * 32);
   const Ranges r = ranges_of(a.blocks, qb, kPassGroups);
-  hipLaunchKernelGGL((sample_kernel<KC, QT>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+  return launch(sample_kernel<KC, QT>, dim3(r.grid), s, a, qb, r.per);
 }
 template <int KC, int QT>
-void pass_with(const PassArgs& a, hipStream_t s) {
+hipError_t pass_with(const PassArgs& a, hipStream_t s) {
   const uint32_t qb = (a.nq + QT * 32 - 1) / (QT * 32);
   const Ranges r = ranges_of(a.blocks, qb, kPassGroups);
-  if (a.allow && a.allow_ld) hipLaunchKernelGGL((pass_kernel<KC, QT, true>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
-  else hipLaunchKernelGGL((pass_kernel<KC, QT, false>), dim3(r.grid), dim3(256), 0, s, a, qb, r.per);
+  if (a.allow && a.allow_ld) return launch(pass_kernel<KC, QT, true>, dim3(r.grid), s, a, qb, r.per);
+  return launch(pass_kernel<KC, QT, false>, dim3(r.grid), s, a, qb, r.per);
 }
 }  // namespace
 
 hipError_t launch_sample(const PassArgs& a, hipStream_t s) {
   const bool few = a.nq <= 32;
   switch (a.pitch / 64) {
-    case 1: few ? sample_with<1, 1>(a, s) : sample_with<1, 4>(a, s); break;
-    case 2: few ? sample_with<2, 1>(a, s) : sample_with<2, 4>(a, s); break;
-    case 3: few ? sample_with<3, 1>(a, s) : sample_with<3, 2>(a, s); break;
-    case 4: few ? sample_with<4, 1>(a, s) : sample_with<4, 2>(a, s); break;
+    case 1: return few ? sample_with<1, 1>(a, s) : sample_with<1, 4>(a, s);
+    case 2: return few ? sample_with<2, 1>(a, s) : sample_with<2, 4>(a, s);
+    case 3: return few ? sample_with<3, 1>(a, s) : sample_with<3, 2>(a, s);
+    case 4: return few ? sample_with<4, 1>(a, s) : sample_with<4, 2>(a, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_pass(const PassArgs& a, hipStream_t s) {
   const bool few = a.nq <= 32;  // 32 x 1M x 128: 59 us a call, 63 with room for 128
   switch (a.pitch / 64) {
-    case 1: few ? pass_with<1, 1>(a, s) : pass_with<1, 4>(a, s); break;
-    case 2: few ? pass_with<2, 1>(a, s) : pass_with<2, 4>(a, s); break;
-    case 3: few ? pass_with<3, 1>(a, s) : pass_with<3, 2>(a, s); break;
-    case 4: few ? pass_with<4, 1>(a, s) : pass_with<4, 2>(a, s); break;
+    case 1: return few ? pass_with<1, 1>(a, s) : pass_with<1, 4>(a, s);
+    case 2: return few ? pass_with<2, 1>(a, s) : pass_with<2, 4>(a, s);
+    case 3: return few ? pass_with<3, 1>(a, s) : pass_with<3, 2>(a, s);
+    case 4: return few ? pass_with<4, 1>(a, s) : pass_with<4, 2>(a, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t s) {
   const uint64_t terms = a.terms ? (a.pass.n + 255) / 256 : 0;
-  hipLaunchKernelGGL(select_kernel, dim3(static_cast<uint32_t>(a.pass.nq + terms)), dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch(select_kernel, dim3(static_cast<uint32_t>(a.pass.nq + terms)), s, a);
 }
 
 hipError_t launch_seen(const SeenArgs& a, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(1 + (a.mask_ld + kMaskWords - 1) / kMaskWords), a.pass.nq);
-  hipLaunchKernelGGL(seen_kernel, grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch(seen_kernel, grid, s, a);
 }
 
 hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s) {
@@ -1892,9 +1893,7 @@ hipError_t launch_adjust(int elem, const AdjustArgs& a, hipStream_t s) {
   const bool wide = a.nq * ((a.n + 8191) / 8192) >= 512;
   const uint64_t tile = wide ? 8192 : 2048;
   const dim3 grid(static_cast<uint32_t>((a.n + tile - 1) / tile), a.nq);
-  SHINE_BY_ELEM(elem, if (wide) hipLaunchKernelGGL((adjust_kernel<T, 8192>), grid, dim3(256), 0, s, a);
-                else hipLaunchKernelGGL((adjust_kernel<T, 2048>), grid, dim3(256), 0, s, a));
-  return hipGetLastError();
+  SHINE_BY_ELEM(elem, launch(wide ? adjust_kernel<T, 8192> : adjust_kernel<T, 2048>, grid, s, a));
 }
 
 // Rows are cut where there are too few for the GPU (1 x 1M: 15 us, in one piece 279; 1024 x 20,000: 20.5 either way).
@@ -1906,13 +1905,11 @@ uint32_t topk_slices(uint32_t nq, uint64_t n) {
 
 hipError_t launch_topk(int elem, bool keys_only, const TopkArgs& a, hipStream_t s) {
   const bool to_keys = keys_only || a.slices > 1;
-  SHINE_BY_ELEM(elem, hipLaunchKernelGGL(topk_kernel<T>, dim3(a.slices, a.nq), dim3(256), 0, s, a, to_keys));
-  return hipGetLastError();
+  SHINE_BY_ELEM(elem, launch(topk_kernel<T>, dim3(a.slices, a.nq), s, a, to_keys));
 }
 
 hipError_t launch_merge(int elem, const MergeArgs& a, hipStream_t s) {
-  SHINE_BY_ELEM(elem, hipLaunchKernelGGL(merge_kernel<T>, dim3(a.nq), dim3(256), 0, s, a));
-  return hipGetLastError();
+  SHINE_BY_ELEM(elem, launch(merge_kernel<T>, dim3(a.nq), s, a));
 }
 
 }  // namespace shine::flat

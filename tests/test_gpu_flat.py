@@ -1071,3 +1071,41 @@ def test_a_history_shared_by_all_rows(nq, n):
         v, i = flat.topk(want, 20)
         values, ids = flat.search(table, q, 20, seen=one, **a)
         assert torch.equal(ids, i) and torch.equal(values, v)
+
+
+def hip_runtime():
+    """the HIP runtime that this process has loaded"""
+    maps = open("/proc/self/maps").read().split()
+    return C.CDLL(next(path for path in maps if "libamdhip64.so" in path))
+
+
+def test_errors_are_reported_once_and_by_the_call_that_met_them():
+    from shine_amd import _lib as L
+    flat = F()
+    x = rows(20, 32, 1).cuda()
+    want, scale = codes64(x.cpu())
+    codes, scales = torch.empty((20, 64), dtype=torch.int8, device="cuda"), torch.empty(20, device="cuda")
+    quantize = L.lib().shine_flat_quantize
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(gpu):
+        return quantize(gpu, x.data_ptr(), 0, 20, 32, 32, codes.data_ptr(), scales.data_ptr(), None, stream)
+
+    assert call(torch.cuda.device_count()) == L.ERR_HIP  # no such device
+    assert call(0) == L.OK
+    assert call(torch.cuda.device_count()) == L.ERR_HIP
+    assert (x + 1).shape == x.shape  # nor do others meet it
+    # what another call left behind is not flat scoring's, to report or to clear
+    hip = hip_runtime()
+    table = flat.FlatTable(x, metric="l2")
+    rc = hip.hipSetDevice(torch.cuda.device_count())
+    assert rc != 0
+    try:
+        assert call(0) == L.OK
+        got = L.lib().shine_flat_topk(0, x.data_ptr(), 0, 20, 32, 32, 1, scales.data_ptr(), codes.data_ptr(), None, 0, stream)
+    finally:
+        left = hip.hipGetLastError()
+    assert got == L.OK and left == rc
+    assert call(0) == L.OK
+    assert torch.equal(codes[:, :32].cpu().double(), want) and torch.equal(scales.cpu().double(), scale)
+    assert (flat.search(table, x, 1)[1][:, 0] >= 0).all()
