@@ -24,6 +24,7 @@ from . import _lib as L
 
 MAX_K = 256
 MAX_DIM = 16384
+MAX_ROWS = 2 ** 32 - 1  # of queries or scores in a call: the C entries count them in 32 bits
 
 _torch = _current = None
 _elems = {}
@@ -71,6 +72,18 @@ def _rows(x, name: str, device=None):
     return x.data_ptr(), elem, ld, n, width
 
 
+def _scores(x):
+    """(pointer, element type, row stride, rows, width) of a score matrix."""
+    rows = _rows(x, "scores")
+    _few_enough(rows[3], "scores")
+    return rows
+
+
+def _few_enough(n: int, name: str):
+    if n > MAX_ROWS:
+        raise ValueError(f"{name} must have at most {MAX_ROWS} rows")
+
+
 def _side(x, name: str, dtype, nq: int, width: int | None, device):
     """(pointer, row stride, width) of an adjustment given for each row (nq, width), or shared (1, width) or (width,)."""
     if not isinstance(x, _torch.Tensor) or x.dtype != dtype or x.device != device:
@@ -97,7 +110,8 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
     if allow is not None:
         a.allow, a.allow_ld, _ = _side(allow, "allow", torch.int32, nq, (n + 31) // 32, device)
     if seen is not None:
-        a.seen, a.seen_ld, a.seen_n = _side(seen, "seen", torch.int32, nq, None, device)
+        a.seen, a.seen_ld, h = _side(seen, "seen", torch.int32, nq, None, device)
+        a.seen_n = min(h, 2 ** 32 - 1)  # refused by the entry, not taken modulo 2^32 here
     for name, x in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
         if x is not None:
             if seen is None:
@@ -181,6 +195,7 @@ def _queries(table, queries):
     ptr, elem, ld, nq, dim = _rows(queries, "queries", table.device)
     if dim != table.dim:
         raise ValueError(f"queries have dim {dim}, the table {table.dim}")
+    _few_enough(nq, "queries")
     return ptr, elem, ld, nq
 
 
@@ -215,7 +230,7 @@ def adjust(scores, bias=None, allow=None, seen=None, repetition=None, frequency=
     `out` may be `scores` itself.
     """
     torch = _t()
-    ptr, elem, ld, nq, n = _rows(scores, "scores")
+    ptr, elem, ld, nq, n = _scores(scores)
     a = _adjustment(nq, n, scores.device, bias, allow, seen, repetition, frequency, presence)
     if out is None:
         out = torch.empty((nq, n), dtype=scores.dtype, device=scores.device)
@@ -231,7 +246,7 @@ def topk(scores, k: int):
     """The k largest scores of every row in descending order, ties to the lower id: values (nq, k) and ids int32 (nq, k).
     -infinity and NaN are never returned: places without an answer hold id -1 and -infinity."""
     torch = _t()
-    ptr, elem, ld, nq, n = _rows(scores, "scores")
+    ptr, elem, ld, nq, n = _scores(scores)
     if not 1 <= k <= MAX_K:
         raise ValueError(f"k must be in [1, {MAX_K}]")
     values = torch.empty((nq, k), dtype=scores.dtype, device=scores.device)

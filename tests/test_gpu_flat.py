@@ -1109,3 +1109,22 @@ def test_errors_are_reported_once_and_by_the_call_that_met_them():
     assert call(0) == L.OK
     assert torch.equal(codes[:, :32].cpu().double(), want) and torch.equal(scales.cpu().double(), scale)
     assert (flat.search(table, x, 1)[1][:, 0] >= 0).all()
+
+
+def test_more_rows_or_shown_ids_than_32_bits_count_are_refused():
+    """they were taken modulo 2^32; nothing here is read or written"""
+    import shine_amd
+    flat = F()
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GB")
+    many = torch.empty((2 ** 32 + 1, 1), dtype=torch.float16, device="cuda")
+    table = flat.FlatTable(rows(5, 1, 1).cuda())
+    for call in (lambda: flat.topk(many, 1), lambda: flat.adjust(many, out=many), lambda: flat.search(table, many, 1),
+                 lambda: flat.scores(table, many)):
+        with pytest.raises(ValueError, match="at most 4294967295 rows"):
+            call()
+    del many
+    ids = torch.empty((1, 2 ** 32 + 3), dtype=torch.int32, device="cuda")
+    for call in (lambda: flat.adjust(rows(2, 10, 1).cuda(), seen=ids), lambda: flat.search(table, rows(2, 1, 1).cuda(), 1, seen=ids)):
+        with pytest.raises(shine_amd.ShineError, match="65535"):
+            call()
