@@ -12,7 +12,9 @@ namespace F = shine::flat;
 
 namespace {
 
-constexpr uint32_t kRowBlock = 32768;        // rows of one launch (the grid's second extent ends at 65,535)
+// Rows of one launch (the grid's second extent ends at 65,535).  Loops over them count in 64 bits: the number behind the last
+// block's first row may be 2^32.
+constexpr uint32_t kRowBlock = 32768;
 constexpr uint64_t kQuantizeBlock = 1 << 24;  // rows of one quantising launch (threads of a grid are a 32-bit number)
 constexpr uint64_t kAlign = 256;
 
@@ -82,7 +84,7 @@ bool tangled(const void* a, uint64_t a_ld, const void* b, uint64_t b_ld, uint64_
   return apart < n * size || a_ld * size - apart < n * size;
 }
 
-F::AdjustArgs adjust_args(const shine_flat_adjustment& a, uint32_t row) {
+F::AdjustArgs adjust_args(const shine_flat_adjustment& a, uint64_t row) {
   F::AdjustArgs r{};
   r.bias = a.bias ? a.bias + row * a.bias_ld : nullptr;
   r.bias_ld = a.bias_ld;
@@ -206,7 +208,7 @@ SearchPlan plan_search(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k, const 
   return p;
 }
 
-hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const shine_flat_adjustment* a, uint32_t q,
+hipError_t search_fused(const SearchPlan& p, const shine_flat_table& t, const shine_flat_adjustment* a, uint64_t q,
                         uint32_t m, uint32_t k, char* ws, float* values, int32_t* ids, hipStream_t s) {
   F::PassArgs pass{};
   pass.qcodes = reinterpret_cast<int8_t*>(ws + p.codes);
@@ -327,8 +329,8 @@ int shine_flat_scores(int gpu_id, const shine_flat_table* table, const void* d_q
   float* scales = reinterpret_cast<float*>(codes + aligned(rows * pitch));
   a.qcodes = codes;
   a.qscales = scales;
-  for (uint32_t q = 0; q < nq; q += kRowBlock) {
-    const uint32_t m = std::min(kRowBlock, nq - q);
+  for (uint64_t q = 0; q < nq; q += kRowBlock) {
+    const uint32_t m = static_cast<uint32_t>(std::min<uint64_t>(kRowBlock, nq - q));
     if (hipError_t e = quantize(static_cast<const char*>(d_queries) + q * ld * elem_size(elem), elem, m, table->dim, ld,
                                 codes, scales, nullptr, s); e != hipSuccess)
       return hip("flat scores", e);
@@ -351,13 +353,13 @@ int shine_flat_adjust(int gpu_id, const void* d_scores, int elem, uint32_t nq, u
     return fail("out overlaps the scores without being the same rows");
   OnDevice dev(gpu_id);
   if (dev.e != hipSuccess) return hip("flat adjust: device", dev.e);
-  for (uint32_t q = 0; q < nq; q += kRowBlock) {
+  for (uint64_t q = 0; q < nq; q += kRowBlock) {
     F::AdjustArgs a = adjust_args(*adjustment, q);
     a.scores = static_cast<const char*>(d_scores) + q * ld * elem_size(elem);
     a.out = static_cast<char*>(d_out) + q * out_ld * elem_size(elem);
     a.ld = ld;
     a.out_ld = out_ld;
-    a.nq = std::min(kRowBlock, nq - q);
+    a.nq = static_cast<uint32_t>(std::min<uint64_t>(kRowBlock, nq - q));
     a.n = n;
     if (hipError_t e = F::launch_adjust(elem, a, static_cast<hipStream_t>(stream)); e != hipSuccess) return hip("flat adjust", e);
   }
@@ -384,18 +386,18 @@ int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uin
   if (dev.e != hipSuccess) return hip("flat topk: device", dev.e);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t slices = F::topk_slices(std::min(nq, kRowBlock), n);
-  for (uint32_t q = 0; q < nq; q += kRowBlock) {
+  for (uint64_t q = 0; q < nq; q += kRowBlock) {
     F::TopkArgs a{};
     a.scores = static_cast<const char*>(d_scores) + q * ld * elem_size(elem);
     a.ld = ld;
-    a.nq = std::min(kRowBlock, nq - q);
+    a.nq = static_cast<uint32_t>(std::min<uint64_t>(kRowBlock, nq - q));
     a.k = k;
     a.n = n;
     a.slices = slices;
     a.keys = static_cast<uint64_t*>(d_workspace);
     a.key_ld = slices;
-    a.values = static_cast<char*>(d_values) + static_cast<uint64_t>(q) * k * elem_size(elem);
-    a.ids = d_ids + static_cast<uint64_t>(q) * k;
+    a.values = static_cast<char*>(d_values) + q * k * elem_size(elem);
+    a.ids = d_ids + q * k;
     if (hipError_t e = F::launch_topk(elem, false, a, s); e != hipSuccess) return hip("flat topk", e);
     if (slices > 1) {
       F::MergeArgs m{a.keys, static_cast<uint64_t>(slices) * k, a.nq, k, a.values, a.ids};
@@ -429,8 +431,8 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t pitch = F::code_pitch(table->dim);
   char* ws = static_cast<char*>(d_workspace);
-  for (uint32_t q = 0; q < nq; q += p.rows) {
-    const uint32_t m = std::min(p.rows, nq - q);
+  for (uint64_t q = 0; q < nq; q += p.rows) {
+    const uint32_t m = static_cast<uint32_t>(std::min<uint64_t>(p.rows, nq - q));
     const char* rows = static_cast<const char*>(d_queries) + q * ld * elem_size(elem);
     const bool from_rows = !p.fused && F::scores_from_rows(m, pitch);
     if (!from_rows)
@@ -438,8 +440,7 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
                                   reinterpret_cast<float*>(ws + p.scales), nullptr, s); e != hipSuccess)
         return hip("flat search", e);
     if (p.fused) {
-      if (hipError_t e = search_fused(p, *table, adjustment, q, m, k, ws, d_values + static_cast<uint64_t>(q) * k,
-                                      d_ids + static_cast<uint64_t>(q) * k, s); e != hipSuccess)
+      if (hipError_t e = search_fused(p, *table, adjustment, q, m, k, ws, d_values + q * k, d_ids + q * k, s); e != hipSuccess)
         return hip("flat search", e);
       continue;
     }
@@ -484,7 +485,7 @@ int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_q
       if (hipError_t e = F::launch_topk(F::kF32, true, t, s); e != hipSuccess) return hip("flat search", e);
     }
     F::MergeArgs g{reinterpret_cast<uint64_t*>(ws + p.keys), static_cast<uint64_t>(p.chunks) * p.slices * k, m, k,
-                   d_values + static_cast<uint64_t>(q) * k, d_ids + static_cast<uint64_t>(q) * k};
+                   d_values + q * k, d_ids + q * k};
     if (hipError_t e = F::launch_merge(F::kF32, g, s); e != hipSuccess) return hip("flat search", e);
   }
   return SHINE_OK;
