@@ -409,6 +409,8 @@ int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uin
 
 uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k,
                                      const shine_flat_adjustment* adjustment) {
+  // what shine_flat_search refuses: a plan has room for the passes over kMaxRecords records
+  if (n > F::kMaxRecords || dim == 0 || dim > F::kMaxDim || k == 0 || k > F::kMaxK) return 0;
   return plan_search(nq, n, dim, k, adjustment).total;
 }
 

@@ -498,7 +498,7 @@ int shine_flat_topk(int gpu_id, const void* d_scores, int elem, uint32_t nq, uin
                     void* d_values, int32_t* d_ids, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
 /* shine_flat_scores (f32), shine_flat_adjust (nullable) and shine_flat_topk of every query, with the same results bit for
- * bit, without the whole score matrix in memory. */
+ * bit, without the whole score matrix in memory.  The workspace's size is 0 only for sizes that the search refuses. */
 uint64_t shine_flat_search_workspace(uint32_t nq, uint64_t n, uint32_t dim, uint32_t k,
                                      const shine_flat_adjustment* adjustment);
 int shine_flat_search(int gpu_id, const shine_flat_table* table, const void* d_queries, int elem, uint32_t nq, uint64_t ld,

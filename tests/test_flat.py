@@ -155,3 +155,12 @@ def test_a_history_of_stride_0_is_shared_by_all_rows():
     a = dict(seen=P, seen_n=3, seen_ld=0)
     refused(L.lib().shine_flat_search(0, table(), P, 0, 4, 32, 10, adjustment(**a), P, P, None, 1 << 40, None), "workspace")
     refused(L.lib().shine_flat_adjust(0, P, 0, 4, 100, 100, adjustment(**a), P + 4, 100, None), "overlaps")
+
+
+def test_search_workspace_of_what_search_refuses():
+    """sizes beyond the limits have no plan: 0, and search refuses them before it asks for a workspace"""
+    f = L.lib().shine_flat_search_workspace
+    assert f(17, 1 << 30, 96, 10, None) > 0
+    for n, dim, k in (((1 << 30) + 1, 96, 10), (1 << 60, 96, 10), ((1 << 64) - 1, 96, 10), (1000, 0, 10), (1000, 16385, 10),
+                      (1000, 2 ** 32 - 1, 10), (1000, 96, 0), (1000, 96, 257)):
+        assert f(17, n, dim, k, None) == 0
