@@ -165,7 +165,12 @@ class FlatTable:
 
     metric "ip": a score is the inner product.  metric "l2": the inner product minus half the record's squared norm, so
     that larger is closer; `distances` turns such scores into squared L2 distances.
+
+    codes (n, code_pitch(dim)), scales (n,) and bias ((n,), None for "ip") may be changed in place, not replaced: the calls
+    read the memory that the table was made with.
     """
+
+    _PARTS = ("codes", "scales", "bias", "n", "dim", "metric", "device", "_c")
 
     def __init__(self, rows, metric: str = "ip"):
         if metric not in ("ip", "l2"):
@@ -175,6 +180,16 @@ class FlatTable:
         self.metric, self.device = metric, rows.device
         self._c = L.FlatTable(self.codes.data_ptr(), self.scales.data_ptr(),
                               self.bias.data_ptr() if metric == "l2" else None, self.n, self.dim, 0)
+
+    def __setattr__(self, name, value):
+        if name in self._PARTS and self.__dict__.get(name, value) is not value:  # `table.bias += x` gives the same one back
+            raise AttributeError(f"a table's {name} cannot be replaced")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name):
+        if name in self._PARTS:
+            raise AttributeError(f"a table's {name} cannot be taken away")
+        super().__delattr__(name)
 
     def distances(self, values, queries):
         """Squared L2 distances of the scores `values` (nq, ...) of an "l2" table: max(|q|^2 - 2 value, 0), between the rows

@@ -164,3 +164,22 @@ def test_search_workspace_of_what_search_refuses():
     for n, dim, k in (((1 << 30) + 1, 96, 10), (1 << 60, 96, 10), ((1 << 64) - 1, 96, 10), (1000, 0, 10), (1000, 16385, 10),
                       (1000, 2 ** 32 - 1, 10), (1000, 96, 0), (1000, 96, 257)):
         assert f(17, n, dim, k, None) == 0
+
+
+def test_a_tables_parts_stay():
+    """the C table names their memory: replacing one would let calls read what is no longer held"""
+    t = flat.FlatTable.__new__(flat.FlatTable)
+    parts = dict(codes=torch.zeros((3, 64), dtype=torch.int8), scales=torch.ones(3), bias=torch.zeros(3), n=3, dim=2, metric="l2",
+                 device=torch.device("cpu"), _c=None)
+    for name, part in parts.items():
+        setattr(t, name, part)
+    for name, part in parts.items():
+        with pytest.raises(AttributeError, match="replaced"):
+            setattr(t, name, part.clone() if isinstance(part, torch.Tensor) else object())
+        with pytest.raises(AttributeError, match="taken away"):
+            delattr(t, name)
+        assert getattr(t, name) is part
+    t.bias += 1  # in place
+    t.name = "a table's own name"
+    del t.name
+    assert t.bias.tolist() == [1, 1, 1]
