@@ -42,8 +42,8 @@ def _t():
     return _torch
 
 
-def _no_gradient(x, name: str):
-    if x.requires_grad and _torch.is_grad_enabled():
+def _learned(name: str):
+    if _torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: flat scoring has none")
 
 
@@ -60,7 +60,8 @@ def _rows(x, name: str, device=None):
         raise ValueError(f"{name} must be on a GPU")
     if device is not None and index != device.index:
         raise ValueError(f"{name} is on {x.device}, not on {device}")
-    _no_gradient(x, name)
+    if x.requires_grad:
+        _learned(name)
     n, width = shape
     ld = width
     if not x.is_contiguous():
@@ -72,23 +73,14 @@ def _rows(x, name: str, device=None):
     return x.data_ptr(), elem, ld, n, width
 
 
-def _scores(x):
-    """(pointer, element type, row stride, rows, width) of a score matrix."""
-    rows = _rows(x, "scores")
-    _few_enough(rows[3], "scores")
-    return rows
-
-
-def _few_enough(n: int, name: str):
-    if n > MAX_ROWS:
-        raise ValueError(f"{name} must have at most {MAX_ROWS} rows")
+def _too_many(name: str):
+    raise ValueError(f"{name} must have at most {MAX_ROWS} rows")
 
 
 def _side(x, name: str, dtype, nq: int, width: int | None, device):
     """(pointer, row stride, width) of an adjustment given for each row (nq, width), or shared (1, width) or (width,)."""
     if not isinstance(x, _torch.Tensor) or x.dtype != dtype or x.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor on {device}")
-    _no_gradient(x, name)
     shape = x.shape
     n, w = (1, *shape) if len(shape) == 1 else shape if len(shape) == 2 else (-1, 0)
     if n != 1 and n != nq or n < 0 or (width is not None and w != width):
@@ -107,11 +99,13 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
     a = L.FlatAdjustment()
     if bias is not None:
         a.bias, a.bias_ld, _ = _side(bias, "bias", torch.float32, nq, n, device)
+        if bias.requires_grad:
+            _learned("bias")
     if allow is not None:
         a.allow, a.allow_ld, _ = _side(allow, "allow", torch.int32, nq, (n + 31) // 32, device)
     if seen is not None:
         a.seen, a.seen_ld, h = _side(seen, "seen", torch.int32, nq, None, device)
-        a.seen_n = min(h, 2 ** 32 - 1)  # refused by the entry, not taken modulo 2^32 here
+        a.seen_n = h if h < 2 ** 32 else 2 ** 32 - 1  # too many are refused by the entry, not taken modulo 2^32 here
     for name, x in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
         if x is not None:
             if seen is None:
@@ -119,7 +113,8 @@ def _adjustment(nq, n, device, bias, allow, seen, repetition, frequency, presenc
             if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != device or \
                     x.shape != (nq,) or not x.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous float32 tensor of {nq} numbers on {device}")
-            _no_gradient(x, name)
+            if x.requires_grad:
+                _learned(name)
             setattr(a, name, x.data_ptr())
     return a
 
@@ -210,7 +205,8 @@ def _queries(table, queries):
     ptr, elem, ld, nq, dim = _rows(queries, "queries", table.device)
     if dim != table.dim:
         raise ValueError(f"queries have dim {dim}, the table {table.dim}")
-    _few_enough(nq, "queries")
+    if nq > MAX_ROWS:
+        _too_many("queries")
     return ptr, elem, ld, nq
 
 
@@ -245,7 +241,9 @@ def adjust(scores, bias=None, allow=None, seen=None, repetition=None, frequency=
     `out` may be `scores` itself.
     """
     torch = _t()
-    ptr, elem, ld, nq, n = _scores(scores)
+    ptr, elem, ld, nq, n = _rows(scores, "scores")
+    if nq > MAX_ROWS:
+        _too_many("scores")
     a = _adjustment(nq, n, scores.device, bias, allow, seen, repetition, frequency, presence)
     if out is None:
         out = torch.empty((nq, n), dtype=scores.dtype, device=scores.device)
@@ -261,7 +259,9 @@ def topk(scores, k: int):
     """The k largest scores of every row in descending order, ties to the lower id: values (nq, k) and ids int32 (nq, k).
     -infinity and NaN are never returned: places without an answer hold id -1 and -infinity."""
     torch = _t()
-    ptr, elem, ld, nq, n = _scores(scores)
+    ptr, elem, ld, nq, n = _rows(scores, "scores")
+    if nq > MAX_ROWS:
+        _too_many("scores")
     if not 1 <= k <= MAX_K:
         raise ValueError(f"k must be in [1, {MAX_K}]")
     values = torch.empty((nq, k), dtype=scores.dtype, device=scores.device)
