@@ -252,7 +252,7 @@ __device__ inline void sums(const Block<KC>& b, const v4i (&q)[KC], const v4i& s
 }
 
 // Workgroups of one record range and all query blocks run on one XCD (workgroup b runs on XCD b % 8), so that its L2
-// serves the range to all of them.  False: nothing to do.
+// serves the range to all of them.
 struct Place {
   uint32_t query_block, range;
 };
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(ScoresArgs a, uint64
 // for their codes, put that off (100 us a call against 106).
 //
 // 1024 x 100,003 x 96, kernel and quantising: f32 166 -> 100 us (with lines' parts written 119), bf16 into four buffers by turns
-// 97 -> 77 (into one, which the caches half hold, 77 -> 60); rows of 100,000: 114 -> 100, 74 -> 69 (47 -> 55).  128 queries a wave:
+// 97 -> 78 (into one, which the caches half hold, 77 -> 58); rows of 100,000: 114 -> 102, 74 -> 72 (47 -> 54).  128 queries a wave:
 // 130; 32, with four waves a SIMD: 125.  What bounds it is the writing: 4.4 TB/s, of 6.7 that a fill reaches.
 template <class T, int KC, int QT, int P>
 __global__ __launch_bounds__(256, 2) void scores_lines_kernel(ScoresArgs a, uint32_t query_blocks, uint64_t per) {
@@ -1189,7 +1189,10 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
 // The best k of all records without the score matrix.  A pass scores every stride-th block of 32 records and lists, for
 // each query, the keys from its threshold on; the k-th best key of a coarser pass (a lower bound of the k-th best of all
 // records) is the next pass's threshold, the coarsest pass stores all its scores, and the last pass is over all records.
-// A list whose room ends loses nothing but time: its row is scanned again, alone, where the answers are selected.
+// A list whose room ends loses nothing but time: its row is scanned again, alone, where the answers are selected, by one workgroup.
+// Lists run full where many records pass that are no answers: a query of scale 0, a threshold or biases too large for the margin
+// test (from 1e9 on, below), more equal scores than room.  1024 x 1M x 128, k = 10, takes 0.23 ms; with one query of zeros 8.3, with
+// 512 of them 14, with half the records at -1e9 20 (at -1e8 0.23).
 
 // The score as shine_flat_scores and then shine_flat_adjust round it; tb and ab count where the biases are given.
 __device__ inline float exact_score(float sum, float qs, float xs, const PassArgs& a, float tb, float ab) {
@@ -1806,7 +1809,7 @@ hipError_t scores_in_lines_of(const ScoresArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t scores_of_codes(const ScoresArgs& a, hipStream_t s) {
-  // Up to 32 queries: streams (32 x 1M x 128: 51 us, in lines 60).  More: lines for rows of 128 codes, and with f32 scores of
+  // Up to 32 queries: streams (32 x 1M x 128: 45 to 60 us from run to run, in lines 60).  More: lines for rows of 128 codes, and with f32 scores of
   // 256 (1024 x 100,003 x 200: 128 us, in tiles 170); 16-bit scores of wider rows than 128 go in tiles (1024 x 100,000 x 200:
   // 68 us, in lines 119).
   if (a.nq <= 32 && a.pitch <= kStreamPitch) {

@@ -1,7 +1,8 @@
 """Flat scoring: every record of a table against every query, on torch tensors (C ABI: shine_flat_*).
 
-The complement of the graph search for filters that leave it too few records, tables too small for a graph, candidate
-lists and ground truth.  Records are held as 8-bit codes with a scale each.
+The complement of the graph search for filters that leave it too few records, tables too small for a graph and candidate
+lists.  Records and queries are held as 8-bit codes with a scale each: answers are exact for the codes, not for the rows
+(of the ten best of 200,000 normal rows of 96 to 768 components, 97.5 to 98 % are found).
 
     table = FlatTable(rows, metric="l2")                 # quantised once
     values, ids = search(table, queries, 10, allow=bits) # the k best allowed records of every query

@@ -433,8 +433,8 @@ int shine_gpu_build_free(shine_gpu_build_t b);
 
 /* ----------------------------------------------------------------------------------------------------------
  * Flat scoring: every record of a table against every query, for filters that leave a graph search too few records,
- * tables too small for a graph, candidate lists and ground truth.  Records are rows of 8-bit codes with a scale each;
- * a score is an inner product of codes times both scales.  All pointers are device pointers of GPU gpu_id, calls are
+ * tables too small for a graph and candidate lists.  Records are rows of 8-bit codes with a scale each; a score is an
+ * inner product of codes times both scales: exact for the codes, near to that of the rows they were made from.  All pointers are device pointers of GPU gpu_id, calls are
  * asynchronous on `stream` (NULL: the default stream), allocate nothing and can be captured into a graph; a workspace
  * belongs to one call at a time (calls on different streams, and graphs that may run at once, take one each).  The
  * caller's current device is left as it was.  Element types: SHINE_ELEM_F32, _F16, _BF16; row strides (ld) are in
