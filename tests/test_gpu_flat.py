@@ -1128,3 +1128,16 @@ def test_more_rows_or_shown_ids_than_32_bits_count_are_refused():
     for call in (lambda: flat.adjust(rows(2, 10, 1).cuda(), seen=ids), lambda: flat.search(table, rows(2, 1, 1).cuda(), 1, seen=ids)):
         with pytest.raises(shine_amd.ShineError, match="65535"):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n,dim", [(3, 400, 96), (40, 1000, 200), (33, 500, 768)])
+def test_scores_are_near_the_products_of_the_rows_themselves(nq, n, dim, dtype):
+    """A component is within half a scale of its code's: with q^ = q + d and x^ = x + e,
+    |<q^, x^> - <q, x>| <= |q|_1 sx / 2 + |x|_1 sq / 2 + dim sq sx / 4, and three roundings of the product."""
+    x, q = rows(n, dim, 1, dtype), rows(nq, dim, 2, dtype)
+    s = F().scores(F().FlatTable(x.cuda()), q.cuda()).cpu().double()
+    x, q = x.double(), q.double()
+    sx, sq = (codes64(r)[1] for r in (x, q))
+    bound = q.abs().sum(1)[:, None] * sx / 2 + sq[:, None] * x.abs().sum(1) / 2 + dim * sq[:, None] * sx / 4
+    assert ((s - q @ x.T).abs() <= bound + 3.01 * U32 * s.abs()).all()
